@@ -25,6 +25,13 @@ cudaError_t hy_launch_qk_norm_rope(int, const void*, int, int, int, int, const i
                                    cudaStream_t);
 cudaError_t hy_launch_kv_append(int, const void*, const void*, int, int, const int32_t*, void*,
                                 int, int32_t*, cudaStream_t);
+cudaError_t hy_launch_kv_append_q4(int, const void*, long, const void*, long, int, int,
+                                   const int32_t*, void*, int, int32_t*, cudaStream_t);
+cudaError_t hy_launch_kv_read_q4(int, const void*, int, int, const int32_t*, int, void*, void*,
+                                 int32_t*, cudaStream_t);
+cudaError_t hy_launch_attn_q4_scalar(int, const void*, void*, int, int, int, const void*, int,
+                                     const int32_t*, int, const int32_t*, const int32_t*,
+                                     const int32_t*, int, float, int32_t*, cudaStream_t);
 cudaError_t hy_launch_argmax(int, const void*, long, int, int, int32_t*, cudaStream_t);
 cudaError_t hy_launch_add_rms_norm(int, void*, long, const void*, long, int, int, const void*,
                                    float, void*, long, const float*, int, long, cudaStream_t,
@@ -49,6 +56,10 @@ int cuda_result(cudaError_t e, const char* what) {
 }
 
 cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
+
+// KV heads of a 4-bit cache: far above any model, and small enough that the
+// kernels' 32-bit row counts hold at least one token.
+constexpr int HY_Q4_MAX_HEADS = 1 << 16;
 
 bool dtype_ok(int32_t dtype) { return dtype == HY_DTYPE_BF16 || dtype == HY_DTYPE_FP32; }
 
@@ -349,6 +360,42 @@ int hy_kv_append(int32_t dtype, const void* k, const void* v, int32_t num_tokens
                      "hy_kv_append");
 }
 
+int hy_kv_append_q4(int32_t dtype, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                    int32_t num_tokens, int32_t kv_heads, const int32_t* slot_mapping,
+                    void* q4_cache_layer, int32_t num_blocks, int32_t* err, void* stream) {
+  if (!dtype_ok(dtype)) return fail(HY_E_INVALID, "hy_kv_append_q4: dtype must be 0 or 1");
+  if (num_tokens == 0) return HY_OK;
+  if (!k || !v || !slot_mapping || !q4_cache_layer || num_tokens < 0 || kv_heads <= 0 ||
+      kv_heads > HY_Q4_MAX_HEADS || num_blocks <= 0)
+    return fail(HY_E_INVALID, "hy_kv_append_q4: bad argument");
+  const int64_t row = (int64_t)kv_heads * HY_HEAD_DIM;
+  if (ldk < row || ldv < row)
+    return fail(HY_E_INVALID, "hy_kv_append_q4: ldk or ldv smaller than one token's heads");
+  const int64_t vec = dtype == HY_DTYPE_BF16 ? 8 : 4;
+  if (!aligned16(k) || !aligned16(v) || !aligned16(q4_cache_layer) || ldk % vec || ldv % vec)
+    return fail(HY_E_INVALID, "hy_kv_append_q4: rows and the cache must be 16-byte aligned");
+  return cuda_result(hy_launch_kv_append_q4(dtype, k, (long)ldk, v, (long)ldv, num_tokens,
+                                            kv_heads, slot_mapping, q4_cache_layer, num_blocks,
+                                            err, as_stream(stream)),
+                     "hy_kv_append_q4");
+}
+
+int hy_kv_read_q4(int32_t dtype, const void* q4_cache_layer, int32_t num_blocks, int32_t kv_heads,
+                  const int32_t* slot_mapping, int32_t num_tokens, void* k_out, void* v_out,
+                  int32_t* err, void* stream) {
+  if (!dtype_ok(dtype)) return fail(HY_E_INVALID, "hy_kv_read_q4: dtype must be 0 or 1");
+  if (num_tokens == 0) return HY_OK;
+  if (!q4_cache_layer || !slot_mapping || !k_out || !v_out || num_tokens < 0 || kv_heads <= 0 ||
+      kv_heads > HY_Q4_MAX_HEADS || num_blocks <= 0)
+    return fail(HY_E_INVALID, "hy_kv_read_q4: bad argument");
+  if (!aligned16(q4_cache_layer) || !aligned16(k_out) || !aligned16(v_out))
+    return fail(HY_E_INVALID, "hy_kv_read_q4: the cache and the outputs must be 16-byte aligned");
+  return cuda_result(hy_launch_kv_read_q4(dtype, q4_cache_layer, num_blocks, kv_heads,
+                                          slot_mapping, num_tokens, k_out, v_out, err,
+                                          as_stream(stream)),
+                     "hy_kv_read_q4");
+}
+
 size_t hy_attention_workspace_size(int32_t max_seqs, int32_t max_tokens, int32_t kv_heads) {
   if (max_seqs <= 0 || max_tokens <= 0 || kv_heads <= 0) return 0;
   return hy_attn_workspace_bytes(hy_attn_plan_dims(max_seqs, max_tokens, kv_heads,
@@ -418,6 +465,35 @@ int hy_varlen_attention(int32_t dtype, const void* q, void* out, int32_t num_tok
                           seq_lens_k, num_seqs, scale, d, workspace, err, dev, as_stream(stream),
                           flags),
       "hy_varlen_attention(bf16)");
+}
+
+int hy_varlen_attention_q4(int32_t dtype, const void* q, void* out, int32_t num_tokens,
+                           int32_t q_heads, int32_t kv_heads, const void* kv_cache,
+                           int32_t num_layers, int32_t num_blocks, int32_t layer,
+                           const int32_t* block_tables, int32_t bt_pitch,
+                           const int32_t* seq_bt_row, const int32_t* cu_seqlens_q,
+                           const int32_t* seq_lens_k, int32_t num_seqs, float scale,
+                           int32_t max_seqs, int32_t max_tokens, void* workspace,
+                           size_t workspace_bytes, int32_t* err, void* stream) {
+  if (!dtype_ok(dtype)) return fail(HY_E_INVALID, "hy_varlen_attention_q4: dtype must be 0 or 1");
+  if (!q || !out || !kv_cache || !block_tables || !cu_seqlens_q || !seq_lens_k ||
+      num_seqs <= 0 || num_tokens < 0 || num_layers <= 0 || num_blocks <= 0 || layer < 0 ||
+      layer >= num_layers || bt_pitch <= 0)
+    return fail(HY_E_INVALID, "hy_varlen_attention_q4: bad argument");
+  if (kv_heads <= 0 || kv_heads > HY_Q4_MAX_HEADS || q_heads != HY_GROUP * kv_heads)
+    return fail(HY_E_UNSUPPORTED, "hy_varlen_attention_q4: q_heads must be 4 x kv_heads");
+  if (!(scale >= 0.0f && scale <= 1e30f))
+    return fail(HY_E_INVALID, "hy_varlen_attention_q4: scale must be finite and not negative");
+  if (!aligned16(q) || !aligned16(out) || !aligned16(kv_cache))
+    return fail(HY_E_INVALID, "hy_varlen_attention_q4: q, out and the cache must be 16-byte aligned");
+  if (num_tokens == 0) return HY_OK;
+  const uint8_t* base = static_cast<const uint8_t*>(kv_cache) +
+                        (size_t)layer * num_blocks * kv_heads * 2 * HY_Q4_TILE_BYTES;
+  return cuda_result(hy_launch_attn_q4_scalar(dtype, q, out, num_tokens, q_heads, kv_heads, base,
+                                              num_blocks, block_tables, bt_pitch, seq_bt_row,
+                                              cu_seqlens_q, seq_lens_k, num_seqs, scale, err,
+                                              as_stream(stream)),
+                     "hy_varlen_attention_q4");
 }
 
 static bool vec_aligned(const void* p, int64_t ld, int32_t dtype, int32_t n) {

@@ -7,6 +7,7 @@ word (bits ``DEV_*``).
 """
 from __future__ import annotations
 
+import contextlib
 from typing import Optional
 
 import torch
@@ -16,7 +17,10 @@ from ._lib import check
 
 DEV_BOUNDS, DEV_TIMEOUT, DEV_POOL, DEV_PLAN = 1, 2, 4, 8
 ATTN_EARLY = 1                      # hy_varlen_attention flag HY_ATTN_EARLY
+Q4_TILE_BYTES = 1152                # HY_Q4_TILE_BYTES: one (block, head, K or V) of the 4-bit cache
 DTYPES = {torch.bfloat16: 0, torch.float32: 1}
+
+_HERE = contextlib.nullcontext()
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -25,6 +29,16 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def _stream():
     return torch.cuda.current_stream().cuda_stream
+
+
+def _on(device: torch.device):
+    """Make ``device`` current for a launch (a no-op context when it already is)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Elements from token to token (a single token's stride says nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
 
 
 def _i32(t: torch.Tensor, name: str):
@@ -145,6 +159,78 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
           "hy_kv_append")
 
 
+def kv_cache_q4(layers: int, num_blocks: int, kv_heads: int, device="cuda") -> torch.Tensor:
+    """An empty 4-bit KV cache (every row reads back as zeros):
+    uint8 [layers][blocks][kv_heads][2 (K,V)][Q4_TILE_BYTES]."""
+    return torch.zeros(layers, num_blocks, kv_heads, 2, Q4_TILE_BYTES, dtype=torch.uint8,
+                       device=device)
+
+
+def _q4_layer(cache: torch.Tensor, ndim: int):
+    if cache.dtype != torch.uint8 or cache.dim() != ndim or not cache.is_contiguous() or \
+            tuple(cache.shape[-2:]) != (2, Q4_TILE_BYTES):
+        raise ValueError("the 4-bit cache must be contiguous uint8 "
+                         f"{'[layers]' * (ndim - 4)}[blocks][kv_heads][2][{Q4_TILE_BYTES}]")
+
+
+def _q4_index(t: torch.Tensor, name: str, n: int, device):
+    _i32(t, name)
+    if t.numel() != n:
+        raise ValueError(f"{name} needs one entry per token")
+    if t.device != device:
+        raise ValueError(f"{name} must be on the cache's device")
+
+
+def kv_append_q4(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
+                 kv_cache_layer: torch.Tensor, err: Optional[torch.Tensor] = None) -> None:
+    """Quantise k and v (tokens, kv_heads, 128) into one layer of a 4-bit cache
+    (``kv_cache_q4``) at ``slot_mapping``; a negative slot skips its token, and
+    the other slots of a call are distinct.  The heads of a token are contiguous;
+    the tokens may be strided (v as a part of the QKV rows)."""
+    _q4_layer(kv_cache_layer, 4)
+    NB, heads = kv_cache_layer.shape[:2]
+    T = k.shape[0]
+    for name, t in (("k", k), ("v", v)):
+        if tuple(t.shape) != (T, heads, 128) or t.dtype != k.dtype or \
+                t.device != kv_cache_layer.device:
+            raise ValueError(f"{name} must be (tokens, {heads}, 128) on the cache's device, "
+                             "k and v of one dtype")
+        if T and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != 128)):
+            raise ValueError(f"the heads of a token must be contiguous in {name}")
+    _q4_index(slot_mapping, "slot_mapping", T, k.device)
+    with _on(k.device):
+        check(_lib.load().hy_kv_append_q4(
+            _dt(k), _ptr(k), _pitch(k), _ptr(v), _pitch(v), T, heads, _ptr(slot_mapping),
+            _ptr(kv_cache_layer), NB, _ptr(err), _stream()), "hy_kv_append_q4")
+
+
+def kv_read_q4(kv_cache_layer: torch.Tensor, slot_mapping: torch.Tensor, dtype: torch.dtype,
+               k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None,
+               err: Optional[torch.Tensor] = None):
+    """(k, v), each (tokens, kv_heads, 128) of ``dtype``: what the rows at
+    ``slot_mapping`` of one layer of a 4-bit cache stand for (zeros for a negative
+    slot)."""
+    _q4_layer(kv_cache_layer, 4)
+    NB, heads = kv_cache_layer.shape[:2]
+    T, device = slot_mapping.numel(), kv_cache_layer.device
+    _q4_index(slot_mapping, "slot_mapping", T, device)
+    outs = []
+    for t in (k_out, v_out):
+        if t is None:
+            t = torch.empty(T, heads, 128, dtype=dtype, device=device)
+        elif tuple(t.shape) != (T, heads, 128) or t.dtype != dtype or t.device != device or \
+                not t.is_contiguous():
+            raise ValueError(f"outputs must be contiguous (tokens, {heads}, 128) {dtype} tensors "
+                             "on the cache's device")
+        outs.append(t)
+    k_out, v_out = outs
+    with _on(device):
+        check(_lib.load().hy_kv_read_q4(
+            _dt(k_out), _ptr(kv_cache_layer), NB, heads, _ptr(slot_mapping), T, _ptr(k_out),
+            _ptr(v_out), _ptr(err), _stream()), "hy_kv_read_q4")
+    return k_out, v_out
+
+
 def attention_workspace_size(max_seqs: int, max_tokens: int, kv_heads: int) -> int:
     return int(_lib.load().hy_attention_workspace_size(max_seqs, max_tokens, kv_heads))
 
@@ -180,6 +266,42 @@ def varlen_attention(q: torch.Tensor, out: torch.Tensor, kv_cache: torch.Tensor,
         _ptr(block_tables), block_tables.shape[1], _ptr(seq_bt_row), _ptr(cu_seqlens_q),
         _ptr(seq_lens_k), num_seqs, float(scale), max_seqs, max_tokens, _ptr(workspace),
         ws_bytes, ATTN_EARLY if early else 0, _ptr(err), _stream()), "hy_varlen_attention")
+
+
+def varlen_attention_q4(q: torch.Tensor, out: torch.Tensor, kv_cache: torch.Tensor, layer: int,
+                        block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                        seq_lens_k: torch.Tensor, num_seqs: int, max_seqs: int, max_tokens: int,
+                        workspace: Optional[torch.Tensor],
+                        seq_bt_row: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                        err: Optional[torch.Tensor] = None) -> None:
+    """``varlen_attention`` over a 4-bit cache (``kv_cache_q4``): the same plan,
+    workspace and block tables."""
+    T, q_heads, D = q.shape
+    _q4_layer(kv_cache, 5)
+    L, NB, kv_heads = kv_cache.shape[:3]
+    if D != 128 or out.shape != q.shape or out.dtype != q.dtype or not q.is_contiguous() or \
+            not out.is_contiguous():
+        raise ValueError("q and out must be contiguous (tokens, q_heads, 128) of one dtype")
+    for name, t, n in (("block_tables", block_tables, 0), ("cu_seqlens_q", cu_seqlens_q, num_seqs + 1),
+                       ("seq_lens_k", seq_lens_k, num_seqs), ("seq_bt_row", seq_bt_row, num_seqs)):
+        if t is None:
+            continue
+        _i32(t, name)
+        if t.numel() < n:
+            raise ValueError(f"{name} is too small for num_seqs")
+    if block_tables.dim() != 2 or (seq_bt_row is None and block_tables.shape[0] < num_seqs):
+        raise ValueError("block_tables must be [rows][pitch] with a row per sequence")
+    for t in (q, out, block_tables, cu_seqlens_q, seq_lens_k):
+        if t.device != kv_cache.device:
+            raise ValueError("every tensor must be on the cache's device")
+    scale = (1.0 / D ** 0.5) if scale is None else scale
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    with _on(q.device):
+        check(_lib.load().hy_varlen_attention_q4(
+            _dt(q), _ptr(q), _ptr(out), T, q_heads, kv_heads, _ptr(kv_cache), L, NB, layer,
+            _ptr(block_tables), block_tables.shape[1], _ptr(seq_bt_row), _ptr(cu_seqlens_q),
+            _ptr(seq_lens_k), num_seqs, float(scale), max_seqs, max_tokens, _ptr(workspace),
+            ws_bytes, _ptr(err), _stream()), "hy_varlen_attention_q4")
 
 
 def add_rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float,

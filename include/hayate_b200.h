@@ -17,6 +17,7 @@
  *   q, out        [tokens][q_heads][128]
  *   KV cache      [layer][block][2 (K,V)][kv_heads][16][128]
  *   block tables  [rows][bt_pitch] int32 physical block ids in position order
+ *   4-bit cache   [layer][block][kv_heads][2 (K,V)][HY_Q4_TILE_BYTES], see hy_kv_append_q4
  *   schedule      int32[4][num_seqs]: slot, start, q_len, flags (bit 0: sample)
  * dtype: 0 = bf16, 1 = fp32.  q_heads must be 4 x kv_heads; head_dim is 128; a
  * KV block holds 16 tokens.
@@ -131,6 +132,42 @@ int hy_kv_append(int32_t dtype, const void* k, const void* v, int32_t num_tokens
                  int32_t kv_heads, const int32_t* slot_mapping, void* kv_cache_layer,
                  int32_t num_blocks, int32_t* err, void* stream);
 
+/* ------------------------------------------------------- 4-bit KV cache */
+
+/* A tile of the 4-bit cache: the 16 rows (tokens) of one block, K or V, of one
+ * KV head.  Rows of 64 code bytes come first, then rows of 8 parameter bytes,
+ * four fp16: scale and minimum of dimensions 0-63, scale and minimum of
+ * dimensions 64-127.  Little-endian word i of a row's codes holds dimensions
+ * 8i..8i+7: nibble j (bits 4j..4j+3) is dimension 8i + 2j, nibble 4 + j
+ * dimension 8i + 2j + 1.  A code stands for scale * code + minimum. */
+#define HY_Q4_TILE_BYTES 1152
+
+/* Quantise k and v rows into the 4-bit cache of one layer at slot_mapping (slot
+ * < 0: skipped; past the pool: HY_DEV_BOUNDS and skipped).  k and v are
+ * [tokens][kv_heads][128] with ldk / ldv elements from token to token (v may be
+ * a part of the QKV rows); rows and the cache are 16-byte aligned, ldk and ldv
+ * a multiple of 8 (bf16) / 4 (fp32).  The slots >= 0 of one call are distinct,
+ * as hy_pack_batch makes them: a slot given twice ends with either row, or with
+ * parts of both.  For the 64 dimensions x of half a row, in fp32:
+ *   x clamped to +-32768,  minimum = fp16(min x),
+ *   scale = fp16((max x - min x) * fp32(1/15)),
+ *   code = clamp(round_half_even((x - minimum) * (1 / scale)), 0, 15),
+ * codes 0 where the scale is 0; a NaN makes its half row read back as NaN.
+ * Replaces: torch.cat of new K/V onto the cache (hayate/model/attention.py:52-54),
+ * at 144 bytes a token and KV head instead of 512. */
+int hy_kv_append_q4(int32_t dtype, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                    int32_t num_tokens, int32_t kv_heads, const int32_t* slot_mapping,
+                    void* q4_cache_layer, int32_t num_blocks, int32_t* err, void* stream);
+
+/* Read rows of one layer's 4-bit cache back: k_out and v_out
+ * [tokens][kv_heads][128] (16-byte aligned) take what the codes at slot_mapping
+ * stand for, rounded once to dtype; a slot < 0 (or past the pool, which also
+ * sets HY_DEV_BOUNDS) gives rows of zeros.  A slot may appear any number of times.
+ * No reference counterpart: the reference's cache is in the model dtype. */
+int hy_kv_read_q4(int32_t dtype, const void* q4_cache_layer, int32_t num_blocks, int32_t kv_heads,
+                  const int32_t* slot_mapping, int32_t num_tokens, void* k_out, void* v_out,
+                  int32_t* err, void* stream);
+
 /* ------------------------------------------------------------- attention */
 
 /* Bytes of attention workspace for batches of at most max_seqs sequences and
@@ -192,6 +229,24 @@ int hy_varlen_attention_noalloc(const void* q, void* out, int32_t num_tokens, in
                                 int32_t bt_pitch, const int32_t* seq_bt_row,
                                 const int32_t* cu_seqlens_q, const int32_t* seq_lens_k,
                                 int32_t num_seqs, float scale, int32_t* err, void* stream);
+
+/* hy_varlen_attention over the 4-bit cache: the same sequences, block tables,
+ * plan and workspace, with kv_cache [num_layers][num_blocks][kv_heads][2]
+ * [HY_Q4_TILE_BYTES] (16-byte aligned) and keys and values what their codes
+ * stand for; scale is finite and not negative.  Rows of q past the last sequence (cu_seqlens_q[num_seqs]) leave
+ * out as it was.  A block id outside the pool, a sequence longer than its
+ * block-table row or with fewer keys than query tokens ORs HY_DEV_BOUNDS into
+ * err; the sequence's output rows are then not meaningful.  bf16 needs the
+ * planned workspace; fp32 runs a scalar kernel for parity runs and ignores it.
+ * Replaces: as hy_varlen_attention. */
+int hy_varlen_attention_q4(int32_t dtype, const void* q, void* out, int32_t num_tokens,
+                           int32_t q_heads, int32_t kv_heads, const void* kv_cache,
+                           int32_t num_layers, int32_t num_blocks, int32_t layer,
+                           const int32_t* block_tables, int32_t bt_pitch,
+                           const int32_t* seq_bt_row, const int32_t* cu_seqlens_q,
+                           const int32_t* seq_lens_k, int32_t num_seqs, float scale,
+                           int32_t max_seqs, int32_t max_tokens, void* workspace,
+                           size_t workspace_bytes, int32_t* err, void* stream);
 
 /* ------------------------------------------------------- layer elementwise */
 
