@@ -92,7 +92,7 @@ constexpr int GROUP_MAX_BLOCKS = HY_GROUP_MAX_BLOCKS;
 constexpr int MERGE_BAR = 1;                                     // named barrier of the decode warps
 constexpr int PRE_LOAD_BAR = 2;                                  // named barrier of the two prefill
                                                                  // load warps
-constexpr int GRAB_INTS = 4;                                     // per layer: decode item, CTAs
+constexpr int GRAB_INTS = HY_GRAB_INTS;                          // per layer: decode item, CTAs
                                                                  // done, prefill item, spare
 // a split-K merge stages the partials of MERGE_CHUNK splits at a time (2 KB of O
 // and 32 B of (m, l) each, then their weights) in the merging warp's TMA ring
@@ -101,6 +101,7 @@ constexpr int MERGE_O_BYTES = MERGE_CHUNK * HY_GROUP * HY_HEAD_DIM * 4;
 constexpr int MERGE_ML_BYTES = MERGE_CHUNK * HY_GROUP * 8;
 static_assert(MERGE_O_BYTES + MERGE_ML_BYTES + MERGE_CHUNK * HY_GROUP * 4 <= DEC_WARP_BYTES,
               "merge staging must fit a decode warp's ring");
+static_assert(ATT_WARPS == HY_PLAN_WARPS, "per-CTA decode pairs have at most ATT_WARPS items");
 constexpr float NEG_INF = -INFINITY;
 // Split prefill items: a step with fewer prefill items (64 query tokens x one
 // KV head) than SMs cuts the long ones into pieces over equal key-tile ranges,
@@ -1526,6 +1527,8 @@ int device_sms(int dev) {
 }  // namespace
 
 // ------------------------------------------------------------------ host side
+int hy_attn_num_sms(int dev) { return device_sms(dev); }
+
 int hy_attn_warp_slots(int dev) { return device_sms(dev) * ATT_WARPS; }
 
 PlanDims hy_attn_plan_dims(int max_seqs, int max_tokens, int kv_heads, int dev,
@@ -1559,7 +1562,7 @@ size_t hy_attn_workspace_bytes(const PlanDims& d) {
   return off;
 }
 
-static PlanView make_view(void* ws, const PlanDims& d) {
+PlanView hy_attn_plan_view(void* ws, const PlanDims& d) {
   PlanView v;
   uint8_t* p = static_cast<uint8_t*>(ws);
   size_t off = 0;
@@ -1599,7 +1602,7 @@ cudaError_t hy_launch_attn_plan(const int32_t* cu_q, const int32_t* seq_lens_k, 
                                 int kv_heads, const PlanDims& d, void* ws, int32_t* err,
                                 int dev, cudaStream_t st) {
   return hy_launch(plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, cu_q, seq_lens_k, S,
-                   kv_heads, hy_attn_warp_slots(dev), make_view(ws, d), err);
+                   kv_heads, hy_attn_warp_slots(dev), hy_attn_plan_view(ws, d), err);
 }
 
 cudaError_t hy_launch_attn_bf16(const KvMaps& maps, const CUtensorMap& qmap, const void* cache,
@@ -1638,7 +1641,7 @@ cudaError_t hy_launch_attn_bf16(const KvMaps& maps, const CUtensorMap& qmap, con
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = err;
   a.early = (flags & HY_ATTN_EARLY) != 0;
-  const PlanView v = make_view(ws, d);
+  const PlanView v = hy_attn_plan_view(ws, d);
   const int grid = device_sms(dev) * g_ctas_per_sm[dev < 64 && dev >= 0 ? dev : 0];
   return hy_launch(attn_main_kernel, dim3(grid), dim3(ATT_THREADS), SMEM_BYTES, st, maps.kgroups,
                    maps.tiles, qmap, a, v);

@@ -65,6 +65,12 @@ int hy_attn_warp_slots(int dev);
 PlanDims hy_attn_plan_dims(int max_seqs, int max_tokens, int kv_heads, int dev,
                            bool split_prefill = true);
 size_t hy_attn_workspace_bytes(const PlanDims& d);
+PlanView hy_attn_plan_view(void* ws, const PlanDims& d);
+int hy_attn_num_sms(int dev);
+// the plan's items: decode items are dealt per warp of a CTA of this many
+// decode warps, and a per-CTA decode pair has at most as many items
+constexpr int HY_PLAN_WARPS = 8;
+constexpr int HY_GRAB_INTS = 4;   // counters per layer in PlanView::grab
 
 cudaError_t hy_launch_attn_plan(const int32_t* cu_q, const int32_t* seq_lens_k, int S,
                                 int kv_heads, const PlanDims& d, void* ws, int32_t* err,
@@ -87,3 +93,18 @@ cudaError_t hy_launch_attn_fp32(const float* q, float* out, int T, int q_heads, 
                                 const int32_t* seq_bt_row, const int32_t* cu_q,
                                 const int32_t* seq_lens_k, int S, float scale, int32_t* err,
                                 cudaStream_t st);
+
+// The 4-bit cache (attention_q4.cu); cache_layer: the layer's first tile.
+cudaError_t hy_launch_attn_q4_bf16(const void* q, void* out, int tokens, int q_heads, int kv_heads,
+                                   const void* cache_layer, int num_blocks, int layer,
+                                   const int32_t* block_tables, int bt_pitch,
+                                   const int32_t* seq_bt_row, const int32_t* cu_q,
+                                   const int32_t* seq_lens_k, int S, float scale,
+                                   const PlanDims& d, void* ws, int32_t* err, int dev,
+                                   cudaStream_t st);
+cudaError_t hy_launch_attn_q4_fp32(const void* q, void* out, int tokens, int q_heads, int kv_heads,
+                                   const void* cache_layer, int num_blocks,
+                                   const int32_t* block_tables, int bt_pitch,
+                                   const int32_t* seq_bt_row, const int32_t* cu_q,
+                                   const int32_t* seq_lens_k, int S, float scale, int32_t* err,
+                                   cudaStream_t st);

@@ -29,9 +29,6 @@ cudaError_t hy_launch_kv_append_q4(int, const void*, long, const void*, long, in
                                    const int32_t*, void*, int, int32_t*, cudaStream_t);
 cudaError_t hy_launch_kv_read_q4(int, const void*, int, int, const int32_t*, int, void*, void*,
                                  int32_t*, cudaStream_t);
-cudaError_t hy_launch_attn_q4_scalar(int, const void*, void*, int, int, int, const void*, int,
-                                     const int32_t*, int, const int32_t*, const int32_t*,
-                                     const int32_t*, int, float, int32_t*, cudaStream_t);
 cudaError_t hy_launch_argmax(int, const void*, long, int, int, int32_t*, cudaStream_t);
 cudaError_t hy_launch_add_rms_norm(int, void*, long, const void*, long, int, int, const void*,
                                    float, void*, long, const float*, int, long, cudaStream_t,
@@ -489,11 +486,25 @@ int hy_varlen_attention_q4(int32_t dtype, const void* q, void* out, int32_t num_
   if (num_tokens == 0) return HY_OK;
   const uint8_t* base = static_cast<const uint8_t*>(kv_cache) +
                         (size_t)layer * num_blocks * kv_heads * 2 * HY_Q4_TILE_BYTES;
-  return cuda_result(hy_launch_attn_q4_scalar(dtype, q, out, num_tokens, q_heads, kv_heads, base,
+  if (dtype == HY_DTYPE_FP32)
+    return cuda_result(hy_launch_attn_q4_fp32(q, out, num_tokens, q_heads, kv_heads, base,
                                               num_blocks, block_tables, bt_pitch, seq_bt_row,
                                               cu_seqlens_q, seq_lens_k, num_seqs, scale, err,
                                               as_stream(stream)),
-                     "hy_varlen_attention_q4");
+                       "hy_varlen_attention_q4(fp32)");
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
+    return fail(HY_E_INVALID, "hy_varlen_attention_q4: bf16 needs a planned, 256-byte aligned workspace");
+  if (max_seqs <= 0 || max_tokens <= 0 || num_seqs > max_seqs || num_tokens > max_tokens)
+    return fail(HY_E_INVALID, "hy_varlen_attention_q4: num_seqs or num_tokens above the workspace's");
+  const int dev = current_device();
+  const PlanDims d = hy_attn_plan_dims(max_seqs, max_tokens, kv_heads, dev);
+  if (workspace_bytes < hy_attn_workspace_bytes(d))
+    return fail(HY_E_INVALID, "hy_varlen_attention_q4: workspace too small for max_seqs/max_tokens");
+  return cuda_result(hy_launch_attn_q4_bf16(q, out, num_tokens, q_heads, kv_heads, base,
+                                            num_blocks, layer, block_tables, bt_pitch, seq_bt_row,
+                                            cu_seqlens_q, seq_lens_k, num_seqs, scale, d,
+                                            workspace, err, dev, as_stream(stream)),
+                     "hy_varlen_attention_q4(bf16)");
 }
 
 static bool vec_aligned(const void* p, int64_t ld, int32_t dtype, int32_t n) {

@@ -45,3 +45,38 @@ HY_DEVICE void q4_values(uint32_t w, float scale, float low, float (&x)[8]) {
     x[2 * j + 1] = fmaf((float)((w >> (16 + 4 * j)) & 15u), scale, low);
   }
 }
+
+// The values of a word's nibbles as fp16 pairs: x[j] = (nibble j, nibble 4 + j),
+// scaled.  s2 and m2 hold the scale and minimum of the low halves' and the high
+// halves' nibbles.  A nibble under the exponent of 1024 is the number 1024 + n (in
+// bits 0-3) or 1024 + 16 n (in bits 4-7), from which n follows exactly; the only
+// rounding is the last multiply-add's, to fp16 (2^-11 relative, an eighth of bf16's).
+HY_DEVICE uint32_t q4_lop_or(uint32_t w, uint32_t mask) {
+  uint32_t r;                                   // (w & mask) | 0x64006400
+  asm("lop3.b32 %0, %1, %2, 0x64006400, 0xea;" : "=r"(r) : "r"(w), "r"(mask));
+  return r;
+}
+HY_DEVICE void q4_expand(uint32_t w, __half2 s2, __half2 m2, uint32_t (&x)[4]) {
+  const __half2 k1024 = q4_as_half2(0xe400e400u);      // -1024
+  const __half2 k16th = q4_as_half2(0x2c002c00u);      // 1/16
+  const __half2 k64 = q4_as_half2(0xd400d400u);        // -64
+  const uint32_t w8 = w >> 8;
+  const __half2 n0 = __hadd2(q4_as_half2(q4_lop_or(w, 0x000f000fu)), k1024);
+  const __half2 n1 = __hfma2(q4_as_half2(q4_lop_or(w, 0x00f000f0u)), k16th, k64);
+  const __half2 n2 = __hadd2(q4_as_half2(q4_lop_or(w8, 0x000f000fu)), k1024);
+  const __half2 n3 = __hfma2(q4_as_half2(q4_lop_or(w8, 0x00f000f0u)), k16th, k64);
+  x[0] = q4_as_u32(__hfma2(n0, s2, m2));
+  x[1] = q4_as_u32(__hfma2(n1, s2, m2));
+  x[2] = q4_as_u32(__hfma2(n2, s2, m2));
+  x[3] = q4_as_u32(__hfma2(n3, s2, m2));
+}
+
+// A query row in fp16 is taken times 2^-e, e the exponent of its largest |element|
+// (any bf16 row then fits fp16, and what falls below fp16's normal range is 2^-14 of
+// the row's largest element); the score is multiplied by 2^e in fp32.
+HY_DEVICE void q4_query_scale(float amax, float& down, float& up) {
+  const int e = min(max((__float_as_int(amax) >> 23) & 255, 1), 253);
+  const bool finite = amax < INFINITY;            // NaN and infinities pass unscaled
+  down = finite ? __int_as_float((254 - e) << 23) : 1.0f;
+  up = finite ? __int_as_float(e << 23) : 1.0f;
+}

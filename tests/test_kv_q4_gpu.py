@@ -203,6 +203,7 @@ CASES = [
     ([64], [64]), ([65], [130]), ([130], [700]), ([200, 1, 64, 1], [200, 90, 1000, 1]),
     ([512], [1111]), ([33] * 6, [33 + 50 * i for i in range(6)]),
     ([1] * 37, [1 + 61 * i % 900 for i in range(37)]),
+    ([1, 1], [5003, 37]), ([1] * 20, [2500 - 97 * i for i in range(20)]),   # pairs split over many CTAs
 ]
 
 
@@ -238,6 +239,29 @@ def test_attention_block_table_rows(dt):
     tables = np.full((6, b.tables.shape[1]), -1, np.int32)
     tables[perm] = b.tables
     b.check(b.run(seq_bt_row=i32(perm), tables=tables))
+
+
+def test_attention_again_on_the_same_plan():
+    """Every layer of a step reuses the plan and the workspace: the counters are back at zero after
+    each call, in both layers, for split sequences and prefill chunks."""
+    b = Batch([1, 1, 130], [5003, 37, 900], 2, BF, seed=12)
+    S, T = len(b.q_lens), b.T
+    q, cache, cu, kv = b.q.to(dev), torch.from_numpy(b.cache).to(dev), i32(b.cu), i32(b.kv_lens)
+    err = torch.zeros(1, dtype=torch.int32, device=dev)
+    ws = torch.zeros(K.attention_workspace_size(S, T, 2), dtype=torch.uint8, device=dev)
+    K.attention_plan(cu, kv, S, 2, S, T, ws, err)
+    first = {}
+    for rep in range(3):
+        for layer in (0, 1):
+            out = torch.zeros_like(q)
+            K.varlen_attention_q4(q, out, cache, layer, i32(b.tables), cu, kv, S, S, T, ws, err=err)
+            b.layer = layer
+            b.check(out)
+            if layer in first:
+                # no result depends on which CTA came last
+                assert torch.equal(out, first[layer])
+            first[layer] = out
+    assert int(err.item()) == 0
 
 
 @pytest.mark.parametrize("dt", [F32, BF])
