@@ -14,8 +14,12 @@
 // maximum and sum.  The CTA merges its warps' partials in shared memory, so that a
 // sequence split over many items leaves one partial per 8 items in the workspace;
 // the CTA that finishes a (sequence, head) last joins those.
+// Prefill items (64 query tokens x one KV head, 256 score rows) run on tcgen05: four
+// warps expand key tiles to fp16 operands in shared memory, one warp per 128-row
+// sub-tile issues the products, two warpgroups run the softmax.
 // fp32 runs a scalar kernel.
 #include "attention.cuh"
+#include "attention_pieces.cuh"
 #include "q4.cuh"
 
 #include <math.h>
@@ -36,6 +40,23 @@ constexpr int PART_FLOATS = HY_GROUP * HY_HEAD_DIM + 2 * HY_GROUP;   // O [4][12
 constexpr int DEC_SMEM = NW * (RING_BYTES + PART_FLOATS * 4);
 constexpr float RESCALE_LOG2 = 8.0f;                      // see decode_range
 
+// Prefill: warps 0-3 / 4-7 softmax of sub-tile 0 / 1, 8-11 expand, 12 / 13 issue the
+// products of sub-tile 0 / 1.  Sub-tile X, row r: query head 4 g + 2 X + r / 64, token
+// t0 + r % 64.  Q is [column half][128 rows][64] per sub-tile, a K or V ring slot [column
+// half][64 keys][64], rows of 128 bytes with the 128-byte swizzle: the K-major operand
+// of S = Q K^T and the MN-major operand of P V.
+constexpr int EXP_WARP = 8, MMA_WARP = 12;
+constexpr int PS = 4;                                     // K and V ring slots
+constexpr int Q_BYTES = 128 * HY_HEAD_DIM * 2;            // Q of one sub-tile: 32 KB
+constexpr int KV_BYTES = PRE_KEYS * HY_HEAD_DIM * 2;      // K or V of one tile: 16 KB
+constexpr int K_OFF = 2 * Q_BYTES, V_OFF = K_OFF + PS * KV_BYTES;
+constexpr int PRE_SMEM = V_OFF + PS * KV_BYTES;           // 192 KB
+constexpr int SMEM_BYTES = (PRE_SMEM > DEC_SMEM ? PRE_SMEM : DEC_SMEM) + 1024;   // + alignment
+// TMEM columns: two S buffers per sub-tile, P (fp16 pairs) written over the first half
+// of its S; O at 256 + 128 X.
+constexpr uint32_t TMEM_COLS = 512, TM_O = 256;
+HY_DEVICE uint32_t tm_s(int X, uint32_t b) { return 64u * (2u * X + b); }
+
 struct Args {
   const __nv_bfloat16* q;
   __nv_bfloat16* out;
@@ -54,6 +75,17 @@ struct Shared {
   uint64_t bar[NW][NS];
   int chunk;              // the CTA's next chunk of decode items
   int last;               // bit j: this CTA finished pair j of its two open ones
+  // prefill; ring barriers complete once per use of their slot, the others once
+  // per key tile (per use of their S buffer), qfull once per item
+  uint64_t full[PS];      // K and V of a tile expanded (one arrival per expanding warp)
+  uint64_t free_[PS];     // both P V products of the slot's tile are done
+  uint64_t sfull[2][2];   // S_X[b] complete
+  uint64_t pfull[2][2];   // P_X[b] written (one arrival per softmax warp)
+  uint64_t odone[2];      // O_X += P_X V complete
+  uint64_t drain[2];      // error path: everything an issuing warp issued is complete
+  uint64_t qfull;         // Q written (one arrival per softmax warp)
+  uint32_t tmem_base;
+  int pre_item, pre_last;
 };
 
 // Row of the score matrix S^T (row r or r + 8 of the 16-key block) -> key of the
@@ -371,49 +403,388 @@ __device__ bool decode_chunk(const Args& a, const PlanView& v, int i0, int cnt, 
   return true;
 }
 
+// ------------------------------------------------------------------ prefill item
+struct PreItem {
+  int seq, g, t0, row0, nrows, prefix, kv_len, kv_end, tlo, thi, w;
+};
+HY_DEVICE PreItem pre_item_geom(const Args& a, const PlanView& v, int item) {
+  const int4 it = v.pre_sorted[item];
+  PreItem p;
+  p.seq = it.x;
+  p.g = it.y;
+  p.t0 = it.z;
+  p.w = it.w;
+  p.row0 = a.cu_q[p.seq];
+  const int q_len = a.cu_q[p.seq + 1] - p.row0;
+  p.kv_len = a.seq_lens_k[p.seq];
+  p.prefix = p.kv_len - q_len;
+  p.nrows = min(PRE_QROWS, q_len - p.t0);
+  p.kv_end = p.prefix + p.t0 + p.nrows;                   // keys its last row sees
+  pre_piece_range(p.w, (p.kv_end + PRE_KEYS - 1) / PRE_KEYS, p.tlo, p.thi);
+  return p;
+}
+
+// Expanding warps: thread t of 128 takes row t % 64 of every key tile's K (t < 64) or
+// V: its 64 code bytes and parameters from global memory, the next tile's loaded
+// ahead, to 256 bytes of fp16 in the ring.  Rows past the item's keys become zeros:
+// their scores are masked, and a zero weight times a zero adds nothing.
+struct RowCodes {
+  uint4 w[4];
+  uint32_t par[2];
+};
+HY_DEVICE int tile_block(const Args& a, const PreItem& P, const int32_t* bt, int pos) {
+  if (pos >= P.kv_end) return -1;
+  const int b = pos / HY_BLOCK;
+  const int id = b < a.bt_pitch ? __ldg(bt + b) : -1;
+  if (id >= 0 && id < a.num_blocks) return id;
+  hy_flag(a.err, HY_ERR_BOUNDS);
+  return -1;
+}
+HY_DEVICE void load_row(const Args& a, const PreItem& P, int part, int pos, int blk, RowCodes& x) {
+  if (blk < 0) {
+    x.w[0] = x.w[1] = x.w[2] = x.w[3] = make_uint4(0, 0, 0, 0);
+    x.par[0] = x.par[1] = 0u;
+    return;
+  }
+  const uint8_t* tile = a.cache + q4_tile(blk, P.g, part, a.kv_heads);
+  const uint4* src = reinterpret_cast<const uint4*>(tile + (pos % HY_BLOCK) * Q4_ROW_BYTES);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x.w[i] = src[i];
+  const uint2 p = *reinterpret_cast<const uint2*>(tile + Q4_PARAM_OFF + (pos % HY_BLOCK) * Q4_PARAM_BYTES);
+  x.par[0] = p.x;
+  x.par[1] = p.y;
+}
+HY_DEVICE void expand_row(const RowCodes& x, uint8_t* slot, int key) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const __half2 sm = q4_as_half2(x.par[half]);
+    const __half2 s2 = __low2half2(sm), m2 = __high2half2(sm);
+    uint8_t* row = slot + half * (KV_BYTES / 2) + key * 128;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint4 q = x.w[2 * half + (i >> 2)];
+      const uint32_t w = (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
+      uint32_t y[4];
+      q4_expand(w, s2, m2, y);
+      *reinterpret_cast<uint4*>(row + ((i ^ (key & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+    }
+  }
+}
+
+// One prefill item, all warps of the CTA (roles as above).  The products, barriers
+// and softmax follow attention.cu's prefill: S(t + 1) is issued while the softmax
+// works on S(t); S(t) may overwrite its buffer because P V(t - 2) was issued before it
+// by the same thread; the softmax writes P(t) over S(t) and waits for P V(t - 1) only
+// to rescale O.  c = c0 + t counts key tiles over all items of the launch.
+// Returns false if a wait ran out; the roles then drain what they issued.
+__device__ bool prefill_item(const Args& a, const PlanView& v, int item, uint8_t* payload,
+                             Shared& sh, uint32_t tmem, uint32_t& ctr, uint32_t qpar) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const PreItem P = pre_item_geom(a, v, item);
+  const int ntiles = P.thi - P.tlo;
+  const uint32_t sbase = smem_u32(payload);
+  const uint32_t c0 = ctr;
+  ctr += ntiles;
+  bool ok = true;
+
+  if (warp >= EXP_WARP && warp < MMA_WARP) {
+    const int t128 = tid - EXP_WARP * 32, part = t128 >> 6, key = t128 & 63;
+    const int32_t* bt = a.block_tables + (size_t)(a.seq_bt_row ? a.seq_bt_row[P.seq] : P.seq) * a.bt_pitch;
+    uint8_t* ring = payload + (part ? V_OFF : K_OFF);
+    RowCodes cur, nxt;
+    int pos = P.tlo * PRE_KEYS + key;
+    load_row(a, P, part, pos, tile_block(a, P, bt, pos), nxt);
+    int blk = ntiles > 1 ? tile_block(a, P, bt, pos + PRE_KEYS) : -1;
+    for (int t = 0; t < ntiles; ++t) {
+      cur = nxt;
+      pos += PRE_KEYS;
+      if (t + 1 < ntiles) load_row(a, P, part, pos, blk, nxt);
+      if (t + 2 < ntiles) blk = tile_block(a, P, bt, pos + PRE_KEYS);
+      const uint32_t c = c0 + t, slot = c % PS;
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.free_[slot], ((c / PS) & 1) ^ 1, a.err));
+      if (!ok) break;
+      expand_row(cur, ring + slot * KV_BYTES, key);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.full[slot]);
+    }
+  } else if (warp == MMA_WARP || warp == MMA_WARP + 1) {
+    const int X = warp - MMA_WARP;
+    if (lane == 0) {
+      constexpr uint32_t ID_S = tc_idesc_f16(128, PRE_KEYS, false);
+      constexpr uint32_t ID_O = tc_idesc_f16(128, HY_HEAD_DIM, true);
+      const uint64_t dQ = tc_desc_sw128(sbase + X * Q_BYTES, 16, 1024);
+      ok = mbar_wait(&sh.qfull, qpar, a.err);
+      tc_fence_after();
+      for (int t = 0; t <= ntiles && ok; ++t) {
+        if (t < ntiles) {                                 // S_X(t) = Q_X K_t^T
+          const uint32_t c = c0 + t, slot = c % PS;
+          ok = mbar_wait(&sh.full[slot], (c / PS) & 1, a.err);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t dK = tc_desc_sw128(sbase + K_OFF + slot * KV_BYTES, 16, 1024);
+#pragma unroll
+          for (int kk = 0; kk < HY_HEAD_DIM / 16; ++kk)
+            tc_mma_bf16(tmem + tm_s(X, c & 1),
+                        dQ + (uint64_t)((((kk >> 2) * (Q_BYTES / 2)) + (kk & 3) * 32) >> 4),
+                        dK + (uint64_t)((((kk >> 2) * (KV_BYTES / 2)) + (kk & 3) * 32) >> 4), ID_S,
+                        kk > 0);
+          tc_commit(&sh.sfull[X][c & 1]);
+        }
+        if (t > 0) {                                      // O_X += P_X(t - 1) V_{t-1}
+          const uint32_t c = c0 + t - 1, slot = c % PS;
+          ok = mbar_wait(&sh.pfull[X][c & 1], (c >> 1) & 1, a.err);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t dV = tc_desc_sw128(sbase + V_OFF + slot * KV_BYTES, KV_BYTES / 2, 1024);
+#pragma unroll
+          for (int kk = 0; kk < PRE_KEYS / 16; ++kk)
+            tc_mma_bf16_ta(tmem + TM_O + 128 * X, tmem + tm_s(X, c & 1) + 8 * kk,
+                           dV + (uint64_t)((kk * 2048) >> 4), ID_O, (t > 1 || kk > 0));
+          tc_commit(&sh.odone[X]);
+          tc_commit(&sh.free_[slot]);
+        }
+      }
+      if (!ok) {                                          // let every issued product finish
+        tc_commit(&sh.drain[X]);
+        mbar_wait(&sh.drain[X], 0, nullptr);
+      }
+    }
+    __syncwarp();
+  } else if (warp < EXP_WARP) {                           // softmax: thread = row = TMEM lane
+    const int X = warp >> 2, r = (warp & 3) * 32 + lane, j = r & 63;
+    const int head = P.g * HY_GROUP + 2 * X + (r >> 6);
+    const size_t at = ((size_t)(P.row0 + P.t0 + j) * a.q_heads + head) * HY_HEAD_DIM;
+    const bool real = j < P.nrows;
+    float sl2;                                            // scale to log2 units of this row
+    {                                                     // Q row r in fp16 (q4_query_scale)
+      uint4 u[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        u[i] = real ? reinterpret_cast<const uint4*>(a.q + at)[i] : make_uint4(0, 0, 0, 0);
+      float amax = 0.f, down, up;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float lo = __uint_as_float(w[k] << 16), hi = __uint_as_float(w[k] & 0xffff0000u);
+          amax = fmax3f(amax, fabsf(lo), fabsf(hi));
+        }
+      }
+      q4_query_scale(amax, down, up);
+      // not 0 (a scale of 0, a row of tiny elements): masked scores are -inf times it,
+      // and the scores it multiplies, at most 2^24, stay 0 to fp32 either way
+      sl2 = fmaxf(a.scale_log2 * up, 1e-30f);
+      uint8_t* row = payload + X * Q_BYTES + r * 128;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+        uint32_t y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          y[k] = q4_as_u32(__floats2half2_rn(__uint_as_float(w[k] << 16) * down,
+                                             __uint_as_float(w[k] & 0xffff0000u) * down));
+        *reinterpret_cast<uint4*>(row + (i >> 3) * (Q_BYTES / 2) + (((i & 7) ^ (r & 7)) << 4)) =
+            make_uint4(y[0], y[1], y[2], y[3]);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.qfull);
+    }
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tO = tmem + lane_base + TM_O + 128 * X;
+    const int lim = P.prefix + P.t0 + j;                  // last key row r may see
+    float m = NEG_INF, l = 0.f;                           // m in scaled log2 units
+    for (int t = 0; t < ntiles && ok; ++t) {
+      const uint32_t c = c0 + t;
+      const uint32_t tS = tmem + lane_base + tm_s(X, c & 1);
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.sfull[X][c & 1], (c >> 1) & 1, a.err));
+      if (!ok) break;
+      tc_fence_after();
+      float s[64];
+      tmem_ld32(tS, *reinterpret_cast<float(*)[32]>(&s[0]));
+      tmem_ld32(tS + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
+      tmem_wait_ld();
+      const int kb = (P.tlo + t) * PRE_KEYS;
+      if (kb + PRE_KEYS - 1 > P.prefix + P.t0) {          // the tile reaches the diagonal or the end
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+          if (kb + i > lim || kb + i >= P.kv_end) s[i] = NEG_INF;
+      }
+      float mxs[8];                                       // 8 independent chains
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mxs[k] = fmax3f(s[k], s[8 + k], s[16 + k]);
+#pragma unroll
+      for (int i = 24; i < 56; i += 16)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mxs[k] = fmax3f(mxs[k], s[i + k], s[i + 8 + k]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mxs[k] = fmaxf(mxs[k], s[56 + k]);
+      const float mx = sl2 * fmax3f(fmax3f(mxs[0], mxs[1], mxs[2]), fmax3f(mxs[3], mxs[4], mxs[5]),
+                                    fmaxf(mxs[6], mxs[7]));
+      const bool grow = mx > m + RESCALE_LOG2;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float mnew = grow ? mx : m;
+        const float alpha = mnew == NEG_INF ? 1.f : ex2_ftz(m - mnew);
+        l *= alpha;
+        m = mnew;
+        if (t > 0) {                                      // O holds tiles < t: wait for P V(t - 1)
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.odone[X], (c & 1) ^ 1, a.err));
+          tc_fence_after();
+#pragma unroll 1
+          for (int cc = 0; cc < 4; ++cc) {
+            float o[32];
+            tmem_ld32(tO + 32 * cc, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= alpha;
+            tmem_st32(tO + 32 * cc, o);
+          }
+          tmem_wait_st();
+        }
+      }
+      const float mneg = (m == NEG_INF) ? 0.f : -m;
+      const float2 sl2v = make_float2(sl2, sl2), mnegv = make_float2(mneg, mneg);
+      uint32_t pk[32];
+      float2 ls[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
+                      make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), sl2v, mnegv);
+        const float p0 = ex2_ftz(x.x), p1 = ex2_ftz(x.y);
+        ls[i & 3] = __fadd2_rn(ls[i & 3], make_float2(p0, p1));
+        pk[i] = q4_as_u32(__floats2half2_rn(p0, p1));
+      }
+      l += ((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y)) + ((ls[2].x + ls[2].y) + (ls[3].x + ls[3].y));
+      tmem_st32u(tS, pk);                                 // P(t) over the first 32 columns of S(t)
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.pfull[X][c & 1]);
+    }
+    if (ok) {                                             // epilogue: O_X complete
+      const uint32_t c = c0 + ntiles - 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.odone[X], c & 1, a.err));
+      tc_fence_after();
+    }
+    const bool store = ok && real;
+    __nv_bfloat16* op = a.out + at;
+    if (P.w != 0) {                                       // a piece: every softmax thread takes part
+      ok = prefill_piece_finish(v, P.w, X * 128 + r, tO, m, l, ok, store ? op : nullptr,
+                                sh.pre_last);
+    } else if (ok) {
+      const float inv = 1.f / l;
+#pragma unroll 1
+      for (int cc = 0; cc < 4; ++cc) {
+        float o[32];
+        tmem_ld32(tO + 32 * cc, o);                       // warp-collective: every lane loads
+        tmem_wait_ld();
+        if (store) {
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4)
+            *reinterpret_cast<uint4*>(op + 32 * cc + 8 * q4) =
+                make_uint4(pack_bf16(o[8 * q4 + 0] * inv, o[8 * q4 + 1] * inv),
+                           pack_bf16(o[8 * q4 + 2] * inv, o[8 * q4 + 3] * inv),
+                           pack_bf16(o[8 * q4 + 4] * inv, o[8 * q4 + 5] * inv),
+                           pack_bf16(o[8 * q4 + 6] * inv, o[8 * q4 + 7] * inv));
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  if (__syncthreads_or(!ok)) ok = false;
+  return ok;
+}
+
+// Decode items, in whichever way suits their number.  Returns false if a wait ran out.
+__device__ bool decode_items(const Args& a, const PlanView& v, int n_pre, int n_dec, int n_pairs,
+                             uint8_t* payload, Shared& sh) {
+  uint32_t phase = 0;
+  if (n_pairs > 0) {                                      // a (sequence, KV head) pair per CTA
+    if ((int)blockIdx.x >= n_pairs) return true;
+    const int seq = (int)blockIdx.x / a.kv_heads, g = (int)blockIdx.x - seq * a.kv_heads;
+    const int2 si = v.seqinfo[seq];                       // first item, items per head
+    return si.y == 0 || decode_chunk(a, v, si.x + g * si.y, si.y, payload, sh, phase);
+  }
+  const int chunks = (n_dec + CHUNK - 1) / CHUNK;
+  if (n_pre == 0 && chunks <= (int)gridDim.x) {           // one round: no counters
+    if ((int)blockIdx.x >= chunks) return true;
+    const int i0 = (int)blockIdx.x * CHUNK;
+    return decode_chunk(a, v, i0, min(CHUNK, n_dec - i0), payload, sh, phase);
+  }
+  int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
+  for (;;) {
+    if (threadIdx.x == 0) sh.chunk = atomicAdd(&grab[0], 1);
+    __syncthreads();
+    const int k = sh.chunk;
+    __syncthreads();
+    if (k >= chunks) return true;
+    if (!decode_chunk(a, v, k * CHUNK, min(CHUNK, n_dec - k * CHUNK), payload, sh, phase))
+      return false;
+  }
+}
+
 __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(Args a, PlanView v) {
   __shared__ Shared sh;
-  extern __shared__ __align__(128) uint8_t payload[];
+  extern __shared__ uint8_t dyn_smem[];
+  uint8_t* payload = dyn_smem + ((1024u - (smem_u32(dyn_smem) & 1023u)) & 1023u);
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     for (int w = 0; w < NW; ++w)
       for (int s = 0; s < NS; ++s) mbar_init(&sh.bar[w][s], 1);
+    for (int s = 0; s < PS; ++s) {
+      mbar_init(&sh.full[s], MMA_WARP - EXP_WARP);
+      mbar_init(&sh.free_[s], 2);                         // one commit per MMA warp
+    }
+    for (int x = 0; x < 2; ++x) {
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&sh.sfull[x][b], 1);
+        mbar_init(&sh.pfull[x][b], 4);
+      }
+      mbar_init(&sh.odone[x], 1);
+      mbar_init(&sh.drain[x], 1);
+    }
+    mbar_init(&sh.qfull, EXP_WARP);
     fence_mbar_init();
   }
   __syncthreads();
   hy_grid_wait();
   hy_grid_trigger();
   const uint64_t keep = l2_keep_policy();
-  const int n_dec = ld_keep(v.header + 1, keep), n_pairs = ld_keep(v.header + 4, keep);
-  uint32_t phase = 0;
-  (void)warp;
-  if (n_pairs > 0) {                                      // a (sequence, KV head) pair per CTA
-    for (int p = blockIdx.x; p < n_pairs; p += gridDim.x) {
-      const int seq = p / a.kv_heads, g = p - seq * a.kv_heads;
-      const int2 si = v.seqinfo[seq];                     // first item, items per head
-      if (si.y > 0 && !decode_chunk(a, v, si.x + g * si.y, si.y, payload, sh, phase)) return;
-    }
-    return;
-  }
-  const int chunks = (n_dec + CHUNK - 1) / CHUNK;
-  if (chunks <= (int)gridDim.x) {                         // one round: no counters
-    if ((int)blockIdx.x < chunks)
-      decode_chunk(a, v, blockIdx.x * CHUNK, min(CHUNK, n_dec - (int)blockIdx.x * CHUNK), payload,
-                   sh, phase);
-    return;
-  }
+  const int n_pre = ld_keep(v.header, keep), n_dec = ld_keep(v.header + 1, keep);
+  const int n_pairs = ld_keep(v.header + 4, keep);
   int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
   bool ok = true;
-  for (;;) {
-    if (threadIdx.x == 0) sh.chunk = ok ? atomicAdd(&grab[0], 1) : chunks;
+  if ((int)blockIdx.x < n_pre) {                          // the first n_pre CTAs take prefill items
+    if (warp == 0) {
+      tmem_alloc(&sh.tmem_base, TMEM_COLS);
+      tmem_relinquish();
+    }
+    tc_fence_before();
     __syncthreads();
-    const int k = sh.chunk;
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem_base;
+    uint32_t tile_ctr = 0;
+    for (uint32_t n = 0; ok; ++n) {
+      if (threadIdx.x == 0) sh.pre_item = atomicAdd(&grab[2], 1);
+      __syncthreads();
+      const int k = sh.pre_item;
+      __syncthreads();
+      if (k >= n_pre) break;
+      ok = prefill_item(a, v, k, payload, sh, tmem, tile_ctr, n & 1);
+    }
+    tc_fence_before();
     __syncthreads();
-    if (k >= chunks) break;
-    ok = decode_chunk(a, v, k * CHUNK, min(CHUNK, n_dec - k * CHUNK), payload, sh, phase);
+    if (warp == 0) {
+      tc_fence_after();
+      tmem_dealloc(tmem, TMEM_COLS);
+    }
   }
-  if (threadIdx.x == 0) {                                 // the last CTA out resets the counters
-    __threadfence();
+  if (ok) decode_items(a, v, n_pre, n_dec, n_pairs, payload, sh);
+  __syncthreads();
+  if ((n_pre > 0 || n_dec > CHUNK * (int)gridDim.x) && threadIdx.x == 0) {
+    __threadfence();                                      // the last CTA out resets the counters
     if (atomicAdd(&grab[1], 1) == (int)gridDim.x - 1) {
       atomicExch(&grab[0], 0);
       atomicExch(&grab[2], 0);
@@ -461,7 +832,7 @@ __global__ void __launch_bounds__(256) attn_q4_scalar_kernel(
     const uint8_t* __restrict__ cache_layer, int num_blocks,
     const int32_t* __restrict__ block_tables, int bt_pitch,
     const int32_t* __restrict__ seq_bt_row, const int32_t* __restrict__ cu_q,
-    const int32_t* __restrict__ seq_lens_k, int S, float scale, bool skip_decodes, int32_t* err) {
+    const int32_t* __restrict__ seq_lens_k, int S, float scale, int32_t* err) {
   hy_grid_wait();
   hy_grid_trigger();
   const int lane = threadIdx.x & 31;
@@ -476,7 +847,6 @@ __global__ void __launch_bounds__(256) attn_q4_scalar_kernel(
       if (cu_q[mid] <= row) lo = mid; else hi = mid;
     }
     const int seq = lo;
-    if (skip_decodes && cu_q[seq + 1] - cu_q[seq] == 1) continue;
     const int prefix = seq_lens_k[seq] - (cu_q[seq + 1] - cu_q[seq]);
     const int key_end = prefix + (row - cu_q[seq]) + 1;
     if (prefix < 0 || (long)key_end > (long)bt_pitch * HY_BLOCK) {
@@ -519,12 +889,12 @@ cudaError_t launch_scalar(const void* q, void* out, int tokens, int q_heads, int
                           const uint8_t* cache_layer, int num_blocks,
                           const int32_t* block_tables, int bt_pitch, const int32_t* seq_bt_row,
                           const int32_t* cu_q, const int32_t* seq_lens_k, int S, float scale,
-                          bool skip_decodes, int32_t* err, cudaStream_t st) {
+                          int32_t* err, cudaStream_t st) {
   const long blocks = ((long)tokens * q_heads + 7) / 8;
   return hy_launch(attn_q4_scalar_kernel<T>, dim3((int)(blocks < 148L * 32 ? blocks : 148L * 32)),
                    dim3(256), 0, st, static_cast<const T*>(q), static_cast<T*>(out), tokens,
                    q_heads, kv_heads, cache_layer, num_blocks, block_tables, bt_pitch, seq_bt_row,
-                   cu_q, seq_lens_k, S, scale, skip_decodes, err);
+                   cu_q, seq_lens_k, S, scale, err);
 }
 
 }  // namespace
@@ -537,10 +907,10 @@ cudaError_t hy_launch_attn_q4_fp32(const void* q, void* out, int tokens, int q_h
                                    cudaStream_t st) {
   return launch_scalar<float>(q, out, tokens, q_heads, kv_heads,
                               static_cast<const uint8_t*>(cache_layer), num_blocks, block_tables,
-                              bt_pitch, seq_bt_row, cu_q, seq_lens_k, S, scale, false, err, st);
+                              bt_pitch, seq_bt_row, cu_q, seq_lens_k, S, scale, err, st);
 }
 
-cudaError_t hy_launch_attn_q4_bf16(const void* q, void* out, int tokens, int q_heads, int kv_heads,
+cudaError_t hy_launch_attn_q4_bf16(const void* q, void* out, int q_heads, int kv_heads,
                                    const void* cache_layer, int num_blocks, int layer,
                                    const int32_t* block_tables, int bt_pitch,
                                    const int32_t* seq_bt_row, const int32_t* cu_q,
@@ -548,7 +918,7 @@ cudaError_t hy_launch_attn_q4_bf16(const void* q, void* out, int tokens, int q_h
                                    const PlanDims& dims, void* ws, int32_t* err, int dev,
                                    cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(attn_q4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       DEC_SMEM);
+                                       SMEM_BYTES);
   if (e != cudaSuccess) return e;
   Args a;
   a.q = static_cast<const __nv_bfloat16*>(q);
@@ -565,10 +935,6 @@ cudaError_t hy_launch_attn_q4_bf16(const void* q, void* out, int tokens, int q_h
   a.seq_lens_k = seq_lens_k;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = err;
-  e = hy_launch(attn_q4_kernel, dim3(hy_attn_num_sms(dev)), dim3(NT), DEC_SMEM, st, a,
-                hy_attn_plan_view(ws, dims));
-  if (e != cudaSuccess) return e;
-  return launch_scalar<__nv_bfloat16>(q, out, tokens, q_heads, kv_heads, a.cache, num_blocks,
-                                      block_tables, bt_pitch, seq_bt_row, cu_q, seq_lens_k, S,
-                                      scale, true, err, st);
+  return hy_launch(attn_q4_kernel, dim3(hy_attn_num_sms(dev)), dim3(NT), SMEM_BYTES, st, a,
+                   hy_attn_plan_view(ws, dims));
 }

@@ -345,7 +345,8 @@ HY_DEVICE void tc_commit(uint64_t* bar) {
                :: "r"(smem_u32(bar)) : "memory");
 }
 
-// D[tmem] (+)= A[smem] * B[smem], bf16 inputs, fp32 accumulators; one thread issues.
+// D[tmem] (+)= A[smem] * B[smem], bf16 (or fp16, by the instruction descriptor)
+// inputs, fp32 accumulators; one thread issues.
 HY_DEVICE void tc_mma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                            uint32_t accumulate) {
   asm volatile(
@@ -375,6 +376,11 @@ HY_DEVICE constexpr uint32_t tc_idesc_bf16(int M, int N, bool b_mn_major) {
          | ((b_mn_major ? 1u : 0u) << 16)            // B major-ness
          | ((uint32_t)(N >> 3) << 17)                // N / 8
          | ((uint32_t)(M >> 4) << 24);               // M / 16
+}
+
+// The same with fp16 A/B.
+HY_DEVICE constexpr uint32_t tc_idesc_f16(int M, int N, bool b_mn_major) {
+  return tc_idesc_bf16(M, N, b_mn_major) & ~((1u << 7) | (1u << 10));
 }
 
 // Shared-memory matrix descriptor for a 128-byte-swizzled canonical layout

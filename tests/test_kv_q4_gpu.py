@@ -177,7 +177,7 @@ class Batch:
             self.q[:self.T].float().numpy(), self.cache[self.layer], self.tables, self.q_lens,
             self.kv_lens, scale)
         got = out[:self.T].double().cpu().numpy()
-        assert np.isfinite(got).all()
+        assert np.isfinite(got).all(), np.argwhere(~np.isfinite(got))[:5]
         keys, vmax, reach = (a[..., None] for a in (keys, vmax, reach))
         if self.dt == F32:
             # fp32: dot products and sums of `keys` terms, each term rounded (2^-24); exp of
@@ -192,7 +192,7 @@ class Batch:
                                                       2.0 ** -23 * (keys + 300 * (reach + 1))) +
                    keys * 2.0 ** -25 * vmax + 1e-30) * 1.01
         bad = np.abs(got - want) > tol
-        assert not bad.any(), (np.argwhere(bad)[:5], np.abs(got - want)[bad][:5], tol[bad][:5])
+        assert bad.sum() == 0, (np.argwhere(bad)[:5], np.abs(got - want)[bad][:5], tol[bad][:5])
 
 
 CASES = [
@@ -221,6 +221,20 @@ def test_attention(case, heads, dt):
 def test_attention_score_ranges(qscale, scale, dt):
     b = Batch([1, 70], [500, 300], 2, dt, seed=11, qscale=qscale)
     b.check(b.run(scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+def test_attention_query_row_ranges(dt):
+    """Query rows of zeros, of the type's smallest and of very large elements beside ordinary ones."""
+    b = Batch([1, 1, 70], [90, 33, 300], 2, dt, seed=13)
+    b.q[0] = 0
+    b.q[1, 3] *= 1e-38
+    b.q[5] = 0
+    b.q[6] *= 1e-38
+    b.q[7] *= 1e-20
+    b.q[8, :, ::2] *= 1e-6            # far below its row's largest element
+    b.q[9] *= 1e5                     # past fp16's range
+    b.check(b.run())
 
 
 @pytest.mark.parametrize("dt", [F32, BF])
