@@ -15,7 +15,8 @@ log-uniform prompts, chunked prefill mixed into decodes), ``replicas``
 
 ``python -m hayate_b200.benchmark 10 [--repetitions 5] [--max-tokens 256]
 [--seed 1337] [--arrival-gap-ms 25] [--min-prompt-tokens 160]
-[--max-prompt-tokens 320] [--verbose] [--modes single,upfront,staggered]``
+[--max-prompt-tokens 320] [--verbose] [--modes single,upfront,staggered]
+[--kv-cache-dtype auto|int4]``
 """
 from __future__ import annotations
 
@@ -169,7 +170,8 @@ def bench_poisson(engine, seed, reps):
     return out
 
 
-def bench_shared_prefix(n_requests, seed, reps, prefix_caching, prefix_len=1024, max_tokens=128):
+def bench_shared_prefix(n_requests, seed, reps, prefix_caching, prefix_len=1024, max_tokens=128,
+                        kv_cache_dtype="auto"):
     """Requests sharing a ``prefix_len``-token prefix (a common system prompt) with
     unique suffixes of U[16,128] tokens, all submitted at once, on an engine with
     or without the prefix cache.  The first request runs alone beforehand, as an
@@ -179,7 +181,8 @@ def bench_shared_prefix(n_requests, seed, reps, prefix_caching, prefix_len=1024,
     prefix = torch.randint(0, workloads.VOCAB, (prefix_len,), generator=g).tolist()
     reqs = [prefix + torch.randint(0, workloads.VOCAB, (rng.randint(16, 128),),
                                    generator=g).tolist() for _ in range(n_requests)]
-    ecfg = default_engine_config(max_tokens, prefix_len + 128).with_(prefix_caching=prefix_caching)
+    ecfg = default_engine_config(max_tokens, prefix_len + 128).with_(
+        prefix_caching=prefix_caching, kv_cache_dtype=kv_cache_dtype)
     eng = Engine("Qwen/Qwen3-4B", engine_config=ecfg)
     eng.capture_graphs()
     eng.generate_text(reqs[0], max_tokens=max_tokens)
@@ -258,6 +261,8 @@ def main(argv=None):
                          "shared_prefix")
     ap.add_argument("--gpus", type=int, default=1, help="replicas mode: GPU count")
     ap.add_argument("--replica-requests", type=int, default=2048)
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "int4"],
+                    help="what the engine's KV cache holds")
     ap.add_argument("--verbose", action="store_true")
     ap.add_argument("--json", default=None, help="write the results here")
     a = ap.parse_args(argv)
@@ -272,7 +277,7 @@ def main(argv=None):
     if any(m in modes for m in ("single", "upfront", "staggered", "poisson")):
         max_prompt = max(a.max_prompt_tokens, 2048 if "poisson" in modes else 0)
         eng = Engine("Qwen/Qwen3-4B", engine_config=default_engine_config(
-            max(a.max_tokens, 512), max_prompt))
+            max(a.max_tokens, 512), max_prompt).with_(kv_cache_dtype=a.kv_cache_dtype))
         if "single" in modes:
             rows.append(("single request", bench_single(eng, reqs, a.repetitions)))
         if "upfront" in modes:
@@ -287,9 +292,11 @@ def main(argv=None):
     if "shared_prefix" in modes:
         for on in (False, True):
             rows.append((f"shared prefix, cache {'on' if on else 'off'}",
-                         bench_shared_prefix(64, a.seed, a.repetitions, on)))
+                         bench_shared_prefix(64, a.seed, a.repetitions, on,
+                                             kv_cache_dtype=a.kv_cache_dtype)))
     if "replicas" in modes:
-        kw = {"engine_config": default_engine_config(256, 4096)}
+        kw = {"engine_config": default_engine_config(256, 4096).with_(
+            kv_cache_dtype=a.kv_cache_dtype)}
         rows.append((f"replicas x{a.gpus}", bench_replicas(a.gpus, a.seed, a.replica_requests, kw)))
     summarize(rows, a.verbose)
     if a.json:

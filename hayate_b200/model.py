@@ -82,7 +82,10 @@ class Runner:
             raise ValueError("dtype must be bf16 or fp32")
         if ecfg.block_size != BLOCK_SIZE:
             raise ValueError(f"block_size must be {BLOCK_SIZE}")
+        if ecfg.kv_cache_dtype not in ("auto", "int4"):
+            raise ValueError(f"kv_cache_dtype must be auto or int4, got {ecfg.kv_cache_dtype!r}")
         self.cfg, self.ecfg, self.dtype, self.device = cfg, ecfg, dtype, device
+        self.kv_q4 = ecfg.kv_cache_dtype == "int4"
         H, I = cfg.hidden_size, cfg.intermediate_size
         dev = device
 
@@ -110,10 +113,14 @@ class Runner:
         self.final_norm = dn("norm.weight", H)
         self.rope_cos, self.rope_sin = rope_half_tables(cfg, dev)
 
-        # ---- KV cache: [layer][block][K/V][kv_head][16][128]
+        # ---- KV cache: [layer][block][K/V][kv_head][16][128], or 4-bit tiles
+        # [layer][block][kv_head][K/V][1152 bytes]
         self.num_blocks = ecfg.num_kv_blocks or self._blocks_from_memory()
-        self.kv_cache = torch.zeros(cfg.num_layers, self.num_blocks, 2, cfg.num_kv_heads,
-                                    BLOCK_SIZE, cfg.head_dim, dtype=dtype, device=dev)
+        if self.kv_q4:
+            self.kv_cache = K.kv_cache_q4(cfg.num_layers, self.num_blocks, cfg.num_kv_heads, dev)
+        else:
+            self.kv_cache = torch.zeros(cfg.num_layers, self.num_blocks, 2, cfg.num_kv_heads,
+                                        BLOCK_SIZE, cfg.head_dim, dtype=dtype, device=dev)
         # ---- request rows (slot max_reqs-1 is the graph padding row)
         self.max_reqs = ecfg.max_num_seqs + 1
         self.bt_pitch = -(-ecfg.max_model_len // BLOCK_SIZE)
@@ -137,6 +144,8 @@ class Runner:
         self.out_buf = torch.zeros(1 + S, **i32)        # [error word | next tokens]
         self.q_buf = torch.empty(T, cfg.num_heads, cfg.head_dim, dtype=dtype, device=dev)
         self.attn_buf = torch.empty_like(self.q_buf)
+        self.k_buf = torch.empty(T, cfg.num_kv_heads, cfg.head_dim, dtype=dtype, device=dev) \
+            if self.kv_q4 else None                      # rotated keys on their way to 4 bits
         self.ws = None
         self.lm_ws = None                                # fused LM head + argmax (bf16)
         if dtype == torch.bfloat16:
@@ -150,8 +159,9 @@ class Runner:
     # ------------------------------------------------------------------ memory
     def _blocks_from_memory(self) -> int:
         free, _ = torch.cuda.mem_get_info(self.device)
-        per_block = (2 * self.cfg.num_kv_heads * BLOCK_SIZE * self.cfg.head_dim *
-                     self.cfg.num_layers * torch.tensor([], dtype=self.dtype).element_size())
+        tile = K.Q4_TILE_BYTES if self.kv_q4 else (         # K or V of one block and head
+            BLOCK_SIZE * self.cfg.head_dim * torch.tensor([], dtype=self.dtype).element_size())
+        per_block = 2 * self.cfg.num_kv_heads * self.cfg.num_layers * tile
         act = 4 << 30                                    # activations + workspace headroom
         n = int((free - act) * self.ecfg.kv_cache_fraction) // per_block
         if n < 16:
@@ -244,17 +254,30 @@ class Runner:
         for l, w in enumerate(self.layers):
             last = l == nl - 1
             qkv = F.linear(h, w.w_qkv)
-            K.qk_norm_rope(qkv, Hq, Hkv, pos, w.q_norm, w.k_norm, self.rope_cos, self.rope_sin,
-                           eps, q_out=q, kv_cache_layer=self.kv_cache[l], slot_mapping=smap,
-                           num_blocks=self.num_blocks, err=err)
-            launches += 1
+            if self.kv_q4:
+                k = self.k_buf[:T]
+                K.qk_norm_rope(qkv, Hq, Hkv, pos, w.q_norm, w.k_norm, self.rope_cos,
+                               self.rope_sin, eps, q_out=q, k_out=k, err=err)
+                v = qkv[:, (Hq + Hkv) * D:].unflatten(1, (Hkv, D))
+                K.kv_append_q4(k, v, smap, self.kv_cache[l], err=err)
+                launches += 2
+            else:
+                K.qk_norm_rope(qkv, Hq, Hkv, pos, w.q_norm, w.k_norm, self.rope_cos,
+                               self.rope_sin, eps, q_out=q, kv_cache_layer=self.kv_cache[l],
+                               slot_mapping=smap, num_blocks=self.num_blocks, err=err)
+                launches += 1
             if last and n_sample == 0:
                 break                       # K/V appended; nothing samples this step
-            # from the second layer on, the plan, the block tables and the item id
-            # cache are at least two launches old: decode loads may start early
-            K.varlen_attention(q, attn, self.kv_cache, l, self.block_tables, cu_q, kv_lens, S,
-                               ecfg.max_num_seqs, ecfg.max_batched_tokens, self.ws,
-                               seq_bt_row=slots, err=err, early=l > 0)
+            if self.kv_q4:
+                K.varlen_attention_q4(q, attn, self.kv_cache, l, self.block_tables, cu_q, kv_lens,
+                                      S, ecfg.max_num_seqs, ecfg.max_batched_tokens, self.ws,
+                                      seq_bt_row=slots, err=err)
+            else:
+                # from the second layer on, the plan, the block tables and the item id
+                # cache are at least two launches old: decode loads may start early
+                K.varlen_attention(q, attn, self.kv_cache, l, self.block_tables, cu_q, kv_lens, S,
+                                   ecfg.max_num_seqs, ecfg.max_batched_tokens, self.ws,
+                                   seq_bt_row=slots, err=err, early=l > 0)
             launches += 1
             a2 = attn.view(T, Hq * D)
             nxt = self.final_norm if last else self.layers[l + 1].ln1
@@ -331,7 +354,7 @@ class Runner:
     def launches_per_step(self, n_sample: bool = True) -> int:
         """Kernels of this library one decode step (every row sampled) launches:
         pack, plan, the first RMSNorm, per layer QK-norm+RoPE, attention, two
-        add+RMSNorm and SiLU*up, then the argmax (fused with the LM head in
-        bf16) and commit."""
-        per_layer = 5
+        add+RMSNorm and SiLU*up (and the 4-bit cache's append), then the argmax
+        (fused with the LM head in bf16) and commit."""
+        per_layer = 5 + self.kv_q4
         return 2 + (self.ws is not None) + per_layer * len(self.layers) + (2 if n_sample else 0)

@@ -101,3 +101,10 @@ def test_wrappers_refuse_what_is_not_a_cache():
         K.kv_append_q4(k, k, slots, cache[0])
     with pytest.raises(ValueError, match="4-bit cache"):
         K.varlen_attention_q4(k, k, cache[0], 0, slots, slots, slots, 1, 1, 4, None)
+
+
+def test_engine_refuses_unknown_cache_types():
+    from hayate_b200.config import EngineConfig, TINY
+    from hayate_b200.model import Runner
+    with pytest.raises(ValueError, match="kv_cache_dtype"):
+        Runner(TINY, EngineConfig(kv_cache_dtype="fp8"), torch.float32, torch.device("cpu"), None, [])
