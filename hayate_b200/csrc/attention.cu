@@ -102,7 +102,6 @@ constexpr int MERGE_ML_BYTES = MERGE_CHUNK * HY_GROUP * 8;
 static_assert(MERGE_O_BYTES + MERGE_ML_BYTES + MERGE_CHUNK * HY_GROUP * 4 <= DEC_WARP_BYTES,
               "merge staging must fit a decode warp's ring");
 static_assert(ATT_WARPS * 32 == PRE_ROWS, "one softmax thread per row");
-static_assert(ATT_WARPS == HY_PLAN_WARPS, "per-CTA decode pairs have at most ATT_WARPS items");
 #ifndef HY_EXP2_POLY_EVERY
 #define HY_EXP2_POLY_EVERY 0
 #endif
@@ -185,9 +184,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
   hy_grid_trigger();
   __shared__ int ws[32];
   __shared__ int s_total, s_cpre, s_cdec, s_cpart, s_bad, s_maxblk, s_anypre, s_ptiles, s_pitems;
+  __shared__ int s_cblk;
   if (threadIdx.x == 0) {
     s_total = 0; s_cpre = 0; s_cdec = 0; s_cpart = 0; s_bad = 0; s_maxblk = 0; s_anypre = 0;
-    s_ptiles = 0; s_pitems = 0;
+    s_ptiles = 0; s_pitems = 0; s_cblk = 0;
   }
   __syncthreads();
   // Pass 1: KV blocks over all decode sequences, the longest, any prefill, and
@@ -272,11 +272,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
         npart = kv_heads * psl;
       }
     }
-    int tpre, tdec, tpart;
+    int tpre, tdec, tpart, tblk;
+    const int oblk = plan_scan(nblk, ws, tblk);
     const int opre = plan_scan(npre, ws, tpre);
     const int odec = plan_scan(ndec, ws, tdec);
     const int opart = plan_scan(npart, ws, tpart);
     const int cpre = s_cpre, cdec = s_cdec, cpart = s_cpart;
+    if (i < S && i < v.max_seqs) v.dec_blocks[i] = s_cblk + oblk;
     if (i < S && i < v.max_seqs)
       for (int g = 0; g < kv_heads; ++g) v.counters[i * kv_heads + g] = 0;
     bool wr = false;
@@ -331,7 +333,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
       }
     }
     __syncthreads();
-    if (threadIdx.x == 0) { s_cpre += tpre; s_cdec += tdec; s_cpart += tpart; }
+    if (threadIdx.x == 0) { s_cpre += tpre; s_cdec += tdec; s_cpart += tpart; s_cblk += tblk; }
     __syncthreads();
   }
   if (threadIdx.x < 64 * GRAB_INTS) v.grab[threadIdx.x] = 0;
@@ -367,6 +369,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
     v.header[2] = split;
     v.header[3] = s_bad;
     v.header[4] = group && !bad ? S * kv_heads : 0;   // per-CTA decode: its pair count
+    v.header[5] = bad ? 0 : s_cblk;
+    if (S <= v.max_seqs) v.dec_blocks[S] = s_cblk;
     if (bad) hy_flag(err, s_bad);
   }
 }
@@ -1434,6 +1438,7 @@ size_t hy_attn_workspace_bytes(const PlanDims& d) {
   off = align256(off + (size_t)d.max_pre_part * PRE_PART_F4 * sizeof(float4));
   off = align256(off + (size_t)d.max_pre_part * 256 * sizeof(float2));
   off = align256(off + (size_t)d.max_pre_part * sizeof(int));
+  off = align256(off + (size_t)(d.max_seqs + 1) * sizeof(int));
   return off;
 }
 
@@ -1466,6 +1471,8 @@ PlanView hy_attn_plan_view(void* ws, const PlanDims& d) {
   v.pre_part_ml = reinterpret_cast<float2*>(p + off);
   off = align256(off + (size_t)d.max_pre_part * 256 * sizeof(float2));
   v.pre_ctr = reinterpret_cast<int*>(p + off);
+  off = align256(off + (size_t)d.max_pre_part * sizeof(int));
+  v.dec_blocks = reinterpret_cast<int*>(p + off);
   v.max_pre = d.max_pre;
   v.max_dec = d.max_dec;
   v.max_seqs = d.max_seqs;

@@ -36,7 +36,8 @@ struct PlanDims {
 // Device view of a workspace (see attention.cu for the layout).
 struct PlanView {
   int* header;        // n_pre, n_dec, split, status, (sequence, KV head) pairs of a
-                      // per-CTA decode step (0: decode items split over all warps)
+                      // per-CTA decode step (0: decode items split over all warps),
+                      // key blocks of all decode sequences
   int4* pre;          // prefill items by sequence (plan scratch)
   int4* pre_sorted;   // the same items, most key tiles first (what the kernel runs)
   int4* dec;          // per decode item: (seq, kv head, first block, end block), then
@@ -56,6 +57,8 @@ struct PlanView {
   float2* pre_part_ml;// [max_pre_part][256] (running max in log2 units, sum) per row
   int* pre_ctr;       // [max_pre_part] finished pieces, at a split item's first slot
                       // (zeroed by the plan and by the merging piece)
+  int* dec_blocks;    // [max_seqs + 1] key blocks of the decode sequences before each
+                      // sequence (the 4-bit cache's kernel deals blocks, not items)
   int max_pre, max_dec, max_seqs, max_pre_part;
 };
 
@@ -67,9 +70,6 @@ PlanDims hy_attn_plan_dims(int max_seqs, int max_tokens, int kv_heads, int dev,
 size_t hy_attn_workspace_bytes(const PlanDims& d);
 PlanView hy_attn_plan_view(void* ws, const PlanDims& d);
 int hy_attn_num_sms(int dev);
-// the plan's items: decode items are dealt per warp of a CTA of this many
-// decode warps, and a per-CTA decode pair has at most as many items
-constexpr int HY_PLAN_WARPS = 8;
 constexpr int HY_GRAB_INTS = 4;   // counters per layer in PlanView::grab
 
 cudaError_t hy_launch_attn_plan(const int32_t* cu_q, const int32_t* seq_lens_k, int S,

@@ -72,7 +72,7 @@ HY_DEVICE bool prefill_piece_finish(const PlanView& v, int w, int rr, uint32_t t
     for (int cc = 0; cc < 4; ++cc) {
       float o[32];
       tmem_ld32(tO + 32 * cc, o);
-      tmem_wait_ld();
+      tmem_wait_ld(o);
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         __stcg(po + (cc * 8 + k) * 256,

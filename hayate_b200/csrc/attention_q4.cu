@@ -6,14 +6,11 @@
 // masks of hayate/model/qwen.py:66-106); here a key or value is what its codes
 // stand for, scale * code + minimum.
 //
-// bf16 runs the work items of hy_attention_plan (attention.cu) on the tensor cores.
-// Decode items (one query token): CTAs take 8 consecutive items at a time, two of
-// their 16 warps per item; each warp streams its blocks (2304 bytes: K and V of one
-// block and head are adjacent) through its own ring of bulk copies, expands the
-// codes to fp16 in registers, in the operand layout of mma.sync, and keeps a running
-// maximum and sum.  The CTA merges its warps' partials in shared memory, so that a
-// sequence split over many items leaves one partial per 8 items in the workspace;
-// the CTA that finishes a (sequence, head) last joins those.
+// bf16 runs on the tensor cores.  Decode sequences (one query token): the key blocks of all
+// (sequence, head) pairs, one after the other, are dealt evenly over every warp of the
+// grid; a warp streams its blocks (2304 bytes: K and V of one block and head are adjacent)
+// through a ring of bulk copies and feeds their codes to mma.sync as they are; warps of a
+// CTA merge what they share in shared memory, CTAs through the workspace.
 // Prefill items (64 query tokens x one KV head, 256 score rows) run on tcgen05: four
 // warps expand key tiles to fp16 operands in shared memory, one warp per 128-row
 // sub-tile issues the products, two warpgroups run the softmax.
@@ -28,17 +25,16 @@ namespace {
 
 constexpr int NW = 16;                                    // warps per CTA
 constexpr int NT = NW * 32;
-constexpr int CHUNK = NW / 2;                             // decode items a CTA takes at a time
-static_assert(CHUNK == HY_PLAN_WARPS, "a per-CTA decode pair's items fit one chunk");
 #ifndef HY_Q4_STAGES
 #define HY_Q4_STAGES 4
 #endif
 constexpr int NS = HY_Q4_STAGES;                          // blocks in flight per warp
 constexpr int BLK_BYTES = 2 * Q4_TILE_BYTES;              // K and V tile of one block and head
 constexpr int RING_BYTES = NS * BLK_BYTES;
-constexpr int PART_FLOATS = HY_GROUP * HY_HEAD_DIM + 2 * HY_GROUP;   // O [4][128], then (m, l) [4]
-constexpr int DEC_SMEM = NW * (RING_BYTES + PART_FLOATS * 4);
-constexpr float RESCALE_LOG2 = 8.0f;                      // see decode_range
+// a warp's partial result of one (sequence, head): O [4][128], then (m, l) [4]
+constexpr int PART_FLOATS = HY_GROUP * HY_HEAD_DIM + 2 * HY_GROUP;
+constexpr int DEC_SMEM = NW * (RING_BYTES + 2 * PART_FLOATS * 4);
+constexpr float RESCALE_LOG2 = 8.0f;                      // see decode_warp
 
 // Prefill: warps 0-3 / 4-7 softmax of sub-tile 0 / 1, 8-11 expand, 12 / 13 issue the
 // products of sub-tile 0 / 1.  Sub-tile X, row r: query head 4 g + 2 X + r / 64, token
@@ -61,7 +57,7 @@ struct Args {
   const __nv_bfloat16* q;
   __nv_bfloat16* out;
   const uint8_t* cache;   // this layer's tiles
-  int q_heads, kv_heads, num_blocks, layer;
+  int q_heads, kv_heads, num_blocks, layer, num_seqs;
   const int32_t* block_tables;
   int bt_pitch;
   const int32_t* seq_bt_row;
@@ -73,15 +69,17 @@ struct Args {
 
 struct Shared {
   uint64_t bar[NW][NS];
-  int chunk;              // the CTA's next chunk of decode items
+  int unit;               // the CTA's next unit of decode work
   int last;               // bit j: this CTA finished pair j of its two open ones
+  int part_pair[NW][2];   // each warp's partials in block order: sequence * kv_heads + head
+  int part_blocks[NW][2]; // (-1: none), and the blocks they cover
   // prefill; ring barriers complete once per use of their slot, the others once
   // per key tile (per use of their S buffer), qfull once per item
   uint64_t full[PS];      // K and V of a tile expanded (one arrival per expanding warp)
   uint64_t free_[PS];     // both P V products of the slot's tile are done
   uint64_t sfull[2][2];   // S_X[b] complete
   uint64_t pfull[2][2];   // P_X[b] written (one arrival per softmax warp)
-  uint64_t odone[2];      // O_X += P_X V complete
+  uint64_t odone[2][2];   // O_X += P_X[b] V complete
   uint64_t drain[2];      // error path: everything an issuing warp issued is complete
   uint64_t qfull;         // Q written (one arrival per softmax warp)
   uint32_t tmem_base;
@@ -97,266 +95,417 @@ HY_DEVICE int key_of(int c, int e, int h) {               // row 2 c + e + 8 h, 
   return ((c ^ e) & 1) | (e << 1) | (h << 2) | ((c >> 1) << 3);
 }
 
-// One warp: attention of query token `tok`, KV head g (4 query heads) over key
-// blocks [lo, hi) of a sequence of kv_len keys.  Scores are computed transposed,
-// S^T = K Q^T (16 keys x 8 columns, 4 of them heads), and so is the output, O^T = V^T
-// P^T: the codes then fill the 16-row operand of mma.sync, where the 4 heads
-// alone would leave three quarters of it empty, at half the instructions.
-// On return lane (r, c) = (lane / 4, lane % 4) with c < 2 holds, for heads
-// 2c + k (k = 0, 1), the unnormalised output at dimensions 8 r + i (+64) as
-// o[i / 2 + 4 (i % 2)][k (+2)], and m[k], l[k]: the running maximum (log2 units) and
-// this lane's part of the sum (l sums over the 8 lanes of equal c).
-// The maximum is only raised when a score exceeds it by more than 2^8 (weights stay
-// far below fp16's 65504), so that most blocks need no exchange between lanes.
-// Returns false if a wait ran out.
-__device__ bool decode_range(const Args& a, uint8_t* ring, uint64_t* bars, uint32_t& phase,
-                             const int32_t* bt, int tok, int g, int lo, int hi, int kv_len,
-                             float (&o)[8][4], float (&m)[2], float (&l)[2]) {
-  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int n = hi - lo;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-  m[0] = m[1] = -INFINITY;
-  l[0] = l[1] = 0.f;
-  if (n <= 0) return true;
+// A word's nibbles as fp16 pairs without any arithmetic: nibble n in bits 0-3 of a half
+// is the subnormal n 2^-24, in bits 4-7 it is 16 n 2^-24; the tensor core multiplies
+// subnormals exactly.  x[0], x[2] hold n, x[1], x[3] 16 n (pairs as in q4_expand).
+HY_DEVICE void q4_bits(uint32_t w, uint32_t (&x)[4]) {
+  const uint32_t w8 = w >> 8;
+  x[0] = w & 0x000f000fu;
+  x[1] = w & 0x00f000f0u;
+  x[2] = w8 & 0x000f000fu;
+  x[3] = w8 & 0x00f000f0u;
+}
 
-  // block ids 32 at a time, one per lane, the next 32 loaded ahead
-  auto id_at = [&](int j) {
-    const int b = lo + j;
-    return j < n && b < a.bt_pitch ? __ldg(bt + b) : -1;
-  };
-  int ids = id_at(lane), ids_next = id_at(32 + lane);
-  auto issue = [&](int j) {                               // the whole warp; j in issue order
-    if (j > 0 && (j & 31) == 0) {
-      ids = ids_next;
-      ids_next = id_at(j + 32 + lane);
+// A place in the flattened list of key blocks (sequence, head, block) of the step's
+// decode sequences, with what a load from there needs.
+struct Cursor {
+  int seq, g, b, nb;                                      // block b of nb
+  const int32_t* bt;
+  int wbase, ids;                                         // lane i holds block wbase + i's id
+};
+HY_DEVICE void cursor_sequence(const Args& a, const PlanView& v, Cursor& k) {
+  k.nb = v.dec_blocks[k.seq + 1] - v.dec_blocks[k.seq];
+  k.bt = a.block_tables + (size_t)(a.seq_bt_row ? a.seq_bt_row[k.seq] : k.seq) * a.bt_pitch;
+  k.wbase = -64;
+}
+// The place of flattened block f: the last sequence that starts at or before it, found
+// by the whole warp 32 sequences (or runs of 32^n) at a time.
+HY_DEVICE Cursor cursor_at(const Args& a, const PlanView& v, long f) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, step = 1;
+  while ((long)step * 32 < a.num_seqs) step *= 32;
+  for (; step >= 1; step >>= 5) {
+    const long i = lo + (long)lane * step;
+    const bool le = i < a.num_seqs && (long)v.dec_blocks[i] * a.kv_heads <= f;
+    lo += (31 - __clz(__ballot_sync(0xffffffffu, le) | 1u)) * step;
+  }
+  Cursor k;
+  k.seq = lo;
+  cursor_sequence(a, v, k);
+  const long in = f - (long)v.dec_blocks[lo] * a.kv_heads;
+  k.g = (int)(in / k.nb);
+  k.b = (int)(in - (long)k.g * k.nb);
+  return k;
+}
+// Step to the next (sequence, head) once all blocks of this one are passed.
+HY_DEVICE void cursor_next_pair(const Args& a, const PlanView& v, Cursor& k) {
+  k.b = 0;
+  if (++k.g < a.kv_heads) return;
+  k.g = 0;
+  do {
+    ++k.seq;
+  } while (v.dec_blocks[k.seq + 1] == v.dec_blocks[k.seq]);
+  cursor_sequence(a, v, k);
+}
+
+// One warp's running state over a (sequence, head); see decode_warp.
+struct DecState {
+  float o[8][4];          // O^T fragments, in units of 2^-24 vs (odd m-tiles 2^-20 vs)
+  float z[2][2];          // [half][k]: this lane's sum of p times V's minimum
+  float m[2], l[2];       // running maximum (log2 units), this lane's part of the sum
+  float vs, vcap;         // 2^k that V's scales are multiplied by, and the largest scale it fits
+};
+
+// One warp: key blocks [f0, f1) of the flattened list, pair by pair.
+//
+// Scores are computed transposed, S^T = K Q^T (16 keys x 8 columns, 4 of them heads),
+// and so is the output, O^T = V^T P^T: the codes then fill the 16-row operand of
+// mma.sync, where the 4 heads alone would leave three quarters of it empty.  The codes
+// enter the products as they are (q4_bits), and the parameters outside them, in fp32 or
+// folded into the weights:
+//   score = sum over halves of scale_K (code . q) + minimum_K (sum of q)
+//   out   = sum over keys of (p scale_V) code + p minimum_V
+// so that an expanded value costs 5/8 of an instruction, keys are exact, and the
+// only roundings are p scale_V's to fp16 (2^-11) and the output's.  p scale_V is kept
+// inside fp16's normal range by a power of two 2^k (vs): p is at most 2^8 (the maximum
+// is only raised when a score exceeds it by more than that, so that most blocks need
+// no exchange between lanes), scale_V 2^k at most 2^7.
+// Lane (r, c) = (lane / 4, lane % 4) with c < 2 ends with heads 2 c + k (k = 0, 1) at
+// dimensions 8 r + i and 64 + 8 r + i.  Returns false if a wait ran out.
+__device__ bool decode_warp(const Args& a, const PlanView& v, long f0, long f1, uint8_t* ring,
+                            float* part, int (&part_pair)[2], int (&part_blocks)[2],
+                            uint64_t* bars, uint32_t& ring_ctr) {
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  if (f0 >= f1) return true;
+  Cursor ld = cursor_at(a, v, f0);                        // the next block to load
+  Cursor k = ld;                                          // the pair being computed
+  int left_to_load = (int)(f1 - f0), left = left_to_load;
+  uint32_t put = ring_ctr, get = ring_ctr;                // ring slots used so far
+  auto issue = [&]() {
+    if (left_to_load <= 0) return;
+    --left_to_load;
+    if (ld.b == ld.nb) cursor_next_pair(a, v, ld);
+    if ((unsigned)(ld.b - ld.wbase) >= 32u) {
+      ld.wbase = ld.b;
+      ld.ids = ld.b + lane < ld.nb && ld.b + lane < a.bt_pitch ? __ldg(ld.bt + ld.b + lane) : -1;
     }
-    int blk = __shfl_sync(0xffffffffu, ids, j & 31);
+    int blk = __shfl_sync(0xffffffffu, ld.ids, ld.b - ld.wbase);
     if (lane == 0) {
       if (blk < 0 || blk >= a.num_blocks) {
         hy_flag(a.err, HY_ERR_BOUNDS);
         blk = 0;
       }
-      const int s = j % NS;
+      const uint32_t s = put % NS;
       fence_proxy_async();
       mbar_arrive_expect_tx(&bars[s], BLK_BYTES);
-      bulk_load(ring + s * BLK_BYTES, a.cache + q4_tile(blk, g, 0, a.kv_heads), BLK_BYTES,
+      bulk_load(ring + s * BLK_BYTES, a.cache + q4_tile(blk, ld.g, 0, a.kv_heads), BLK_BYTES,
                 &bars[s]);
     }
+    ++ld.b;
+    ++put;
   };
-  for (int j = 0; j < NS && j < n; ++j) issue(j);
-
-  // Q: lane (r, c) holds head r's dimensions 32 c .. 32 c + 31 (rows 4-7: zero)
-  uint32_t qb[4][4];
-  float mult[2];
-  {
-    float x[32], amax = 0.f, down, up;
-    const __nv_bfloat16* qp = a.q + ((size_t)tok * a.q_heads + g * HY_GROUP + r) * HY_HEAD_DIM + 32 * c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4 u = r < HY_GROUP ? *reinterpret_cast<const uint4*>(qp + 8 * i) : make_uint4(0, 0, 0, 0);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
-        x[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(x[i]));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    q4_query_scale(amax, down, up);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        qb[i][j] = q4_as_u32(__floats2half2_rn(x[8 * i + 2 * j] * down, x[8 * i + 2 * j + 1] * down));
-    mult[0] = a.scale_log2 * __shfl_sync(0xffffffffu, up, 8 * c);        // head 2 c: lanes of row 2 c
-    mult[1] = a.scale_log2 * __shfl_sync(0xffffffffu, up, 8 * c + 4);
-  }
+#pragma unroll 1
+  for (int j = 0; j < NS; ++j) issue();
 
   const int keyA = key_of(r >> 1, r & 1, 0), keyB = keyA | 4;            // this lane's score rows
-  bool ok = true;
+  bool ok = true, first_pair = true;
 #pragma unroll 1
-  for (int i = 0; i < n; ++i) {
-    const int s = i % NS;
-    const bool w_ok = mbar_wait(&bars[s], (phase >> s) & 1u, a.err);
-    if (__any_sync(0xffffffffu, !w_ok)) { ok = false; break; }
-    phase ^= 1u << s;
-    const uint8_t* kt = ring + s * BLK_BYTES;
-    const uint8_t* vt = kt + Q4_TILE_BYTES;
-
-    // S^T = K Q^T
-    float sc[4] = {0.f, 0.f, 0.f, 0.f};
+  while (left > 0 && ok) {
+    const int n = min(left, k.nb - k.b), b_first = k.b;   // this pair's blocks in the range
+    left -= n;
+    const int tok = a.cu_q[k.seq], kv_len = a.seq_lens_k[k.seq];
+    // Q in fp16 (q4_query_scale): lane (r, c) holds head r's words 2 c, 2 c + 1 (dimensions
+    // 16 c ..) of both halves; rows 4-7 are zero.  Codes in bits 0-3 meet 2^14 q, codes
+    // in bits 4-7 2^10 q, so that a score comes out as 2^-10 code . q.
+    uint32_t qb[2][2][4];
+    float qs[2][2], mult[2];                              // sums of q of heads 2 c + k, scale
     {
-      const uint4 wa = *reinterpret_cast<const uint4*>(kt + keyA * Q4_ROW_BYTES + 16 * c);
-      const uint4 wb = *reinterpret_cast<const uint4*>(kt + keyB * Q4_ROW_BYTES + 16 * c);
-      const __half2 pa = *reinterpret_cast<const __half2*>(kt + Q4_PARAM_OFF + keyA * Q4_PARAM_BYTES + 4 * (c >> 1));
-      const __half2 pb = *reinterpret_cast<const __half2*>(kt + Q4_PARAM_OFF + keyB * Q4_PARAM_BYTES + 4 * (c >> 1));
-      const __half2 sa = __low2half2(pa), ma = __high2half2(pa);
-      const __half2 sb = __low2half2(pb), mb = __high2half2(pb);
-      const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
+      float x[32], amax = 0.f, down, up;
+      const __nv_bfloat16* qp = a.q + ((size_t)tok * a.q_heads + k.g * HY_GROUP + r) * HY_HEAD_DIM + 16 * c;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t xa[4], xb[4];
-        q4_expand(ua[w], sa, ma, xa);
-        q4_expand(ub[w], sb, mb, xb);
-        mma_f16_16816(sc, xa[0], xb[0], xa[1], xb[1], qb[w][0], qb[w][1]);
-        mma_f16_16816(sc, xa[2], xb[2], xa[3], xb[3], qb[w][2], qb[w][3]);
-      }
-    }
-    const int kbase = (lo + i) * HY_BLOCK, left = kv_len - kbase;
-    const bool tail = left < HY_BLOCK;                    // only the last block is partial
-    float x[4] = {sc[0] * mult[0], sc[1] * mult[1], sc[2] * mult[0], sc[3] * mult[1]};
-    if (tail) {
-      if (keyA >= left) x[0] = x[1] = -INFINITY;
-      if (keyB >= left) x[2] = x[3] = -INFINITY;
-    }
-    float mx[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
-    const bool grow = mx[0] > m[0] + RESCALE_LOG2 || mx[1] > m[1] + RESCALE_LOG2;
-    if (__any_sync(0xffffffffu, grow)) {
+      for (int i = 0; i < 4; ++i) {
+        const uint4 u = r < HY_GROUP ? *reinterpret_cast<const uint4*>(qp + 64 * (i >> 1) + 8 * (i & 1))
+                                     : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], d));
-        const float m_new = fmaxf(m[k], mx[k]);
-        const float alpha = m_new == -INFINITY ? 1.f : ex2_ftz(m[k] - m_new);
-        m[k] = m_new;
-        l[k] *= alpha;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) { o[j][k] *= alpha; o[j][2 + k] *= alpha; }
-      }
-    }
-    const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
-    x[0] = ex2_ftz(x[0] - m0);
-    x[1] = ex2_ftz(x[1] - m1);
-    x[2] = ex2_ftz(x[2] - m0);
-    x[3] = ex2_ftz(x[3] - m1);
-    l[0] += x[0] + x[2];
-    l[1] += x[1] + x[3];
-    // P^T as the 16 x 8 operand: weights in fp16 (2^-11; their sum l stays fp32)
-    const uint32_t b0 = movmatrix_trans(q4_as_u32(__floats2half2_rn(x[0], x[1])));
-    const uint32_t b1 = movmatrix_trans(q4_as_u32(__floats2half2_rn(x[2], x[3])));
-
-    // O^T += V^T P^T: words r and 8 + r (dimensions 8 r .. and 64 + 8 r ..) of four keys
-    uint32_t xv[2][2][4];                                 // [half of the keys][low, high nibbles]
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {                // dimensions 0-63, then 64-127: rows r, r + 8
-      uint32_t y[2][2][4];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k0 = key_of(c, 0, h), k1 = key_of(c, 1, h);
-        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(vt + k0 * Q4_ROW_BYTES + 32 * half + 4 * r);
-        const uint32_t w1 = *reinterpret_cast<const uint32_t*>(vt + k1 * Q4_ROW_BYTES + 32 * half + 4 * r);
-        uint32_t p0 = *reinterpret_cast<const uint32_t*>(vt + Q4_PARAM_OFF + k0 * Q4_PARAM_BYTES + 4 * half);
-        uint32_t p1 = *reinterpret_cast<const uint32_t*>(vt + Q4_PARAM_OFF + k1 * Q4_PARAM_BYTES + 4 * half);
-        if (tail) {                                       // rows past the end hold anything
-          if (k0 >= left) p0 = 0u;
-          if (k1 >= left) p1 = 0u;
+        for (int j = 0; j < 4; ++j) {
+          x[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+          x[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
         }
-        const __half2 s2 = q4_as_half2(__byte_perm(p0, p1, 0x5410));
-        const __half2 m2 = q4_as_half2(__byte_perm(p0, p1, 0x7632));
-        q4_expand(__byte_perm(w0, w1, 0x5410), s2, m2, y[h][0]);
-        q4_expand(__byte_perm(w0, w1, 0x7632), s2, m2, y[h][1]);
       }
-      if (half == 0) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+      for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(x[i]));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      q4_query_scale(amax, down, up);
+      float sum[2] = {0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) xv[h][e][j] = y[h][e][j];
-      } else {
+        for (int j = 0; j < 4; ++j) {
+          const float f = (j & 1) ? 1024.f : 16384.f;     // after down: their product may overflow
+          const __half2 h = __floats2half2_rn(x[8 * i + 2 * j] * down * f, x[8 * i + 2 * j + 1] * down * f);
+          qb[i >> 1][i & 1][j] = q4_as_u32(h);
+          const float2 back = __half22float2(h);          // what the product sees, times 2^-10
+          sum[i >> 1] += (back.x + back.y) * ((j & 1) ? 0x1p-20f : 0x1p-24f);
+        }
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        sum[hf] += __shfl_xor_sync(0xffffffffu, sum[hf], 1);
+        sum[hf] += __shfl_xor_sync(0xffffffffu, sum[hf], 2);
+        qs[hf][0] = __shfl_sync(0xffffffffu, sum[hf], 8 * c);            // head 2 c: lanes of row 2 c
+        qs[hf][1] = __shfl_sync(0xffffffffu, sum[hf], 8 * c + 4);
+      }
+      mult[0] = a.scale_log2 * (1024.f * __shfl_sync(0xffffffffu, up, 8 * c));
+      mult[1] = a.scale_log2 * (1024.f * __shfl_sync(0xffffffffu, up, 8 * c + 4));
+    }
+    DecState t;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t.o[j][0] = t.o[j][1] = t.o[j][2] = t.o[j][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      t.z[i][0] = t.z[i][1] = 0.f;
+      t.m[i] = -INFINITY;
+      t.l[i] = 0.f;
+    }
+    t.vs = 1.f;
+    t.vcap = -1.f;                                        // the first block sets them
+
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const uint32_t s = get % NS;
+      const bool w_ok = mbar_wait(&bars[s], (get / NS) & 1u, a.err);
+      if (__any_sync(0xffffffffu, !w_ok)) { ok = false; break; }
+      ++get;
+      const uint8_t* kt = ring + s * BLK_BYTES;
+      const uint8_t* vt = kt + Q4_TILE_BYTES;
+
+      // S^T = K Q^T, one accumulator per half of the dimensions
+      float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const uint2 wa = *reinterpret_cast<const uint2*>(kt + keyA * Q4_ROW_BYTES + 32 * hf + 8 * c);
+        const uint2 wb = *reinterpret_cast<const uint2*>(kt + keyB * Q4_ROW_BYTES + 32 * hf + 8 * c);
+        uint32_t xa[4], xb[4];
+        q4_bits(wa.x, xa);
+        q4_bits(wb.x, xb);
+        mma_f16_16816(sc[hf], xa[0], xb[0], xa[1], xb[1], qb[hf][0][0], qb[hf][0][1]);
+        mma_f16_16816(sc[hf], xa[2], xb[2], xa[3], xb[3], qb[hf][0][2], qb[hf][0][3]);
+        q4_bits(wa.y, xa);
+        q4_bits(wb.y, xb);
+        mma_f16_16816(sc[hf], xa[0], xb[0], xa[1], xb[1], qb[hf][1][0], qb[hf][1][1]);
+        mma_f16_16816(sc[hf], xa[2], xb[2], xa[3], xb[3], qb[hf][1][2], qb[hf][1][3]);
+      }
+      float x[4], sv[2][2], mv[2][2];                     // scores; V's scales and minima [row][half]
+      {
+        const uint2 pa = *reinterpret_cast<const uint2*>(kt + Q4_PARAM_OFF + keyA * Q4_PARAM_BYTES);
+        const uint2 pb = *reinterpret_cast<const uint2*>(kt + Q4_PARAM_OFF + keyB * Q4_PARAM_BYTES);
+        const float2 a0 = __half22float2(q4_as_half2(pa.x)), a1 = __half22float2(q4_as_half2(pa.y));
+        const float2 b0 = __half22float2(q4_as_half2(pb.x)), b1 = __half22float2(q4_as_half2(pb.y));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          x[e] = mult[e] * fmaf(a0.x, sc[0][e], fmaf(a1.x, sc[1][e], fmaf(a0.y, qs[0][e], a1.y * qs[1][e])));
+          x[2 + e] = mult[e] * fmaf(b0.x, sc[0][2 + e], fmaf(b1.x, sc[1][2 + e], fmaf(b0.y, qs[0][e], b1.y * qs[1][e])));
+        }
+        uint2 va = *reinterpret_cast<const uint2*>(vt + Q4_PARAM_OFF + keyA * Q4_PARAM_BYTES);
+        uint2 vb = *reinterpret_cast<const uint2*>(vt + Q4_PARAM_OFF + keyB * Q4_PARAM_BYTES);
+        const int rest = kv_len - (b_first + i) * HY_BLOCK;
+        if (rest < HY_BLOCK) {                            // the last block: rows past the end hold anything
+          if (keyA >= rest) { x[0] = x[1] = -INFINITY; va = make_uint2(0u, 0u); }
+          if (keyB >= rest) { x[2] = x[3] = -INFINITY; vb = make_uint2(0u, 0u); }
+        }
+        const float2 c0 = __half22float2(q4_as_half2(va.x)), c1 = __half22float2(q4_as_half2(va.y));
+        const float2 d0 = __half22float2(q4_as_half2(vb.x)), d1 = __half22float2(q4_as_half2(vb.y));
+        sv[0][0] = c0.x; sv[0][1] = c1.x; sv[1][0] = d0.x; sv[1][1] = d1.x;
+        mv[0][0] = c0.y; mv[0][1] = c1.y; mv[1][0] = d0.y; mv[1][1] = d1.y;
+      }
+      float mx[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+      float smax = fmax3f(sv[0][0], sv[0][1], fmaxf(sv[1][0], sv[1][1]));
+      const bool grow = mx[0] > t.m[0] + RESCALE_LOG2 || mx[1] > t.m[1] + RESCALE_LOG2 || smax > t.vcap;
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, d));
+        float vr = 1.f;                                   // change of vs
+        if (smax > t.vcap) {                              // 2^(6 - exponent), for scales of 2^-24 and up
+          const int e = min(max((__float_as_int(smax) >> 23) & 255, 103), 254) - 127;
+          const float vs = __int_as_float((6 - e + 127) << 23);
+          vr = t.vcap < 0.f ? 1.f : vs / t.vs;
+          t.vs = vs;
+          t.vcap = __int_as_float((e + 127) << 23) * 1.9990234375f;   // the largest fp16 below 2^(e + 1)
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], d));
+          const float m_new = fmaxf(t.m[e], mx[e]);
+          const float alpha = m_new == -INFINITY ? 1.f : ex2_ftz(t.m[e] - m_new);
+          t.m[e] = m_new;
+          t.l[e] *= alpha;
+          t.z[0][e] *= alpha;
+          t.z[1][e] *= alpha;
+          const float ao = alpha * vr;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) { t.o[j][e] *= ao; t.o[j][2 + e] *= ao; }
+        }
+      }
+      const float m0 = t.m[0] == -INFINITY ? 0.f : t.m[0], m1 = t.m[1] == -INFINITY ? 0.f : t.m[1];
+      x[0] = ex2_ftz(x[0] - m0);
+      x[1] = ex2_ftz(x[1] - m1);
+      x[2] = ex2_ftz(x[2] - m0);
+      x[3] = ex2_ftz(x[3] - m1);
+      t.l[0] += x[0] + x[2];
+      t.l[1] += x[1] + x[3];
+      uint32_t pb[2][2];                                  // P^T operands [half][keys 0-7, 8-15]
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const float wa = sv[0][hf] * t.vs, wb = sv[1][hf] * t.vs;
+        pb[hf][0] = movmatrix_trans(q4_as_u32(__floats2half2_rn(x[0] * wa, x[1] * wa)));
+        pb[hf][1] = movmatrix_trans(q4_as_u32(__floats2half2_rn(x[2] * wb, x[3] * wb)));
+        t.z[hf][0] = fmaf(x[0], mv[0][hf], fmaf(x[2], mv[1][hf], t.z[hf][0]));
+        t.z[hf][1] = fmaf(x[1], mv[0][hf], fmaf(x[3], mv[1][hf], t.z[hf][1]));
+      }
+      // O^T += V^T (scale P)^T, a half of the dimensions per product: rows r / r + 8 of m-tile
+      // (hf, e, j) are nibble 4 e + j of words r / ... of the half: its word r holds
+      // dimensions 8 r .. 8 r + 7, one per m-tile, so both row groups come from it
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        uint32_t y[2][2][4];                              // [keys 0-7, 8-15][low, high nibbles]
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(vt + key_of(c, 0, h) * Q4_ROW_BYTES + 32 * hf + 4 * r);
+          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(vt + key_of(c, 1, h) * Q4_ROW_BYTES + 32 * hf + 4 * r);
+          q4_bits(__byte_perm(w0, w1, 0x5410), y[h][0]);
+          q4_bits(__byte_perm(w0, w1, 0x7632), y[h][1]);
+        }
+        // two nibbles of equal weight share an m-tile: rows 0-7 nibble j, rows 8-15 nibble j + 2
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma_f16_16816(o[4 * e + j], xv[0][e][j], y[0][e][j], xv[1][e][j], y[1][e][j], b0, b1);
+          for (int j = 0; j < 2; ++j)
+            mma_f16_16816(t.o[4 * hf + 2 * e + j], y[0][e][j], y[0][e][j + 2], y[1][e][j], y[1][e][j + 2],
+                          pb[hf][0], pb[hf][1]);
       }
+      __syncwarp();                                       // the stage is read
+      issue();
     }
-    __syncwarp();                                         // the stage is read
-    if (i + NS < n) issue(i + NS);
-  }
-  if (!ok) {                                              // copies in flight land before the CTA exits
-    for (int s = 0; s < NS; ++s) mbar_wait(&bars[s], (phase >> s) & 1u, nullptr);
-    return false;
-  }
-  return true;
-}
+    if (!ok) break;
 
-// The CTA runs decode items [i0, i0 + cnt), cnt <= CHUNK: warp w takes half w % 2
-// of item w / 2's blocks; then thread t merges head t / 128, dimension t % 128 of every
-// (sequence, head) among them.  A pair whose items are all here is done; of the
-// others (the first and the last at most) one partial per chunk goes to the slot of
-// its first item in the chunk, and the CTA whose count completes the pair joins the
-// partials.  Returns false if a wait ran out.
-__device__ bool decode_chunk(const Args& a, const PlanView& v, int i0, int cnt, uint8_t* payload,
-                             Shared& sh, uint32_t& phase) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
-  float* parts = reinterpret_cast<float*>(payload + NW * RING_BYTES);
-  bool ok = true;
-  if ((warp >> 1) < cnt) {
-    const int item = i0 + (warp >> 1);
-    const int4 it = v.dec[2 * item], info = v.dec[2 * item + 1];
-    const int seq = it.x, g = it.y, mid = (it.z + it.w + 1) >> 1;
-    const int32_t* bt = a.block_tables + (size_t)(a.seq_bt_row ? a.seq_bt_row[seq] : seq) * a.bt_pitch;
-    float o[8][4], m[2], l[2];
-    ok = decode_range(a, payload + warp * RING_BYTES, sh.bar[warp], phase, bt, info.x, g,
-                      (warp & 1) ? mid : it.z, (warp & 1) ? it.w : mid, info.y, o, m, l);
+    // the pair's result, or a partial of it
+    const bool whole = b_first == 0 && n == k.nb;
+    const int slot = first_pair ? 0 : 1;
+    float inv[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int e = 0; e < 2; ++e) {
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1) l[k] += __shfl_xor_sync(0xffffffffu, l[k], d);
-    float* pw = parts + warp * PART_FLOATS;
+      for (int d = 4; d < 32; d <<= 1) {
+        t.l[e] += __shfl_xor_sync(0xffffffffu, t.l[e], d);
+        t.z[0][e] += __shfl_xor_sync(0xffffffffu, t.z[0][e], d);
+        t.z[1][e] += __shfl_xor_sync(0xffffffffu, t.z[1][e], d);
+      }
+      inv[e] = whole ? 1.f / t.l[e] : 1.f;
+    }
+    const float unit0 = 0x1p24f / t.vs, unit1 = 0x1p20f / t.vs;   // m-tiles of bits 0-3, 4-7
     if (c < 2) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float* ph = pw + (2 * c + k) * HY_HEAD_DIM + 8 * r;
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float4* p4 = reinterpret_cast<float4*>(ph + 64 * half);
-          p4[0] = make_float4(o[0][2 * half + k], o[4][2 * half + k], o[1][2 * half + k], o[5][2 * half + k]);
-          p4[1] = make_float4(o[2][2 * half + k], o[6][2 * half + k], o[3][2 * half + k], o[7][2 * half + k]);
+        for (int hf = 0; hf < 2; ++hf) {
+          // nibble i (of 8): m-tile 4 hf + 2 (i / 4) + i % 2, row group (i % 4) / 2
+          float y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float u = t.o[4 * hf + 2 * (i >> 2) + (i & 1)][2 * ((i & 3) >> 1) + e];
+            y[i < 4 ? 2 * i : 2 * (i - 4) + 1] = fmaf(u, (i & 1) ? unit1 : unit0, t.z[hf][e]) * inv[e];
+          }
+          const int at = (2 * c + e) * HY_HEAD_DIM + 64 * hf + 8 * r;
+          if (whole) {
+            *reinterpret_cast<uint4*>(a.out + ((size_t)tok * a.q_heads + k.g * HY_GROUP) * HY_HEAD_DIM + at) =
+                make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]),
+                           pack_bf16(y[6], y[7]));
+          } else {
+            float4* p4 = reinterpret_cast<float4*>(part + slot * PART_FLOATS + at);
+            p4[0] = make_float4(y[0], y[1], y[2], y[3]);
+            p4[1] = make_float4(y[4], y[5], y[6], y[7]);
+          }
         }
-        if (r == 0) {
-          pw[HY_GROUP * HY_HEAD_DIM + 2 * (2 * c + k)] = m[k];
-          pw[HY_GROUP * HY_HEAD_DIM + 2 * (2 * c + k) + 1] = l[k];
-        }
-      }
+      if (!whole && r == 0)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<float2*>(part + slot * PART_FLOATS + HY_GROUP * HY_HEAD_DIM + 2 * (2 * c + e)) =
+              make_float2(t.m[e], t.l[e]);
     }
+    if (!whole && lane == 0) {
+      part_pair[slot] = k.seq * a.kv_heads + k.g;
+      part_blocks[slot] = n;
+    }
+    first_pair = false;
+    k.b += n;
+    if (left > 0) cursor_next_pair(a, v, k);
   }
+  ring_ctr = put;
+  if (!ok)                                                // copies in flight land before the CTA exits
+    for (uint32_t j = get; j < put; ++j) mbar_wait(&bars[j % NS], (j / NS) & 1u, nullptr);
+  return ok;
+}
+
+// The CTA runs key blocks [f0, f1) of the flattened list: its warps take equal parts,
+// then thread t merges head t / 128, dimension t % 128 of every pair that a warp did not
+// finish alone.  A pair that reaches out of the range (its first or last) leaves one
+// partial in the workspace (slot 2 unit, or 2 unit + 1 where the pair starts inside the
+// range), and the CTA whose count of blocks completes a pair joins its partials.
+// Returns false if a wait ran out.
+HY_DEVICE long unit_start(long total, int units, int u) { return total * u / units; }
+
+__device__ bool decode_unit(const Args& a, const PlanView& v, long total, int units, int unit,
+                            long f0, long f1, uint8_t* payload, Shared& sh, uint32_t& ring_ctr) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  float* parts = reinterpret_cast<float*>(payload + NW * RING_BYTES);
+  if (lane < 2) sh.part_pair[warp][lane] = -1;
+  __syncwarp();
+  const long n = f1 - f0;
+  const bool ok = decode_warp(a, v, f0 + n * warp / NW, f0 + n * (warp + 1) / NW,
+                              payload + warp * RING_BYTES, parts + warp * 2 * PART_FLOATS,
+                              sh.part_pair[warp], sh.part_blocks[warp], sh.bar[warp], ring_ctr);
   if (__syncthreads_or(!ok)) return false;
 
   const int head = tid >> 7, d = tid & 127;
-  int open_first[2] = {-1, -1}, open_ns[2], open_cnt[2], n_open = 0;
-  for (int j = 0; j < cnt;) {
-    const int4 it = v.dec[2 * (i0 + j)], info = v.dec[2 * (i0 + j) + 1];
-    const int ns = info.z, first = info.w;
-    const int run = min(cnt - j, first + ns - (i0 + j));  // items of this pair in the chunk
+  int open_pair[2], open_blocks[2], n_open = 0;
+  for (int i = 0; i < 2 * NW;) {
+    const int pair = sh.part_pair[i >> 1][i & 1];
+    if (pair < 0) { ++i; continue; }
+    int end = i, blocks = 0;
     float M = -INFINITY;
-    for (int w = 2 * j; w < 2 * (j + run); ++w)
-      M = fmaxf(M, parts[w * PART_FLOATS + HY_GROUP * HY_HEAD_DIM + 2 * head]);
+    for (; end < 2 * NW; ++end) {
+      const int p = sh.part_pair[end >> 1][end & 1];
+      if (p < 0) continue;
+      if (p != pair) break;
+      blocks += sh.part_blocks[end >> 1][end & 1];
+      M = fmaxf(M, parts[end * PART_FLOATS + HY_GROUP * HY_HEAD_DIM + 2 * head]);
+    }
     const float Mu = M == -INFINITY ? 0.f : M;
     float L = 0.f, acc = 0.f;
-    for (int w = 2 * j; w < 2 * (j + run); ++w) {
-      const float* pw = parts + w * PART_FLOATS;
+    for (int j = i; j < end; ++j) {
+      if (sh.part_pair[j >> 1][j & 1] < 0) continue;
+      const float* pw = parts + j * PART_FLOATS;
       const float wt = ex2_ftz(pw[HY_GROUP * HY_HEAD_DIM + 2 * head] - Mu);
       L = fmaf(wt, pw[HY_GROUP * HY_HEAD_DIM + 2 * head + 1], L);
       acc = fmaf(wt, pw[tid], acc);
     }
-    if (run == ns) {
-      a.out[((size_t)info.x * a.q_heads + it.y * HY_GROUP + head) * HY_HEAD_DIM + d] =
+    const int seq = pair / a.kv_heads, g = pair - seq * a.kv_heads;
+    const int p0 = v.dec_blocks[seq], nb = v.dec_blocks[seq + 1] - p0;
+    if (blocks == nb) {
+      a.out[((size_t)a.cu_q[seq] * a.q_heads + g * HY_GROUP + head) * HY_HEAD_DIM + d] =
           __float2bfloat16_rn(acc / L);
     } else {
-      __stcg(v.part_o + (size_t)(i0 + j) * (HY_GROUP * HY_HEAD_DIM) + tid, acc);
-      if (d == 0) __stcg(v.part_ml + (size_t)(i0 + j) * HY_GROUP + head, make_float2(M, L));
-      open_first[n_open & 1] = first;
-      open_ns[n_open & 1] = ns;
-      open_cnt[n_open & 1] = run;
+      const long F0 = (long)p0 * a.kv_heads + (long)g * nb;
+      const size_t slot = 2 * unit + (F0 > f0);
+      __stcg(v.part_o + slot * (HY_GROUP * HY_HEAD_DIM) + tid, acc);
+      if (d == 0) __stcg(v.part_ml + slot * HY_GROUP + head, make_float2(M, L));
+      open_pair[n_open & 1] = pair;
+      open_blocks[n_open & 1] = blocks;
       ++n_open;
     }
-    j += run;
+    i = end;
   }
   if (n_open == 0) {
     __syncthreads();                                      // parts are read
@@ -366,11 +515,11 @@ __device__ bool decode_chunk(const Args& a, const PlanView& v, int i0, int cnt, 
   __syncthreads();
   if (tid == 0) {
     int last = 0;
-    for (int k = 0; k < n_open; ++k) {
-      const int4 it = v.dec[2 * open_first[k]];
-      int* ctr = &v.counters[it.x * a.kv_heads + it.y];
-      if (atomicAdd(ctr, open_cnt[k]) + open_cnt[k] == open_ns[k]) {
-        last |= 1 << k;
+    for (int j = 0; j < n_open; ++j) {
+      const int seq = open_pair[j] / a.kv_heads;
+      int* ctr = &v.counters[open_pair[j]];
+      if (atomicAdd(ctr, open_blocks[j]) + open_blocks[j] == v.dec_blocks[seq + 1] - v.dec_blocks[seq]) {
+        last |= 1 << j;
         *ctr = 0;                                         // for the next launch on this plan
       }
     }
@@ -379,25 +528,30 @@ __device__ bool decode_chunk(const Args& a, const PlanView& v, int i0, int cnt, 
   __syncthreads();
   const int last = sh.last;
   __threadfence();                                        // the others' partials, after the count
-  for (int k = 0; k < n_open; ++k) {
-    if (!((last >> k) & 1)) continue;
-    const int first = open_first[k], end = first + open_ns[k];
-    const int4 it = v.dec[2 * first], info = v.dec[2 * first + 1];
-    // partials stand at the pair's first item and at every chunk boundary inside it
-    auto next = [](int i) { return (i / CHUNK + 1) * CHUNK; };
-    float M = -INFINITY;
-    for (int i = first; i < end; i = next(i))
-      M = fmaxf(M, __ldcg(v.part_ml + (size_t)i * HY_GROUP + head).x);
-    const float Mu = M == -INFINITY ? 0.f : M;
-    float L = 0.f, acc = 0.f;
+  for (int j = 0; j < n_open; ++j) {
+    if (!((last >> j) & 1)) continue;
+    const int seq = open_pair[j] / a.kv_heads, g = open_pair[j] - seq * a.kv_heads;
+    const int p0 = v.dec_blocks[seq], nb = v.dec_blocks[seq + 1] - p0;
+    const long F0 = (long)p0 * a.kv_heads + (long)g * nb, F1 = F0 + nb;
+    int u0 = (int)(F0 * units / total);                   // the unit that holds block F0
+    while (unit_start(total, units, u0 + 1) <= F0) ++u0;
+    float M = -INFINITY, L = 0.f, acc = 0.f;
 #pragma unroll 4
-    for (int i = first; i < end; i = next(i)) {
-      const float2 ml = __ldcg(v.part_ml + (size_t)i * HY_GROUP + head);
-      const float wt = ex2_ftz(ml.x - Mu);
-      L = fmaf(wt, ml.y, L);
-      acc = fmaf(wt, __ldcg(v.part_o + (size_t)i * (HY_GROUP * HY_HEAD_DIM) + tid), acc);
+    for (int u = u0; u < units; ++u) {
+      const long s0 = unit_start(total, units, u), s1 = unit_start(total, units, u + 1);
+      if (s0 >= F1) break;
+      if (s0 == s1) continue;
+      const size_t slot = 2 * u + (F0 > s0);
+      const float2 ml = __ldcg(v.part_ml + slot * HY_GROUP + head);
+      const float po = __ldcg(v.part_o + slot * (HY_GROUP * HY_HEAD_DIM) + tid);
+      const float m_new = fmaxf(M, ml.x);
+      const float w0 = m_new == -INFINITY ? 1.f : ex2_ftz(M - m_new);
+      const float w1 = m_new == -INFINITY ? 1.f : ex2_ftz(ml.x - m_new);
+      L = fmaf(L, w0, ml.y * w1);
+      acc = fmaf(acc, w0, po * w1);
+      M = m_new;
     }
-    a.out[((size_t)info.x * a.q_heads + it.y * HY_GROUP + head) * HY_HEAD_DIM + d] =
+    a.out[((size_t)a.cu_q[seq] * a.q_heads + g * HY_GROUP + head) * HY_HEAD_DIM + d] =
         __float2bfloat16_rn(acc / L);
   }
   return true;
@@ -473,9 +627,8 @@ HY_DEVICE void expand_row(const RowCodes& x, uint8_t* slot, int key) {
 
 // One prefill item, all warps of the CTA (roles as above).  The products, barriers
 // and softmax follow attention.cu's prefill: S(t + 1) is issued while the softmax
-// works on S(t); S(t) may overwrite its buffer because P V(t - 2) was issued before it
-// by the same thread; the softmax writes P(t) over S(t) and waits for P V(t - 1) only
-// to rescale O.  c = c0 + t counts key tiles over all items of the launch.
+// works on S(t); the softmax writes P(t) over S(t) and waits for P V(t - 1) only to
+// rescale O.  c = c0 + t counts key tiles over all items of the launch.
 // Returns false if a wait ran out; the roles then drain what they issued.
 __device__ bool prefill_item(const Args& a, const PlanView& v, int item, uint8_t* payload,
                              Shared& sh, uint32_t tmem, uint32_t& ctr, uint32_t qpar) {
@@ -521,6 +674,11 @@ __device__ bool prefill_item(const Args& a, const PlanView& v, int item, uint8_t
           const uint32_t c = c0 + t, slot = c % PS;
           ok = mbar_wait(&sh.full[slot], (c / PS) & 1, a.err);
           if (!ok) break;
+          // S(t) goes over P(t - 2): products of different shapes are not ordered among
+          // themselves, so the one that reads it is waited for (it was issued a softmax
+          // tile ago; the wait also tells the softmax, which waits for S(t), that it is done)
+          if (t > 1) ok = mbar_wait(&sh.odone[X][c & 1], ((c - 2) >> 1) & 1, a.err);
+          if (!ok) break;
           tc_fence_after();
           const uint64_t dK = tc_desc_sw128(sbase + K_OFF + slot * KV_BYTES, 16, 1024);
 #pragma unroll
@@ -541,7 +699,7 @@ __device__ bool prefill_item(const Args& a, const PlanView& v, int item, uint8_t
           for (int kk = 0; kk < PRE_KEYS / 16; ++kk)
             tc_mma_bf16_ta(tmem + TM_O + 128 * X, tmem + tm_s(X, c & 1) + 8 * kk,
                            dV + (uint64_t)((kk * 2048) >> 4), ID_O, (t > 1 || kk > 0));
-          tc_commit(&sh.odone[X]);
+          tc_commit(&sh.odone[X][c & 1]);
           tc_commit(&sh.free_[slot]);
         }
       }
@@ -603,9 +761,12 @@ __device__ bool prefill_item(const Args& a, const PlanView& v, int item, uint8_t
       if (!ok) break;
       tc_fence_after();
       float s[64];
-      tmem_ld32(tS, *reinterpret_cast<float(*)[32]>(&s[0]));
-      tmem_ld32(tS + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
-      tmem_wait_ld();
+      float (&s_lo)[32] = *reinterpret_cast<float(*)[32]>(&s[0]);
+      float (&s_hi)[32] = *reinterpret_cast<float(*)[32]>(&s[32]);
+      tmem_ld32(tS, s_lo);
+      tmem_ld32(tS + 32, s_hi);
+      tmem_wait_ld(s_lo);
+      tmem_wait_ld(s_hi);
       const int kb = (P.tlo + t) * PRE_KEYS;
       if (kb + PRE_KEYS - 1 > P.prefix + P.t0) {          // the tile reaches the diagonal or the end
 #pragma unroll
@@ -630,13 +791,13 @@ __device__ bool prefill_item(const Args& a, const PlanView& v, int item, uint8_t
         l *= alpha;
         m = mnew;
         if (t > 0) {                                      // O holds tiles < t: wait for P V(t - 1)
-          ok = __all_sync(0xffffffffu, mbar_wait(&sh.odone[X], (c & 1) ^ 1, a.err));
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.odone[X][(c & 1) ^ 1], ((c - 1) >> 1) & 1, a.err));
           tc_fence_after();
 #pragma unroll 1
           for (int cc = 0; cc < 4; ++cc) {
             float o[32];
             tmem_ld32(tO + 32 * cc, o);
-            tmem_wait_ld();
+            tmem_wait_ld(o);
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] *= alpha;
             tmem_st32(tO + 32 * cc, o);
@@ -665,7 +826,7 @@ __device__ bool prefill_item(const Args& a, const PlanView& v, int item, uint8_t
     }
     if (ok) {                                             // epilogue: O_X complete
       const uint32_t c = c0 + ntiles - 1;
-      ok = __all_sync(0xffffffffu, mbar_wait(&sh.odone[X], c & 1, a.err));
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.odone[X][c & 1], (c >> 1) & 1, a.err));
       tc_fence_after();
     }
     const bool store = ok && real;
@@ -679,7 +840,7 @@ __device__ bool prefill_item(const Args& a, const PlanView& v, int item, uint8_t
       for (int cc = 0; cc < 4; ++cc) {
         float o[32];
         tmem_ld32(tO + 32 * cc, o);                       // warp-collective: every lane loads
-        tmem_wait_ld();
+        tmem_wait_ld(o);
         if (store) {
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4)
@@ -697,30 +858,38 @@ __device__ bool prefill_item(const Args& a, const PlanView& v, int item, uint8_t
   return ok;
 }
 
-// Decode items, in whichever way suits their number.  Returns false if a wait ran out.
-__device__ bool decode_items(const Args& a, const PlanView& v, int n_pre, int n_dec, int n_pairs,
-                             uint8_t* payload, Shared& sh) {
-  uint32_t phase = 0;
-  if (n_pairs > 0) {                                      // a (sequence, KV head) pair per CTA
+// The step's decode sequences.  Alone in the launch, their key blocks are dealt evenly
+// over the CTAs; a small step's pairs go one to a CTA, which merges them in shared memory;
+// beside prefill items, whose CTAs come late, CTAs take units of a third of an even
+// share.  Returns false if a wait ran out.
+constexpr int MIXED_UNITS = 3;
+__device__ bool decode_all(const Args& a, const PlanView& v, int n_pre, int n_pairs, long blocks,
+                           uint8_t* payload, Shared& sh) {
+  uint32_t ring_ctr = 0;
+  const long total = blocks * a.kv_heads;
+  if (total == 0) return true;
+  if (n_pairs > 0) {
     if ((int)blockIdx.x >= n_pairs) return true;
     const int seq = (int)blockIdx.x / a.kv_heads, g = (int)blockIdx.x - seq * a.kv_heads;
-    const int2 si = v.seqinfo[seq];                       // first item, items per head
-    return si.y == 0 || decode_chunk(a, v, si.x + g * si.y, si.y, payload, sh, phase);
+    const int p0 = v.dec_blocks[seq], nb = v.dec_blocks[seq + 1] - p0;
+    const long f0 = (long)p0 * a.kv_heads + (long)g * nb;
+    return nb == 0 || decode_unit(a, v, total, 0, 0, f0, f0 + nb, payload, sh, ring_ctr);
   }
-  const int chunks = (n_dec + CHUNK - 1) / CHUNK;
-  if (n_pre == 0 && chunks <= (int)gridDim.x) {           // one round: no counters
-    if ((int)blockIdx.x >= chunks) return true;
-    const int i0 = (int)blockIdx.x * CHUNK;
-    return decode_chunk(a, v, i0, min(CHUNK, n_dec - i0), payload, sh, phase);
+  if (n_pre == 0) {
+    const int u = blockIdx.x, units = gridDim.x;
+    return decode_unit(a, v, total, units, u, unit_start(total, units, u),
+                       unit_start(total, units, u + 1), payload, sh, ring_ctr);
   }
+  const int units = MIXED_UNITS * gridDim.x;
   int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
   for (;;) {
-    if (threadIdx.x == 0) sh.chunk = atomicAdd(&grab[0], 1);
+    if (threadIdx.x == 0) sh.unit = atomicAdd(&grab[0], 1);
     __syncthreads();
-    const int k = sh.chunk;
+    const int u = sh.unit;
     __syncthreads();
-    if (k >= chunks) return true;
-    if (!decode_chunk(a, v, k * CHUNK, min(CHUNK, n_dec - k * CHUNK), payload, sh, phase))
+    if (u >= units) return true;
+    if (!decode_unit(a, v, total, units, u, unit_start(total, units, u),
+                     unit_start(total, units, u + 1), payload, sh, ring_ctr))
       return false;
   }
 }
@@ -741,8 +910,8 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(Args a, PlanView v) {
       for (int b = 0; b < 2; ++b) {
         mbar_init(&sh.sfull[x][b], 1);
         mbar_init(&sh.pfull[x][b], 4);
+        mbar_init(&sh.odone[x][b], 1);
       }
-      mbar_init(&sh.odone[x], 1);
       mbar_init(&sh.drain[x], 1);
     }
     mbar_init(&sh.qfull, EXP_WARP);
@@ -752,8 +921,8 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(Args a, PlanView v) {
   hy_grid_wait();
   hy_grid_trigger();
   const uint64_t keep = l2_keep_policy();
-  const int n_pre = ld_keep(v.header, keep), n_dec = ld_keep(v.header + 1, keep);
-  const int n_pairs = ld_keep(v.header + 4, keep);
+  const int n_pre = ld_keep(v.header, keep), n_pairs = ld_keep(v.header + 4, keep);
+  const int blocks = ld_keep(v.header + 5, keep);         // key blocks of the decode sequences
   int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
   bool ok = true;
   if ((int)blockIdx.x < n_pre) {                          // the first n_pre CTAs take prefill items
@@ -781,9 +950,9 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(Args a, PlanView v) {
       tmem_dealloc(tmem, TMEM_COLS);
     }
   }
-  if (ok) decode_items(a, v, n_pre, n_dec, n_pairs, payload, sh);
+  if (ok) decode_all(a, v, n_pre, n_pairs, blocks, payload, sh);
   __syncthreads();
-  if ((n_pre > 0 || n_dec > CHUNK * (int)gridDim.x) && threadIdx.x == 0) {
+  if (n_pre > 0 && threadIdx.x == 0) {
     __threadfence();                                      // the last CTA out resets the counters
     if (atomicAdd(&grab[1], 1) == (int)gridDim.x - 1) {
       atomicExch(&grab[0], 0);
@@ -928,6 +1097,7 @@ cudaError_t hy_launch_attn_q4_bf16(const void* q, void* out, int q_heads, int kv
   a.kv_heads = kv_heads;
   a.num_blocks = num_blocks;
   a.layer = layer;
+  a.num_seqs = S;
   a.block_tables = block_tables;
   a.bt_pitch = bt_pitch;
   a.seq_bt_row = seq_bt_row;

@@ -94,7 +94,7 @@ def read(cache_layer: np.ndarray, slots):
 def attention(q: np.ndarray, cache_layer: np.ndarray, tables: np.ndarray, q_lens, kv_lens,
               scale: float):
     """float64 causal attention (T, Hq, 128) and, per output row, what an error
-    bound needs: sum of p |v|, the largest |scale| sum |q k| over visible keys,
+    bound needs: sum of p (|v| + |minimum of v's half row|), the largest |scale| sum |q k| over visible keys,
     the number of visible keys and the largest |v|."""
     out = np.zeros(q.shape, np.float64)
     absv = np.zeros(q.shape, np.float64)
@@ -106,7 +106,10 @@ def attention(q: np.ndarray, cache_layer: np.ndarray, tables: np.ndarray, q_lens
         x = None
         if ql:
             blocks = tables[i, :-(-kv // BLOCK)]
-            x = values(tile_codes(cache_layer[blocks]), tile_params(cache_layer[blocks]))
+            par = tile_params(cache_layer[blocks])
+            x = values(tile_codes(cache_layer[blocks]), par)
+            low = np.repeat(np.abs(par[:, :, 1, :, 1::2].astype(np.float64)), HALF, -1)
+            low = low.transpose(1, 0, 2, 3).reshape(low.shape[1], -1, HEAD_DIM)[:, :kv]
             x = x.transpose(1, 2, 0, 3, 4).reshape(x.shape[1], 2, -1, HEAD_DIM)[:, :, :kv]
         for h in range(q.shape[1] if ql else 0):
             k, v = x[h // GROUP]
@@ -117,9 +120,9 @@ def attention(q: np.ndarray, cache_layer: np.ndarray, tables: np.ndarray, q_lens
             p = np.exp(z - z.max(-1, keepdims=True))
             p /= p.sum(-1, keepdims=True)
             out[first:first + ql, h] = p @ v
-            absv[first:first + ql, h] = p @ np.abs(v)
+            absv[first:first + ql, h] = p @ (np.abs(v) + low[h // GROUP])
             reach[first:first + ql, h] = np.where(hidden, 0, r).max(-1)
             keys[first:first + ql, h] = (~hidden).sum(-1)
-            vmax[first:first + ql, h] = np.abs(v).max()
+            vmax[first:first + ql, h] = (np.abs(v) + low[h // GROUP]).max()
         first += ql
     return out, absv, reach, keys, vmax

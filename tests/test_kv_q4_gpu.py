@@ -177,14 +177,16 @@ class Batch:
             self.q[:self.T].float().numpy(), self.cache[self.layer], self.tables, self.q_lens,
             self.kv_lens, scale)
         got = out[:self.T].double().cpu().numpy()
-        assert np.isfinite(got).all(), np.argwhere(~np.isfinite(got))[:5]
+        odd = np.argwhere(~np.isfinite(got))
+        assert len(odd) == 0, odd[:5]
         keys, vmax, reach = (a[..., None] for a in (keys, vmax, reach))
         if self.dt == F32:
             # fp32: dot products and sums of `keys` terms, each term rounded (2^-24); exp of
             # an argument off by `reach` roundings of the dot product's 128 terms
             tol = absv * (2.0 ** -23 * (keys + 8) + 2 * 132 * 2.0 ** -24 * (reach + 1)) + 1e-30
         else:
-            # keys, values and weights are held in fp16 where the tensor cores take them (2^-11
+            # keys, values and weights (decode: weights times the value's scale, which meet codes
+            # of up to |v| + |minimum|) are held in fp16 where the tensor cores take them (2^-11
             # relative each; weights below 2^-14 to 2^-25), scores move by 2^-11 of their
             # terms' sum; fp32 sums (2^-23 per term); the output is rounded once to bf16 (2^-8)
             shift = reach * 2.0 ** -11 * 1.1
@@ -203,6 +205,7 @@ CASES = [
     ([64], [64]), ([65], [130]), ([130], [700]), ([200, 1, 64, 1], [200, 90, 1000, 1]),
     ([512], [1111]), ([33] * 6, [33 + 50 * i for i in range(6)]),
     ([1] * 37, [1 + 61 * i % 900 for i in range(37)]),
+    ([1, 0, 1, 1, 0], [0 + 40, 9, 1, 200, 3]), ([1] * 70, [1 + 13 * i % 40 for i in range(70)]),
     ([1, 1], [5003, 37]), ([1] * 20, [2500 - 97 * i for i in range(20)]),   # pairs split over many CTAs
 ]
 
@@ -235,6 +238,23 @@ def test_attention_query_row_ranges(dt):
     b.q[8, :, ::2] *= 1e-6            # far below its row's largest element
     b.q[9] *= 1e5                     # past fp16's range
     b.check(b.run())
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+def test_attention_value_ranges(dt):
+    """Rows whose scales differ by many orders of magnitude, constant rows (scale 0) among them."""
+    for lens in (([1, 1], [900, 40]), ([70], [333])):
+        b = Batch(*lens, 2, dt, seed=14)
+        g = torch.Generator().manual_seed(15)
+        par = q4.tile_params(b.cache)                    # (layers, blocks, heads, 2, 16, 4)
+        f = 10.0 ** (torch.rand(par.shape[:-1], generator=g).numpy() * 7 - 5)[..., None]
+        f[:, ::3] = 0.0                                  # whole blocks of zeros
+        f[:, :, :, 0] = 1.0                              # keys as they are
+        par = (par.astype(np.float64) * f).astype(np.float16)
+        b.cache[..., q4.CODE_BYTES:] = par.view(np.uint8).reshape(*b.cache.shape[:-1], -1)
+        for i, kv in enumerate(b.kv_lens):               # no NaN: they were scaled away above
+            assert np.isfinite(par.astype(np.float64)[:, b.tables[i, :kv // 16]]).all()
+        b.check(b.run())
 
 
 @pytest.mark.parametrize("dt", [F32, BF])
