@@ -127,7 +127,7 @@ struct Shared {
                              // same threads) are done too
   uint64_t tc_sfull[2][2];   // S_X[b] = Q_X K^T complete (once per use of buffer b)
   uint64_t tc_pfull[2][2];   // P_X[b] written over S_X[b] by the 4 softmax warps of X
-  uint64_t tc_odone[2];      // O_X += P_X V complete (once per key tile)
+  uint64_t tc_odone[2][2];   // O_X += P_X[b] V complete (once per use of buffer b)
   uint64_t tc_drain[2];      // error path: all MMAs an issuing warp issued are complete
   uint64_t tc_qfull;         // the item's Q landed (TMA transaction bytes, once per item)
   uint32_t tmem_base;        // TMEM columns from tcgen05.alloc
@@ -889,14 +889,15 @@ HY_DEVICE bool pre_issue_tile(const CUtensorMap* kgroups, const CUtensorMap* til
 // With two S buffers the MMA warp issues S(t+1) while the softmax works on
 // S(t), so the softmax never waits for its scores once the pipeline is full.
 // S(t) may overwrite buffer b only after PV(t-2) has read P(t-2) from it: the
-// issuing thread issued PV(t-2) before S(t), and tcgen05.mma operations of one
-// thread execute in issue order (as the K-step accumulation into one D relies
-// on).  The softmax writes P(t) over S(t) after reading S(t), which completed
-// after PV(t-2); it need not wait for PV(t-1) (the other buffer) except to
+// issuing thread waits for PV(t-2) (products of different shapes are not ordered
+// among themselves; a softmax that took S(t) for a sign that PV(t-2) was complete
+// rescaled O too early on rows of large scores).  The softmax writes P(t) over S(t)
+// after reading S(t), which completed after PV(t-2); it need not wait for PV(t-1)
+// (the other buffer) except to
 // rescale O.
 // c = c0 + t counts key tiles over all items of the launch; each barrier
-// completes exactly once per tile (odone), per use of its buffer (sfull, pfull:
-// every second tile) or per use of its slot (ring barriers), and no role can
+// completes exactly once per use of its buffer (sfull, pfull, odone: every second
+// tile) or per use of its slot (ring barriers), and no role can
 // run a full phase ahead of the role that waits on it, so a wait is always on
 // the current or the previous phase (the load warps, which can get ahead of
 // the S MMAs of a short item, wait for its S phases in order).  Returns false if a wait ran out; the
@@ -1025,6 +1026,10 @@ __device__ bool prefill_item_tc(const CUtensorMap* kgroups, const CUtensorMap* t
           const uint32_t c = c0 + t, slot = c % TC_NS;
           ok = mbar_wait(&sh.tc_full[slot], (c / TC_NS) & 1, a.err);   // K and V landed
           if (!ok) break;
+          // S(t) goes over P(t-2): wait for the P V that reads it.  The wait also tells
+          // the softmax, which waits for S(t), that PV(t-2) is complete
+          if (t > 1) ok = mbar_wait(&sh.tc_odone[X][c & 1], ((c - 2) >> 1) & 1, a.err);
+          if (!ok) break;
           tc_fence_after();
           // K slot: 8-key groups 2 KB apart (SBO), column half h at +1 KB
           const uint64_t dK = tc_desc_sw128(sbase + TC_K_OFF + slot * TC_KV_BYTES, 16, 2048);
@@ -1049,7 +1054,7 @@ __device__ bool prefill_item_tc(const CUtensorMap* kgroups, const CUtensorMap* t
           for (int kk = 0; kk < TC_KEYS / 16; ++kk)
             tc_mma_bf16_ta(tmem + TM_O + 128 * X, tmem + tm_s(X, c & 1) + 8 * kk,
                            dV + (uint64_t)((kk * 4096) >> 4), ID_O, (t > 1 || kk > 0));
-          tc_commit(&sh.tc_odone[X]);
+          tc_commit(&sh.tc_odone[X][c & 1]);
           tc_commit(&sh.tc_free[slot]);
         }
       }
@@ -1105,7 +1110,8 @@ __device__ bool prefill_item_tc(const CUtensorMap* kgroups, const CUtensorMap* t
         l *= alpha;
         m = mnew;
         if (t > 0) {                            // O holds tiles < t: wait for PV(t-1)
-          ok = __all_sync(0xffffffffu, mbar_wait(&sh.tc_odone[X], (c & 1) ^ 1, a.err));
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.tc_odone[X][(c & 1) ^ 1], ((c - 1) >> 1) & 1,
+                                                 a.err));
           tc_fence_after();
 #pragma unroll 1
           for (int cc = 0; cc < 4; ++cc) {
@@ -1150,7 +1156,7 @@ __device__ bool prefill_item_tc(const CUtensorMap* kgroups, const CUtensorMap* t
     }
     if (ok) {                                   // epilogue: O_X complete
       const uint32_t c = c0 + ntiles - 1;
-      ok = __all_sync(0xffffffffu, mbar_wait(&sh.tc_odone[X], c & 1, a.err));
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.tc_odone[X][c & 1], (c >> 1) & 1, a.err));
       tc_fence_after();
     }
     // tcgen05.ld is warp-collective: every lane loads, only real rows store
@@ -1207,8 +1213,8 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_main_kernel(
       for (int b = 0; b < 2; ++b) {
         mbar_init(&sh.tc_sfull[x][b], 1);
         mbar_init(&sh.tc_pfull[x][b], 4);       // one arrival per softmax warp
+        mbar_init(&sh.tc_odone[x][b], 1);
       }
-      mbar_init(&sh.tc_odone[x], 1);
     }
     mbar_init(&sh.tc_drain[0], 1);
     mbar_init(&sh.tc_drain[1], 1);
