@@ -171,6 +171,52 @@ __device__ int plan_scan(int v, int* ws, int& total) {
   return before + x - v;
 }
 
+// Exclusive sums over the CTA of N values per thread (in v), and their totals,
+// in one pass of three barriers.
+template <int N>
+__device__ void plan_scan_n(int (&v)[N], int (*ws)[32], int (&total)[N]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) x[k] = v[k];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int y = __shfl_up_sync(0xffffffffu, x[k], o);
+      if (lane >= o) x[k] += y;
+    }
+  if (lane == 31)
+#pragma unroll
+    for (int k = 0; k < N; ++k) ws[k][warp] = x[k];
+  __syncthreads();
+  if (warp < N) {
+    int w = ws[warp][lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    ws[warp][lane] = w;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    v[k] = (warp ? ws[k][warp - 1] : 0) + x[k] - v[k];
+    total[k] = ws[k][31];
+  }
+  __syncthreads();
+}
+
+// The last of PLAN_THREADS ascending entries of `first` at or below k (first[0] = 0).
+__device__ int plan_find(const int* first, int k) {
+  int lo = 0;
+#pragma unroll
+  for (int step = PLAN_THREADS / 2; step > 0; step >>= 1)
+    if (first[lo + step] <= k) lo += step;
+  return lo;
+}
+
 // a * b / c for non-negative ints, in 32-bit arithmetic when the product fits
 HY_DEVICE int mul_div(int a, int b, int c) {
   const long long p = (long long)a * b;
@@ -247,20 +293,25 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
   const bool group = !s_anypre && (long)S * kv_heads <= warp_slots / ATT_WARPS &&
                      s_maxblk <= GROUP_MAX_BLOCKS;
 
-  // Pass 2: item counts, offsets, items.
+  // Pass 2: item counts, offsets, items.  Each thread counts one sequence's, then the
+  // threads write the items of all of them together.
+  enum { PRE, DEC, PART, BLK, UNIT, SUMS };     // UNIT: (query tile, KV head) pairs
+  __shared__ int s_first_dec[PLAN_THREADS], s_first_unit[PLAN_THREADS];
+  __shared__ int s_pre0[PLAN_THREADS], s_slot0[PLAN_THREADS];
+  __shared__ int s_wsn[SUMS][32];
   for (int base = 0; base < S; base += PLAN_THREADS) {
     const int i = base + threadIdx.x;
-    int npre = 0, ndec = 0, ns = 0, ntile = 0, nblk = 0, row = 0, kv = 0, q = 0;
-    int npart = 0, ph = 0, psl = 0;             // pieces and partial slots per KV head
+    int ns = 0, ntile = 0, nblk = 0;
+    int ph = 0, psl = 0;                        // pieces and partial slots per KV head
+    int sums[SUMS] = {0, 0, 0, 0, 0}, total[SUMS];
     if (i < S) {
-      row = cu_q[i];
-      q = cu_q[i + 1] - row;
-      kv = seq_lens_k[i];
+      const int q = cu_q[i + 1] - cu_q[i], kv = seq_lens_k[i];
       if (q < 0 || kv < q) atomicOr(&s_bad, HY_ERR_BOUNDS);
       else if (q == 1) {
         nblk = (kv + HY_BLOCK - 1) / HY_BLOCK;
         ns = group ? max(1, min(ATT_WARPS, nblk)) : (nblk + split - 1) / split;
-        ndec = kv_heads * ns;
+        sums[DEC] = kv_heads * ns;
+        sums[BLK] = nblk;
       } else if (q > 1) {
         ntile = (q + PRE_QROWS - 1) / PRE_QROWS;
         for (int t = 0; t < ntile; ++t) {
@@ -268,72 +319,71 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
           ph += n;
           if (n > 1) psl += n;
         }
-        npre = kv_heads * ph;
-        npart = kv_heads * psl;
+        sums[PRE] = kv_heads * ph;
+        sums[PART] = kv_heads * psl;
+        sums[UNIT] = kv_heads * ntile;
       }
     }
-    int tpre, tdec, tpart, tblk;
-    const int oblk = plan_scan(nblk, ws, tblk);
-    const int opre = plan_scan(npre, ws, tpre);
-    const int odec = plan_scan(ndec, ws, tdec);
-    const int opart = plan_scan(npart, ws, tpart);
+    const int ndec = sums[DEC], npre = sums[PRE], npart = sums[PART];
+    plan_scan_n<SUMS>(sums, s_wsn, total);
     const int cpre = s_cpre, cdec = s_cdec, cpart = s_cpart;
-    if (i < S && i < v.max_seqs) v.dec_blocks[i] = s_cblk + oblk;
-    if (i < S && i < v.max_seqs)
-      for (int g = 0; g < kv_heads; ++g) v.counters[i * kv_heads + g] = 0;
-    bool wr = false;
-    int p0 = 0, d0 = 0, s0 = 0;
+    const int p0 = cpre + sums[PRE], d0 = cdec + sums[DEC], s0 = cpart + sums[PART];
+    s_first_dec[threadIdx.x] = sums[DEC];
+    s_first_unit[threadIdx.x] = sums[UNIT];
+    s_pre0[threadIdx.x] = p0;
+    s_slot0[threadIdx.x] = s0;
     if (i < S) {
-      p0 = cpre + opre;
-      d0 = cdec + odec;
-      s0 = cpart + opart;
       if (p0 + npre > v.max_pre || d0 + ndec > v.max_dec || i >= v.max_seqs ||
           s0 + npart > v.max_pre_part) {
         atomicOr(&s_bad, HY_ERR_PLAN);
       } else {
         v.seqinfo[i] = make_int2(d0, ns);
-        wr = true;
+        v.dec_blocks[i] = s_cblk + sums[BLK];
+        for (int g = 0; g < kv_heads; ++g) v.counters[i * kv_heads + g] = 0;
       }
     }
-    // The warp writes the items of its sequences together, one sequence at a
-    // time (item k of a sequence: head k / n, split or tile k % n).
-    const int lane = threadIdx.x & 31;
-    unsigned todo = __ballot_sync(0xffffffffu, wr);
-    while (todo) {
-      const int j = __ffs(todo) - 1;
-      todo &= todo - 1;
-      const int ji = __shfl_sync(0xffffffffu, i, j);
-      const int jp0 = __shfl_sync(0xffffffffu, p0, j), jd0 = __shfl_sync(0xffffffffu, d0, j);
-      const int jns = __shfl_sync(0xffffffffu, ns, j), jnb = __shfl_sync(0xffffffffu, nblk, j);
-      const int jrow = __shfl_sync(0xffffffffu, row, j), jkv = __shfl_sync(0xffffffffu, kv, j);
-      const int jnt = __shfl_sync(0xffffffffu, ntile, j), jq = __shfl_sync(0xffffffffu, q, j);
-      const int jph = __shfl_sync(0xffffffffu, ph, j), jpsl = __shfl_sync(0xffffffffu, psl, j);
-      const int js0 = __shfl_sync(0xffffffffu, s0, j);
-      for (int k = lane; k < kv_heads * jns; k += 32) {   // splits differ by at most one block
-        const int g = k / jns, sp = k - g * jns;
+    __syncthreads();                            // the offsets, and whether everything fits
+    if (s_bad == 0) {
+      // decode item k: KV head and split of the sequence it falls into (splits differ
+      // by at most one block)
+      for (int k = threadIdx.x; k < total[DEC]; k += PLAN_THREADS) {
+        const int j = plan_find(s_first_dec, k), ji = base + j, kj = k - s_first_dec[j];
+        const int jrow = cu_q[ji], jkv = seq_lens_k[ji];
+        const int jnb = (jkv + HY_BLOCK - 1) / HY_BLOCK;
+        const int jns = group ? max(1, min(ATT_WARPS, jnb)) : (jnb + split - 1) / split;
+        const int g = kj / jns, sp = kj - g * jns;
         const int lo = mul_div(sp, jnb, jns), hi = mul_div(sp + 1, jnb, jns);
-        v.dec[2 * (jd0 + k)] = make_int4(ji, g, lo, hi);
-        v.dec[2 * (jd0 + k) + 1] = make_int4(jrow, jkv, jns, jd0 + g * jns);
-        v.dec_ids[2 * (jd0 + k)] = make_int4(-1, 0, 0, 0);
+        v.dec[2 * (cdec + k)] = make_int4(ji, g, lo, hi);
+        v.dec[2 * (cdec + k) + 1] = make_int4(jrow, jkv, jns, cdec + k - sp);
+        v.dec_ids[2 * (cdec + k)] = make_int4(-1, 0, 0, 0);
       }
       // (KV head g, query tile t): its pieces follow those of head g's earlier
       // query tiles; a cut item's pieces take consecutive partial slots
-      for (int k = lane; k < kv_heads * jnt; k += 32) {
-        const int g = k / jnt, t = k - g * jnt;
-        int pos = jp0 + g * jph, slot = js0 + g * jpsl;
-        for (int u = 0; u < t; ++u) {
-          const int n = pre_pieces(pre_item_tiles(jkv, jq, u * PRE_QROWS), cap);
-          pos += n;
-          if (n > 1) slot += n;
+      for (int k = threadIdx.x; k < total[UNIT]; k += PLAN_THREADS) {
+        const int j = plan_find(s_first_unit, k), ji = base + j, kj = k - s_first_unit[j];
+        const int jq = cu_q[ji + 1] - cu_q[ji], jkv = seq_lens_k[ji];
+        const int jnt = (jq + PRE_QROWS - 1) / PRE_QROWS;
+        const int g = kj / jnt, t = kj - g * jnt;
+        int before = 0, slots = 0, jph = 0, jpsl = 0;
+        for (int u = 0; u < jnt; ++u) {
+          const int n = cap == 0x7fffffff ? 1 : pre_pieces(pre_item_tiles(jkv, jq, u * PRE_QROWS), cap);
+          if (u == t) { before = jph; slots = jpsl; }
+          jph += n;
+          if (n > 1) jpsl += n;
         }
+        const int pos = s_pre0[j] + g * jph + before, slot = s_slot0[j] + g * jpsl + slots;
         const int n = pre_pieces(pre_item_tiles(jkv, jq, t * PRE_QROWS), cap);
         for (int sp = 0; sp < n; ++sp)
           v.pre[pos + sp] = make_int4(ji, g, t * PRE_QROWS, n > 1 ? pre_piece_code(n, sp, slot) : 0);
         if (n > 1) v.pre_ctr[slot] = 0;
       }
     }
-    __syncthreads();
-    if (threadIdx.x == 0) { s_cpre += tpre; s_cdec += tdec; s_cpart += tpart; s_cblk += tblk; }
+    if (threadIdx.x == 0) {
+      s_cpre += total[PRE];
+      s_cdec += total[DEC];
+      s_cpart += total[PART];
+      s_cblk += total[BLK];
+    }
     __syncthreads();
   }
   if (threadIdx.x < 64 * GRAB_INTS) v.grab[threadIdx.x] = 0;
@@ -343,24 +393,26 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
   __syncthreads();                              // the items above are written
   const int np = s_bad ? 0 : min(s_cpre, v.max_pre);
   __shared__ int bins[PLAN_THREADS];
-  auto cost_bin = [&](int4 it) {                // bin 0 = most key tiles
-    const int q = cu_q[it.x + 1] - cu_q[it.x], kv = seq_lens_k[it.x];
-    int lo, hi;
-    pre_piece_range(it.w, pre_item_tiles(kv, q, it.z), lo, hi);
-    return PLAN_THREADS - 1 - min(max(hi - lo, 0), PLAN_THREADS - 1);
-  };
-  bins[threadIdx.x] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < np; i += PLAN_THREADS) atomicAdd(&bins[cost_bin(v.pre[i])], 1);
-  __syncthreads();
-  int nbin_total;
-  const int start = plan_scan(bins[threadIdx.x], ws, nbin_total);
-  __syncthreads();
-  bins[threadIdx.x] = start;
-  __syncthreads();
-  for (int i = threadIdx.x; i < np; i += PLAN_THREADS) {
-    const int4 it = v.pre[i];
-    v.pre_sorted[atomicAdd(&bins[cost_bin(it)], 1)] = it;
+  if (np > 0) {                                 // uniform
+    auto cost_bin = [&](int4 it) {                // bin 0 = most key tiles
+      const int q = cu_q[it.x + 1] - cu_q[it.x], kv = seq_lens_k[it.x];
+      int lo, hi;
+      pre_piece_range(it.w, pre_item_tiles(kv, q, it.z), lo, hi);
+      return PLAN_THREADS - 1 - min(max(hi - lo, 0), PLAN_THREADS - 1);
+    };
+    bins[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < np; i += PLAN_THREADS) atomicAdd(&bins[cost_bin(v.pre[i])], 1);
+    __syncthreads();
+    int nbin_total;
+    const int start = plan_scan(bins[threadIdx.x], ws, nbin_total);
+    __syncthreads();
+    bins[threadIdx.x] = start;
+    __syncthreads();
+    for (int i = threadIdx.x; i < np; i += PLAN_THREADS) {
+      const int4 it = v.pre[i];
+      v.pre_sorted[atomicAdd(&bins[cost_bin(it)], 1)] = it;
+    }
   }
   if (threadIdx.x == 0) {
     const bool bad = s_bad != 0;
