@@ -67,12 +67,18 @@ struct Args {
   int32_t* err;
 };
 
+// What a warp leaves of a pair that it did not finish alone.
+struct Part {
+  int pair;               // sequence * kv_heads + head, -1: none
+  int blocks, nb;         // blocks that it covers, blocks of the pair
+  int tok;                // query row
+};
+
 struct Shared {
   uint64_t bar[NW][NS];
   int unit;               // the CTA's next unit of decode work
   int last;               // bit j: this CTA finished pair j of its two open ones
-  int part_pair[NW][2];   // each warp's partials in block order: sequence * kv_heads + head
-  int part_blocks[NW][2]; // (-1: none), and the blocks they cover
+  Part part[2 * NW];      // each warp's two parts, in block order
   // prefill; ring barriers complete once per use of their slot, the others once
   // per key tile (per use of their S buffer), qfull once per item
   uint64_t full[PS];      // K and V of a tile expanded (one arrival per expanding warp)
@@ -107,34 +113,38 @@ HY_DEVICE void q4_bits(uint32_t w, uint32_t (&x)[4]) {
 }
 
 // A place in the flattened list of key blocks (sequence, head, block) of the step's
-// decode sequences, with what a load from there needs.
+// decode sequences, with what a warp needs of the sequence.
 struct Cursor {
   int seq, g, b, nb;                                      // block b of nb
+  int tok, kv_len;                                        // query row, key length
   const int32_t* bt;
-  int wbase, ids;                                         // lane i holds block wbase + i's id
 };
 HY_DEVICE void cursor_sequence(const Args& a, const PlanView& v, Cursor& k) {
-  k.nb = v.dec_blocks[k.seq + 1] - v.dec_blocks[k.seq];
+  k.tok = a.cu_q[k.seq];
+  k.kv_len = a.seq_lens_k[k.seq];
+  k.nb = (k.kv_len + HY_BLOCK - 1) / HY_BLOCK;            // as the plan counts them
   k.bt = a.block_tables + (size_t)(a.seq_bt_row ? a.seq_bt_row[k.seq] : k.seq) * a.bt_pitch;
-  k.wbase = -64;
 }
-// The place of flattened block f: the last sequence that starts at or before it, found
-// by the whole warp 32 sequences (or runs of 32^n) at a time.
-HY_DEVICE Cursor cursor_at(const Args& a, const PlanView& v, long f) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, step = 1;
-  while ((long)step * 32 < a.num_seqs) step *= 32;
-  for (; step >= 1; step >>= 5) {
-    const long i = lo + (long)lane * step;
-    const bool le = i < a.num_seqs && (long)v.dec_blocks[i] * a.kv_heads <= f;
-    lo += (31 - __clz(__ballot_sync(0xffffffffu, le) | 1u)) * step;
-  }
+// The place of flattened block f: in sequence seq (>= 0), or in the last sequence that
+// starts at or before f, found by the whole warp 32 sequences (or runs of 32^n) at a time.
+HY_DEVICE Cursor cursor_at(const Args& a, const PlanView& v, int seq, long f) {
   Cursor k;
-  k.seq = lo;
+  k.seq = seq;
+  if (seq < 0) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, step = 1;
+    while ((long)step * 32 < a.num_seqs) step *= 32;
+    for (; step >= 1; step >>= 5) {
+      const long i = lo + (long)lane * step;
+      const bool le = i < a.num_seqs && (long)v.dec_blocks[i] * a.kv_heads <= f;
+      lo += (31 - __clz(__ballot_sync(0xffffffffu, le) | 1u)) * step;
+    }
+    k.seq = lo;
+  }
   cursor_sequence(a, v, k);
-  const long in = f - (long)v.dec_blocks[lo] * a.kv_heads;
-  k.g = (int)(in / k.nb);
-  k.b = (int)(in - (long)k.g * k.nb);
+  const int in = (int)(f - (long)v.dec_blocks[k.seq] * a.kv_heads);
+  k.g = in / k.nb;
+  k.b = in - k.g * k.nb;
   return k;
 }
 // Step to the next (sequence, head) once all blocks of this one are passed.
@@ -147,14 +157,6 @@ HY_DEVICE void cursor_next_pair(const Args& a, const PlanView& v, Cursor& k) {
   } while (v.dec_blocks[k.seq + 1] == v.dec_blocks[k.seq]);
   cursor_sequence(a, v, k);
 }
-
-// One warp's running state over a (sequence, head); see decode_warp.
-struct DecState {
-  float o[8][4];          // O^T fragments, in units of 2^-24 vs (odd m-tiles 2^-20 vs)
-  float z[2][2];          // [half][k]: this lane's sum of p times V's minimum
-  float m[2], l[2];       // running maximum (log2 units), this lane's part of the sum
-  float vs, vcap;         // 2^k that V's scales are multiplied by, and the largest scale it fits
-};
 
 // One warp: key blocks [f0, f1) of the flattened list, pair by pair.
 //
@@ -171,49 +173,78 @@ struct DecState {
 // is only raised when a score exceeds it by more than that, so that most blocks need
 // no exchange between lanes), scale_V 2^k at most 2^7.
 // Lane (r, c) = (lane / 4, lane % 4) with c < 2 ends with heads 2 c + k (k = 0, 1) at
-// dimensions 8 r + i and 64 + 8 r + i.  Returns false if a wait ran out.
-__device__ bool decode_warp(const Args& a, const PlanView& v, long f0, long f1, uint8_t* ring,
-                            float* part, int (&part_pair)[2], int (&part_blocks)[2],
-                            uint64_t* bars, uint32_t& ring_ctr) {
+// dimensions 8 r + i and 64 + 8 r + i.  ring: shared-memory address of the warp's ring,
+// ring_pos its next slot, ring_par the parity of its next pass.  Returns false if a
+// wait ran out.
+HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, long f0, long f1,
+                           uint8_t* ring_ptr, float* part, Part* parts, uint64_t* bars,
+                           uint32_t& ring_pos, uint32_t& ring_par) {
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   if (f0 >= f1) return true;
-  Cursor ld = cursor_at(a, v, f0);                        // the next block to load
-  Cursor k = ld;                                          // the pair being computed
-  int left_to_load = (int)(f1 - f0), left = left_to_load;
-  uint32_t put = ring_ctr, get = ring_ctr;                // ring slots used so far
+  const uint32_t ring = smem_u32(ring_ptr);
+  Cursor k = cursor_at(a, v, seq, f0);                    // the pair being computed
+  Cursor ld = k;                                          // the next block to load
+  int to_load = (int)(f1 - f0), left = to_load;
+  const __nv_bfloat16* q0 = a.q + (size_t)r * HY_HEAD_DIM + 16 * c;      // this lane's part of Q
+  uint4 qraw[4];
+  auto load_q = [&]() {
+    const __nv_bfloat16* qp = q0 + ((size_t)k.tok * a.q_heads + k.g * HY_GROUP) * HY_HEAD_DIM;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      qraw[i] = r < HY_GROUP ? *reinterpret_cast<const uint4*>(qp + 64 * (i >> 1) + 8 * (i & 1))
+                             : make_uint4(0, 0, 0, 0);
+  };
+  load_q();
+
+  // Loads: the ids of the next blocks of a pair, up to 32, are held one per lane as the
+  // address of the block's tiles, and each lane issues its own block's copy in turn.
+  const uint8_t* src = nullptr;
+  int turn = 0, run = 0;                                  // lane whose block is next, blocks held
+  uint32_t put = ring_pos;
   auto issue = [&]() {
-    if (left_to_load <= 0) return;
-    --left_to_load;
-    if (ld.b == ld.nb) cursor_next_pair(a, v, ld);
-    if ((unsigned)(ld.b - ld.wbase) >= 32u) {
-      ld.wbase = ld.b;
-      ld.ids = ld.b + lane < ld.nb && ld.b + lane < a.bt_pitch ? __ldg(ld.bt + ld.b + lane) : -1;
-    }
-    int blk = __shfl_sync(0xffffffffu, ld.ids, ld.b - ld.wbase);
-    if (lane == 0) {
+    if (to_load == 0) return;
+    if (run == 0) {
+      if (ld.b == ld.nb) cursor_next_pair(a, v, ld);
+      turn = 0;
+      run = min(32, ld.nb - ld.b);
+      int blk = lane < run && ld.b + lane < a.bt_pitch ? __ldg(ld.bt + ld.b + lane) : -1;
       if (blk < 0 || blk >= a.num_blocks) {
-        hy_flag(a.err, HY_ERR_BOUNDS);
+        if (lane < min(run, to_load)) hy_flag(a.err, HY_ERR_BOUNDS);
         blk = 0;
       }
-      const uint32_t s = put % NS;
-      fence_proxy_async();
-      mbar_arrive_expect_tx(&bars[s], BLK_BYTES);
-      bulk_load(ring + s * BLK_BYTES, a.cache + q4_tile(blk, ld.g, 0, a.kv_heads), BLK_BYTES,
-                &bars[s]);
+      src = a.cache + q4_tile(blk, ld.g, 0, a.kv_heads);
+      ld.b += run;
     }
-    ++ld.b;
-    ++put;
+    if (lane == turn) {
+      fence_proxy_async();
+      mbar_arrive_expect_tx(&bars[put], BLK_BYTES);
+      bulk_load(ring_ptr + put * BLK_BYTES, src, BLK_BYTES, &bars[put]);
+    }
+    ++turn;
+    --run;
+    --to_load;
+    put = put + 1 == NS ? 0 : put + 1;
   };
 #pragma unroll 1
   for (int j = 0; j < NS; ++j) issue();
 
-  const int keyA = key_of(r >> 1, r & 1, 0), keyB = keyA | 4;            // this lane's score rows
+  // shared-memory offsets of this lane inside a block's tiles: its two K rows (keyB is
+  // keyA + 4) and the first of its four V keys of either kind
+  const int keyA = key_of(r >> 1, r & 1, 0);
+  const uint32_t k_off = keyA * Q4_ROW_BYTES + 8 * c, p_off = Q4_PARAM_OFF + keyA * Q4_PARAM_BYTES;
+  const uint32_t v_off0 = Q4_TILE_BYTES + key_of(c, 0, 0) * Q4_ROW_BYTES + 4 * r;
+  const uint32_t v_off1 = Q4_TILE_BYTES + key_of(c, 1, 0) * Q4_ROW_BYTES + 4 * r;
+  constexpr uint32_t ROW4 = 4 * Q4_ROW_BYTES, PAR4 = 4 * Q4_PARAM_BYTES;  // four keys on
+  uint32_t get = ring_pos, par = ring_par;
   bool ok = true, first_pair = true;
+  int pending = 0;
 #pragma unroll 1
-  while (left > 0 && ok) {
+  while (left > 0) {
     const int n = min(left, k.nb - k.b), b_first = k.b;   // this pair's blocks in the range
     left -= n;
-    const int tok = a.cu_q[k.seq], kv_len = a.seq_lens_k[k.seq];
+    // the last block, if it is here and partial, and its keys
+    const int tail = b_first + n == k.nb && (k.kv_len & (HY_BLOCK - 1)) ? n - 1 : -1;
+    const int rest = k.kv_len & (HY_BLOCK - 1);
     // Q in fp16 (q4_query_scale): lane (r, c) holds head r's words 2 c, 2 c + 1 (dimensions
     // 16 c ..) of both halves; rows 4-7 are zero.  Codes in bits 0-3 meet 2^14 q, codes
     // in bits 4-7 2^10 q, so that a score comes out as 2^-10 code . q.
@@ -221,12 +252,9 @@ __device__ bool decode_warp(const Args& a, const PlanView& v, long f0, long f1, 
     float qs[2][2], mult[2];                              // sums of q of heads 2 c + k, scale
     {
       float x[32], amax = 0.f, down, up;
-      const __nv_bfloat16* qp = a.q + ((size_t)tok * a.q_heads + k.g * HY_GROUP + r) * HY_HEAD_DIM + 16 * c;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint4 u = r < HY_GROUP ? *reinterpret_cast<const uint4*>(qp + 64 * (i >> 1) + 8 * (i & 1))
-                                     : make_uint4(0, 0, 0, 0);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        const uint32_t w[4] = {qraw[i].x, qraw[i].y, qraw[i].z, qraw[i].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           x[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
@@ -234,7 +262,7 @@ __device__ bool decode_warp(const Args& a, const PlanView& v, long f0, long f1, 
         }
       }
 #pragma unroll
-      for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(x[i]));
+      for (int i = 0; i < 16; ++i) amax = fmax3f(amax, fabsf(x[2 * i]), fabsf(x[2 * i + 1]));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       q4_query_scale(amax, down, up);
@@ -259,33 +287,30 @@ __device__ bool decode_warp(const Args& a, const PlanView& v, long f0, long f1, 
       mult[0] = a.scale_log2 * (1024.f * __shfl_sync(0xffffffffu, up, 8 * c));
       mult[1] = a.scale_log2 * (1024.f * __shfl_sync(0xffffffffu, up, 8 * c + 4));
     }
-    DecState t;
+    float o[8][4];                                        // O^T, in 2^-24 vs (odd m-tiles 2^-20 vs)
+    float z[2][2] = {{0.f, 0.f}, {0.f, 0.f}};             // [half][k]: sum of p times V's minimum
+    float m[2] = {-INFINITY, -INFINITY};                  // running maximum (log2 units)
+    float ms[2] = {0.f, 0.f};                             // the same, 0 while it is -inf
+    float l[2] = {0.f, 0.f};                              // this lane's part of the sum
+    float vs = 1.f, vcap = -1.f;                          // 2^k, the largest scale that it fits
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t.o[j][0] = t.o[j][1] = t.o[j][2] = t.o[j][3] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      t.z[i][0] = t.z[i][1] = 0.f;
-      t.m[i] = -INFINITY;
-      t.l[i] = 0.f;
-    }
-    t.vs = 1.f;
-    t.vcap = -1.f;                                        // the first block sets them
+    for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
-      const uint32_t s = get % NS;
-      const bool w_ok = mbar_wait(&bars[s], (get / NS) & 1u, a.err);
-      if (__any_sync(0xffffffffu, !w_ok)) { ok = false; break; }
-      ++get;
-      const uint8_t* kt = ring + s * BLK_BYTES;
-      const uint8_t* vt = kt + Q4_TILE_BYTES;
+      if (!__all_sync(0xffffffffu, mbar_try_wait(&bars[get], par)) &&
+          !__all_sync(0xffffffffu, mbar_wait(&bars[get], par, a.err))) {
+        ok = false;
+        pending = left + n - i - to_load;                 // copies not waited for
+        break;
+      }
+      const uint32_t st = ring + get * BLK_BYTES;
 
       // S^T = K Q^T, one accumulator per half of the dimensions
       float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const uint2 wa = *reinterpret_cast<const uint2*>(kt + keyA * Q4_ROW_BYTES + 32 * hf + 8 * c);
-        const uint2 wb = *reinterpret_cast<const uint2*>(kt + keyB * Q4_ROW_BYTES + 32 * hf + 8 * c);
+        const uint2 wa = lds64(st + k_off + 32 * hf), wb = lds64(st + k_off + 32 * hf + ROW4);
         uint32_t xa[4], xb[4];
         q4_bits(wa.x, xa);
         q4_bits(wb.x, xb);
@@ -296,10 +321,9 @@ __device__ bool decode_warp(const Args& a, const PlanView& v, long f0, long f1, 
         mma_f16_16816(sc[hf], xa[0], xb[0], xa[1], xb[1], qb[hf][1][0], qb[hf][1][1]);
         mma_f16_16816(sc[hf], xa[2], xb[2], xa[3], xb[3], qb[hf][1][2], qb[hf][1][3]);
       }
-      float x[4], sv[2][2], mv[2][2];                     // scores; V's scales and minima [row][half]
+      float x[4];                                         // scores of (keyA, keyB) x 2 heads
       {
-        const uint2 pa = *reinterpret_cast<const uint2*>(kt + Q4_PARAM_OFF + keyA * Q4_PARAM_BYTES);
-        const uint2 pb = *reinterpret_cast<const uint2*>(kt + Q4_PARAM_OFF + keyB * Q4_PARAM_BYTES);
+        const uint2 pa = lds64(st + p_off), pb = lds64(st + p_off + PAR4);
         const float2 a0 = __half22float2(q4_as_half2(pa.x)), a1 = __half22float2(q4_as_half2(pa.y));
         const float2 b0 = __half22float2(q4_as_half2(pb.x)), b1 = __half22float2(q4_as_half2(pb.y));
 #pragma unroll
@@ -307,83 +331,81 @@ __device__ bool decode_warp(const Args& a, const PlanView& v, long f0, long f1, 
           x[e] = mult[e] * fmaf(a0.x, sc[0][e], fmaf(a1.x, sc[1][e], fmaf(a0.y, qs[0][e], a1.y * qs[1][e])));
           x[2 + e] = mult[e] * fmaf(b0.x, sc[0][2 + e], fmaf(b1.x, sc[1][2 + e], fmaf(b0.y, qs[0][e], b1.y * qs[1][e])));
         }
-        uint2 va = *reinterpret_cast<const uint2*>(vt + Q4_PARAM_OFF + keyA * Q4_PARAM_BYTES);
-        uint2 vb = *reinterpret_cast<const uint2*>(vt + Q4_PARAM_OFF + keyB * Q4_PARAM_BYTES);
-        const int rest = kv_len - (b_first + i) * HY_BLOCK;
-        if (rest < HY_BLOCK) {                            // the last block: rows past the end hold anything
-          if (keyA >= rest) { x[0] = x[1] = -INFINITY; va = make_uint2(0u, 0u); }
-          if (keyB >= rest) { x[2] = x[3] = -INFINITY; vb = make_uint2(0u, 0u); }
-        }
-        const float2 c0 = __half22float2(q4_as_half2(va.x)), c1 = __half22float2(q4_as_half2(va.y));
-        const float2 d0 = __half22float2(q4_as_half2(vb.x)), d1 = __half22float2(q4_as_half2(vb.y));
-        sv[0][0] = c0.x; sv[0][1] = c1.x; sv[1][0] = d0.x; sv[1][1] = d1.x;
-        mv[0][0] = c0.y; mv[0][1] = c1.y; mv[1][0] = d0.y; mv[1][1] = d1.y;
       }
+      uint2 va = lds64(st + p_off + Q4_TILE_BYTES), vb = lds64(st + p_off + Q4_TILE_BYTES + PAR4);
+      if (i == tail) {                                    // rows past the end hold anything
+        if (keyA >= rest) { x[0] = x[1] = -INFINITY; va = make_uint2(0u, 0u); }
+        if (keyA + 4 >= rest) { x[2] = x[3] = -INFINITY; vb = make_uint2(0u, 0u); }
+      }
+      // V's (scale, minimum) of (keyA, keyB) x half
+      const float2 va0 = __half22float2(q4_as_half2(va.x)), va1 = __half22float2(q4_as_half2(va.y));
+      const float2 vb0 = __half22float2(q4_as_half2(vb.x)), vb1 = __half22float2(q4_as_half2(vb.y));
       float mx[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
-      float smax = fmax3f(sv[0][0], sv[0][1], fmaxf(sv[1][0], sv[1][1]));
-      const bool grow = mx[0] > t.m[0] + RESCALE_LOG2 || mx[1] > t.m[1] + RESCALE_LOG2 || smax > t.vcap;
+      float smax = fmaxf(fmax3f(va0.x, va1.x, vb0.x), vb1.x);
+      const bool grow = mx[0] > m[0] + RESCALE_LOG2 || mx[1] > m[1] + RESCALE_LOG2 || smax > vcap;
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, d));
         float vr = 1.f;                                   // change of vs
-        if (smax > t.vcap) {                              // 2^(6 - exponent), for scales of 2^-24 and up
+        if (smax > vcap) {                                // 2^(6 - exponent), for scales of 2^-24 and up
           const int e = min(max((__float_as_int(smax) >> 23) & 255, 103), 254) - 127;
-          const float vs = __int_as_float((6 - e + 127) << 23);
-          vr = t.vcap < 0.f ? 1.f : vs / t.vs;
-          t.vs = vs;
-          t.vcap = __int_as_float((e + 127) << 23) * 1.9990234375f;   // the largest fp16 below 2^(e + 1)
+          const float vs_new = __int_as_float((6 - e + 127) << 23);
+          vr = vcap < 0.f ? 1.f : vs_new / vs;
+          vs = vs_new;
+          vcap = __int_as_float((e + 127) << 23) * 1.9990234375f;       // the largest fp16 below 2^(e + 1)
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], d));
-          const float m_new = fmaxf(t.m[e], mx[e]);
-          const float alpha = m_new == -INFINITY ? 1.f : ex2_ftz(t.m[e] - m_new);
-          t.m[e] = m_new;
-          t.l[e] *= alpha;
-          t.z[0][e] *= alpha;
-          t.z[1][e] *= alpha;
+          const float m_new = fmaxf(m[e], mx[e]);
+          const float alpha = m_new == -INFINITY ? 1.f : ex2_ftz(m[e] - m_new);
+          m[e] = m_new;
+          ms[e] = m_new == -INFINITY ? 0.f : m_new;
+          l[e] *= alpha;
+          z[0][e] *= alpha;
+          z[1][e] *= alpha;
           const float ao = alpha * vr;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) { t.o[j][e] *= ao; t.o[j][2 + e] *= ao; }
+          for (int j = 0; j < 8; ++j) { o[j][e] *= ao; o[j][2 + e] *= ao; }
         }
       }
-      const float m0 = t.m[0] == -INFINITY ? 0.f : t.m[0], m1 = t.m[1] == -INFINITY ? 0.f : t.m[1];
-      x[0] = ex2_ftz(x[0] - m0);
-      x[1] = ex2_ftz(x[1] - m1);
-      x[2] = ex2_ftz(x[2] - m0);
-      x[3] = ex2_ftz(x[3] - m1);
-      t.l[0] += x[0] + x[2];
-      t.l[1] += x[1] + x[3];
-      uint32_t pb[2][2];                                  // P^T operands [half][keys 0-7, 8-15]
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = ex2_ftz(x[e] - ms[e & 1]);
+      l[0] += x[0] + x[2];
+      l[1] += x[1] + x[3];
+      uint32_t pt[2][2];                                  // P^T operands [half][keys 0-7, 8-15]
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const float wa = sv[0][hf] * t.vs, wb = sv[1][hf] * t.vs;
-        pb[hf][0] = movmatrix_trans(q4_as_u32(__floats2half2_rn(x[0] * wa, x[1] * wa)));
-        pb[hf][1] = movmatrix_trans(q4_as_u32(__floats2half2_rn(x[2] * wb, x[3] * wb)));
-        t.z[hf][0] = fmaf(x[0], mv[0][hf], fmaf(x[2], mv[1][hf], t.z[hf][0]));
-        t.z[hf][1] = fmaf(x[1], mv[0][hf], fmaf(x[3], mv[1][hf], t.z[hf][1]));
+        const float2 ua = hf ? va1 : va0, ub = hf ? vb1 : vb0;
+        const float wa = ua.x * vs, wb = ub.x * vs;
+        pt[hf][0] = movmatrix_trans(q4_as_u32(__floats2half2_rn(x[0] * wa, x[1] * wa)));
+        pt[hf][1] = movmatrix_trans(q4_as_u32(__floats2half2_rn(x[2] * wb, x[3] * wb)));
+        z[hf][0] = fmaf(x[0], ua.y, fmaf(x[2], ub.y, z[hf][0]));
+        z[hf][1] = fmaf(x[1], ua.y, fmaf(x[3], ub.y, z[hf][1]));
       }
-      // O^T += V^T (scale P)^T, a half of the dimensions per product: rows r / r + 8 of m-tile
-      // (hf, e, j) are nibble 4 e + j of words r / ... of the half: its word r holds
-      // dimensions 8 r .. 8 r + 7, one per m-tile, so both row groups come from it
+      // O^T += V^T (scale P)^T, a half of the dimensions per product: the lane's word r of
+      // four keys holds dimensions 8 r .. 8 r + 7; nibbles of equal weight share an m-tile
+      // (rows 0-7 nibble j, rows 8-15 nibble j + 2)
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         uint32_t y[2][2][4];                              // [keys 0-7, 8-15][low, high nibbles]
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(vt + key_of(c, 0, h) * Q4_ROW_BYTES + 32 * hf + 4 * r);
-          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(vt + key_of(c, 1, h) * Q4_ROW_BYTES + 32 * hf + 4 * r);
+          const uint32_t w0 = lds32(st + v_off0 + 32 * hf + ROW4 * h), w1 = lds32(st + v_off1 + 32 * hf + ROW4 * h);
           q4_bits(__byte_perm(w0, w1, 0x5410), y[h][0]);
           q4_bits(__byte_perm(w0, w1, 0x7632), y[h][1]);
         }
-        // two nibbles of equal weight share an m-tile: rows 0-7 nibble j, rows 8-15 nibble j + 2
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            mma_f16_16816(t.o[4 * hf + 2 * e + j], y[0][e][j], y[0][e][j + 2], y[1][e][j], y[1][e][j + 2],
-                          pb[hf][0], pb[hf][1]);
+            mma_f16_16816(o[4 * hf + 2 * e + j], y[0][e][j], y[0][e][j + 2], y[1][e][j], y[1][e][j + 2],
+                          pt[hf][0], pt[hf][1]);
+      }
+      if (++get == NS) {
+        get = 0;
+        par ^= 1u;
       }
       __syncwarp();                                       // the stage is read
       issue();
@@ -398,13 +420,13 @@ __device__ bool decode_warp(const Args& a, const PlanView& v, long f0, long f1, 
     for (int e = 0; e < 2; ++e) {
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) {
-        t.l[e] += __shfl_xor_sync(0xffffffffu, t.l[e], d);
-        t.z[0][e] += __shfl_xor_sync(0xffffffffu, t.z[0][e], d);
-        t.z[1][e] += __shfl_xor_sync(0xffffffffu, t.z[1][e], d);
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
+        z[0][e] += __shfl_xor_sync(0xffffffffu, z[0][e], d);
+        z[1][e] += __shfl_xor_sync(0xffffffffu, z[1][e], d);
       }
-      inv[e] = whole ? 1.f / t.l[e] : 1.f;
+      inv[e] = whole ? 1.f / l[e] : 1.f;
     }
-    const float unit0 = 0x1p24f / t.vs, unit1 = 0x1p20f / t.vs;   // m-tiles of bits 0-3, 4-7
+    const float unit0 = 0x1p24f / vs, unit1 = 0x1p20f / vs;       // m-tiles of bits 0-3, 4-7
     if (c < 2) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
@@ -414,12 +436,12 @@ __device__ bool decode_warp(const Args& a, const PlanView& v, long f0, long f1, 
           float y[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float u = t.o[4 * hf + 2 * (i >> 2) + (i & 1)][2 * ((i & 3) >> 1) + e];
-            y[i < 4 ? 2 * i : 2 * (i - 4) + 1] = fmaf(u, (i & 1) ? unit1 : unit0, t.z[hf][e]) * inv[e];
+            const float u = o[4 * hf + 2 * (i >> 2) + (i & 1)][2 * ((i & 3) >> 1) + e];
+            y[i < 4 ? 2 * i : 2 * (i - 4) + 1] = fmaf(u, (i & 1) ? unit1 : unit0, z[hf][e]) * inv[e];
           }
           const int at = (2 * c + e) * HY_HEAD_DIM + 64 * hf + 8 * r;
           if (whole) {
-            *reinterpret_cast<uint4*>(a.out + ((size_t)tok * a.q_heads + k.g * HY_GROUP) * HY_HEAD_DIM + at) =
+            *reinterpret_cast<uint4*>(a.out + ((size_t)k.tok * a.q_heads + k.g * HY_GROUP) * HY_HEAD_DIM + at) =
                 make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]),
                            pack_bf16(y[6], y[7]));
           } else {
@@ -432,19 +454,27 @@ __device__ bool decode_warp(const Args& a, const PlanView& v, long f0, long f1, 
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           *reinterpret_cast<float2*>(part + slot * PART_FLOATS + HY_GROUP * HY_HEAD_DIM + 2 * (2 * c + e)) =
-              make_float2(t.m[e], t.l[e]);
+              make_float2(m[e], l[e]);
     }
-    if (!whole && lane == 0) {
-      part_pair[slot] = k.seq * a.kv_heads + k.g;
-      part_blocks[slot] = n;
-    }
+    if (!whole && lane == 0) parts[slot] = Part{k.seq * a.kv_heads + k.g, n, k.nb, k.tok};
     first_pair = false;
     k.b += n;
-    if (left > 0) cursor_next_pair(a, v, k);
+    if (left > 0) {
+      cursor_next_pair(a, v, k);
+      load_q();
+    }
   }
-  ring_ctr = put;
-  if (!ok)                                                // copies in flight land before the CTA exits
-    for (uint32_t j = get; j < put; ++j) mbar_wait(&bars[j % NS], (j / NS) & 1u, nullptr);
+  if (!ok) {                                              // copies in flight land before the CTA exits
+    for (; pending > 0; --pending) {
+      mbar_wait(&bars[get], par, nullptr);
+      if (++get == NS) {
+        get = 0;
+        par ^= 1u;
+      }
+    }
+  }
+  ring_pos = get;
+  ring_par = par;
   return ok;
 }
 
@@ -454,58 +484,75 @@ __device__ bool decode_warp(const Args& a, const PlanView& v, long f0, long f1, 
 // partial in the workspace (slot 2 unit, or 2 unit + 1 where the pair starts inside the
 // range), and the CTA whose count of blocks completes a pair joins its partials.
 // Returns false if a wait ran out.
-HY_DEVICE long unit_start(long total, int units, int u) { return total * u / units; }
+struct Units {            // `total` blocks in n units whose sizes differ by at most one
+  long total;
+  int n;
+  long size, more;        // the first `more` units have size + 1 blocks
+  HY_DEVICE Units(long t, int units) : total(t), n(units), size(t / units), more(t - size * units) {}
+  HY_DEVICE long start(int u) const { return u * size + min((long)u, more); }
+  HY_DEVICE int of(long f) const {                        // the unit that holds block f
+    return (int)(f < more * (size + 1) ? f / (size + 1) : more + (f - more * (size + 1)) / size);
+  }
+};
 
-__device__ bool decode_unit(const Args& a, const PlanView& v, long total, int units, int unit,
-                            long f0, long f1, uint8_t* payload, Shared& sh, uint32_t& ring_ctr) {
+HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units, int unit,
+                           int only_seq, long f0, long f1, uint8_t* payload, Shared& sh,
+                           uint32_t& ring_pos, uint32_t& ring_par) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  float* parts = reinterpret_cast<float*>(payload + NW * RING_BYTES);
-  if (lane < 2) sh.part_pair[warp][lane] = -1;
+  const float* parts = reinterpret_cast<const float*>(payload + NW * RING_BYTES);
+  if (lane < 2) sh.part[2 * warp + lane].pair = -1;
   __syncwarp();
-  const long n = f1 - f0;
-  const bool ok = decode_warp(a, v, f0 + n * warp / NW, f0 + n * (warp + 1) / NW,
-                              payload + warp * RING_BYTES, parts + warp * 2 * PART_FLOATS,
-                              sh.part_pair[warp], sh.part_blocks[warp], sh.bar[warp], ring_ctr);
+  const int n = (int)(f1 - f0);
+  const bool ok = decode_warp(a, v, only_seq, f0 + (long)n * warp / NW, f0 + (long)n * (warp + 1) / NW,
+                              payload + warp * RING_BYTES,
+                              const_cast<float*>(parts) + warp * 2 * PART_FLOATS,
+                              sh.part + 2 * warp, sh.bar[warp], ring_pos, ring_par);
   if (__syncthreads_or(!ok)) return false;
 
-  const int head = tid >> 7, d = tid & 127;
-  int open_pair[2], open_blocks[2], n_open = 0;
-  for (int i = 0; i < 2 * NW;) {
-    const int pair = sh.part_pair[i >> 1][i & 1];
-    if (pair < 0) { ++i; continue; }
-    int end = i, blocks = 0;
-    float M = -INFINITY;
-    for (; end < 2 * NW; ++end) {
-      const int p = sh.part_pair[end >> 1][end & 1];
-      if (p < 0) continue;
-      if (p != pair) break;
-      blocks += sh.part_blocks[end >> 1][end & 1];
-      M = fmaxf(M, parts[end * PART_FLOATS + HY_GROUP * HY_HEAD_DIM + 2 * head]);
+  // Lane j of every warp looks after part j: parts of one pair are neighbours (but for
+  // empty ones between them), so the first lane of each run leads it.
+  static_assert(2 * NW == 32, "one part per lane");
+  const int head = warp >> 2, d = tid & 127;              // a warp has one head
+  const Part mine = sh.part[lane];
+  const float2 ml = mine.pair < 0 ? make_float2(-INFINITY, 0.f)
+                                  : *reinterpret_cast<const float2*>(
+                                        parts + lane * PART_FLOATS + HY_GROUP * HY_HEAD_DIM + 2 * head);
+  unsigned todo = __ballot_sync(0xffffffffu, mine.pair >= 0);
+  int open_at[2], open_blocks[2], n_open = 0;             // pairs that reach out: first part, blocks here
+  while (todo) {
+    const int i = __ffs(todo) - 1;
+    const int pair = __shfl_sync(0xffffffffu, mine.pair, i);
+    const bool in = mine.pair == pair;
+    const unsigned group = __ballot_sync(0xffffffffu, in);
+    todo &= ~group;
+    float M = in ? ml.x : -INFINITY, L;
+    int blocks = in ? mine.blocks : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      blocks += __shfl_xor_sync(0xffffffffu, blocks, o);
     }
-    const float Mu = M == -INFINITY ? 0.f : M;
-    float L = 0.f, acc = 0.f;
-    for (int j = i; j < end; ++j) {
-      if (sh.part_pair[j >> 1][j & 1] < 0) continue;
-      const float* pw = parts + j * PART_FLOATS;
-      const float wt = ex2_ftz(pw[HY_GROUP * HY_HEAD_DIM + 2 * head] - Mu);
-      L = fmaf(wt, pw[HY_GROUP * HY_HEAD_DIM + 2 * head + 1], L);
-      acc = fmaf(wt, pw[tid], acc);
+    const float wt = in ? ex2_ftz(ml.x - (M == -INFINITY ? 0.f : M)) : 0.f;
+    L = wt * ml.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    float acc = 0.f;
+    for (unsigned g = group; g; g &= g - 1) {
+      const int j = __ffs(g) - 1;
+      acc = fmaf(__shfl_sync(0xffffffffu, wt, j), parts[j * PART_FLOATS + tid], acc);
     }
+    const int nb = __shfl_sync(0xffffffffu, mine.nb, i), tok = __shfl_sync(0xffffffffu, mine.tok, i);
     const int seq = pair / a.kv_heads, g = pair - seq * a.kv_heads;
-    const int p0 = v.dec_blocks[seq], nb = v.dec_blocks[seq + 1] - p0;
     if (blocks == nb) {
-      a.out[((size_t)a.cu_q[seq] * a.q_heads + g * HY_GROUP + head) * HY_HEAD_DIM + d] =
-          __float2bfloat16_rn(acc / L);
+      a.out[((size_t)tok * a.q_heads + g * HY_GROUP) * HY_HEAD_DIM + tid] = __float2bfloat16_rn(acc / L);
     } else {
-      const long F0 = (long)p0 * a.kv_heads + (long)g * nb;
-      const size_t slot = 2 * unit + (F0 > f0);
+      const size_t slot = 2 * unit + ((long)v.dec_blocks[seq] * a.kv_heads + (long)g * nb > f0);
       __stcg(v.part_o + slot * (HY_GROUP * HY_HEAD_DIM) + tid, acc);
       if (d == 0) __stcg(v.part_ml + slot * HY_GROUP + head, make_float2(M, L));
-      open_pair[n_open & 1] = pair;
+      open_at[n_open & 1] = i;
       open_blocks[n_open & 1] = blocks;
       ++n_open;
     }
-    i = end;
   }
   if (n_open == 0) {
     __syncthreads();                                      // parts are read
@@ -516,9 +563,9 @@ __device__ bool decode_unit(const Args& a, const PlanView& v, long total, int un
   if (tid == 0) {
     int last = 0;
     for (int j = 0; j < n_open; ++j) {
-      const int seq = open_pair[j] / a.kv_heads;
-      int* ctr = &v.counters[open_pair[j]];
-      if (atomicAdd(ctr, open_blocks[j]) + open_blocks[j] == v.dec_blocks[seq + 1] - v.dec_blocks[seq]) {
+      const Part& p = sh.part[open_at[j]];
+      int* ctr = &v.counters[p.pair];
+      if (atomicAdd(ctr, open_blocks[j]) + open_blocks[j] == p.nb) {
         last |= 1 << j;
         *ctr = 0;                                         // for the next launch on this plan
       }
@@ -530,30 +577,26 @@ __device__ bool decode_unit(const Args& a, const PlanView& v, long total, int un
   __threadfence();                                        // the others' partials, after the count
   for (int j = 0; j < n_open; ++j) {
     if (!((last >> j) & 1)) continue;
-    const int seq = open_pair[j] / a.kv_heads, g = open_pair[j] - seq * a.kv_heads;
-    const int p0 = v.dec_blocks[seq], nb = v.dec_blocks[seq + 1] - p0;
-    const long F0 = (long)p0 * a.kv_heads + (long)g * nb, F1 = F0 + nb;
-    int u0 = (int)(F0 * units / total);                   // the unit that holds block F0
-    while (unit_start(total, units, u0 + 1) <= F0) ++u0;
+    const Part p = sh.part[open_at[j]];
+    const int seq = p.pair / a.kv_heads, g = p.pair - seq * a.kv_heads;
+    const long F0 = (long)v.dec_blocks[seq] * a.kv_heads + (long)g * p.nb, F1 = F0 + p.nb;
+    const int u0 = units.of(F0), u1 = units.of(F1 - 1);
     float M = -INFINITY, L = 0.f, acc = 0.f;
 #pragma unroll 4
-    for (int u = u0; u < units; ++u) {
-      const long s0 = unit_start(total, units, u), s1 = unit_start(total, units, u + 1);
-      if (s0 >= F1) break;
-      if (s0 == s1) continue;
-      const size_t slot = 2 * u + (F0 > s0);
-      const float2 ml = __ldcg(v.part_ml + slot * HY_GROUP + head);
+    for (int u = u0; u <= u1; ++u) {                      // none of them is empty
+      const size_t slot = 2 * u + (u == u0 && F0 > units.start(u));
+      const float2 e = __ldcg(v.part_ml + slot * HY_GROUP + head);
       const float po = __ldcg(v.part_o + slot * (HY_GROUP * HY_HEAD_DIM) + tid);
-      const float m_new = fmaxf(M, ml.x);
+      const float m_new = fmaxf(M, e.x);
       const float w0 = m_new == -INFINITY ? 1.f : ex2_ftz(M - m_new);
-      const float w1 = m_new == -INFINITY ? 1.f : ex2_ftz(ml.x - m_new);
-      L = fmaf(L, w0, ml.y * w1);
+      const float w1 = m_new == -INFINITY ? 1.f : ex2_ftz(e.x - m_new);
+      L = fmaf(L, w0, e.y * w1);
       acc = fmaf(acc, w0, po * w1);
       M = m_new;
     }
-    a.out[((size_t)a.cu_q[seq] * a.q_heads + g * HY_GROUP + head) * HY_HEAD_DIM + d] =
-        __float2bfloat16_rn(acc / L);
+    a.out[((size_t)p.tok * a.q_heads + g * HY_GROUP) * HY_HEAD_DIM + tid] = __float2bfloat16_rn(acc / L);
   }
+  __syncthreads();                                        // sh.part is read
   return true;
 }
 
@@ -865,32 +908,31 @@ __device__ bool prefill_item(const Args& a, const PlanView& v, int item, uint8_t
 constexpr int MIXED_UNITS = 3;
 __device__ bool decode_all(const Args& a, const PlanView& v, int n_pre, int n_pairs, long blocks,
                            uint8_t* payload, Shared& sh) {
-  uint32_t ring_ctr = 0;
+  uint32_t ring_pos = 0, ring_par = 0;
   const long total = blocks * a.kv_heads;
   if (total == 0) return true;
-  if (n_pairs > 0) {
-    if ((int)blockIdx.x >= n_pairs) return true;
-    const int seq = (int)blockIdx.x / a.kv_heads, g = (int)blockIdx.x - seq * a.kv_heads;
-    const int p0 = v.dec_blocks[seq], nb = v.dec_blocks[seq + 1] - p0;
-    const long f0 = (long)p0 * a.kv_heads + (long)g * nb;
-    return nb == 0 || decode_unit(a, v, total, 0, 0, f0, f0 + nb, payload, sh, ring_ctr);
-  }
-  if (n_pre == 0) {
-    const int u = blockIdx.x, units = gridDim.x;
-    return decode_unit(a, v, total, units, u, unit_start(total, units, u),
-                       unit_start(total, units, u + 1), payload, sh, ring_ctr);
-  }
-  const int units = MIXED_UNITS * gridDim.x;
+  const Units units(total, n_pairs > 0 ? n_pairs : n_pre > 0 ? MIXED_UNITS * (int)gridDim.x : (int)gridDim.x);
   int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
+  int u = blockIdx.x;
   for (;;) {
-    if (threadIdx.x == 0) sh.unit = atomicAdd(&grab[0], 1);
-    __syncthreads();
-    const int u = sh.unit;
-    __syncthreads();
-    if (u >= units) return true;
-    if (!decode_unit(a, v, total, units, u, unit_start(total, units, u),
-                     unit_start(total, units, u + 1), payload, sh, ring_ctr))
+    if (n_pre > 0) {
+      if (threadIdx.x == 0) sh.unit = atomicAdd(&grab[0], 1);
+      __syncthreads();
+      u = sh.unit;
+      __syncthreads();
+    }
+    if (u >= units.n) return true;
+    int only_seq = -1;
+    long f0 = units.start(u), f1 = units.start(u + 1);
+    if (n_pairs > 0) {
+      only_seq = u / a.kv_heads;
+      const int p0 = v.dec_blocks[only_seq], nb = v.dec_blocks[only_seq + 1] - p0;
+      f0 = (long)p0 * a.kv_heads + (long)(u - only_seq * a.kv_heads) * nb;
+      f1 = f0 + nb;
+    }
+    if (!decode_unit(a, v, units, u, only_seq, f0, f1, payload, sh, ring_pos, ring_par))
       return false;
+    if (n_pre == 0) return true;
   }
 }
 
