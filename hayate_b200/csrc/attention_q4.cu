@@ -25,12 +25,13 @@ namespace {
 
 constexpr int NW = 16;                                    // warps per CTA
 constexpr int NT = NW * 32;
-#ifndef HY_Q4_STAGES
-#define HY_Q4_STAGES 4
-#endif
-constexpr int NS = HY_Q4_STAGES;                          // blocks in flight per warp
 constexpr int BLK_BYTES = 2 * Q4_TILE_BYTES;              // K and V tile of one block and head
-constexpr int RING_BYTES = NS * BLK_BYTES;
+constexpr int STAGE_BYTES = 2 * BLK_BYTES;                // a decode warp takes two blocks at a time
+#ifndef HY_Q4_STAGES
+#define HY_Q4_STAGES 2
+#endif
+constexpr int NS = HY_Q4_STAGES;                          // stages of a decode warp's ring
+constexpr int RING_BYTES = NS * STAGE_BYTES;
 // a warp's partial result of one (sequence, head): O [4][128], then (m, l) [4]
 constexpr int PART_FLOATS = HY_GROUP * HY_HEAD_DIM + 2 * HY_GROUP;
 constexpr int DEC_SMEM = NW * (RING_BYTES + 2 * PART_FLOATS * 4);
@@ -127,7 +128,7 @@ HY_DEVICE void cursor_sequence(const Args& a, const PlanView& v, Cursor& k) {
 }
 // The place of flattened block f: in sequence seq (>= 0), or in the last sequence that
 // starts at or before f, found by the whole warp 32 sequences (or runs of 32^n) at a time.
-HY_DEVICE Cursor cursor_at(const Args& a, const PlanView& v, int seq, long f) {
+HY_DEVICE Cursor cursor_at(const Args& a, const PlanView& v, int seq, int f) {
   Cursor k;
   k.seq = seq;
   if (seq < 0) {
@@ -136,13 +137,13 @@ HY_DEVICE Cursor cursor_at(const Args& a, const PlanView& v, int seq, long f) {
     while ((long)step * 32 < a.num_seqs) step *= 32;
     for (; step >= 1; step >>= 5) {
       const long i = lo + (long)lane * step;
-      const bool le = i < a.num_seqs && (long)v.dec_blocks[i] * a.kv_heads <= f;
+      const bool le = i < a.num_seqs && v.dec_blocks[i] * a.kv_heads <= f;
       lo += (31 - __clz(__ballot_sync(0xffffffffu, le) | 1u)) * step;
     }
     k.seq = lo;
   }
   cursor_sequence(a, v, k);
-  const int in = (int)(f - (long)v.dec_blocks[k.seq] * a.kv_heads);
+  const int in = f - v.dec_blocks[k.seq] * a.kv_heads;
   k.g = in / k.nb;
   k.b = in - k.g * k.nb;
   return k;
@@ -158,25 +159,25 @@ HY_DEVICE void cursor_next_pair(const Args& a, const PlanView& v, Cursor& k) {
   cursor_sequence(a, v, k);
 }
 
-// One warp: key blocks [f0, f1) of the flattened list, pair by pair.
+// One warp: key blocks [f0, f1) of the flattened list, pair by pair, two blocks (32 keys)
+// at a time.
 //
 // Scores are computed transposed, S^T = K Q^T (16 keys x 8 columns, 4 of them heads),
 // and so is the output, O^T = V^T P^T: the codes then fill the 16-row operand of
 // mma.sync, where the 4 heads alone would leave three quarters of it empty.  The codes
-// enter the products as they are (q4_bits), and the parameters outside them, in fp32 or
-// folded into the weights:
+// enter the products as they are (q4_bits), and the parameters outside them:
 //   score = sum over halves of scale_K (code . q) + minimum_K (sum of q)
 //   out   = sum over keys of (p scale_V) code + p minimum_V
-// so that an expanded value costs 5/8 of an instruction, keys are exact, and the
-// only roundings are p scale_V's to fp16 (2^-11) and the output's.  p scale_V is kept
-// inside fp16's normal range by a power of two 2^k (vs): p is at most 2^8 (the maximum
-// is only raised when a score exceeds it by more than that, so that most blocks need
-// no exchange between lanes), scale_V 2^k at most 2^7.
+// so that an expanded value costs 5/8 of an instruction and keys are exact.  The
+// minima of K meet the sums of q in a product of their own (the sums as two fp16
+// parts, 22 bits); p and p scale_V are rounded to fp16 (2^-11 each), the output to bf16.
+// p scale_V is kept inside fp16's normal range by a power of two vs: p is at most 2^8
+// (the maximum is only raised when a score exceeds it by more than that, so that most
+// blocks need no exchange between lanes), scale_V vs at most 2^7.
 // Lane (r, c) = (lane / 4, lane % 4) with c < 2 ends with heads 2 c + k (k = 0, 1) at
-// dimensions 8 r + i and 64 + 8 r + i.  ring: shared-memory address of the warp's ring,
-// ring_pos its next slot, ring_par the parity of its next pass.  Returns false if a
-// wait ran out.
-HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, long f0, long f1,
+// dimensions 8 r + i and 64 + 8 r + i.  ring_pos: the ring's next stage, ring_par the
+// parity of its next pass.  Returns false if a wait ran out.
+HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, int f0, int f1,
                            uint8_t* ring_ptr, float* part, Part* parts, uint64_t* bars,
                            uint32_t& ring_pos, uint32_t& ring_par) {
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
@@ -184,11 +185,11 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, long f0, l
   const uint32_t ring = smem_u32(ring_ptr);
   Cursor k = cursor_at(a, v, seq, f0);                    // the pair being computed
   Cursor ld = k;                                          // the next block to load
-  int to_load = (int)(f1 - f0), left = to_load;
-  const __nv_bfloat16* q0 = a.q + (size_t)r * HY_HEAD_DIM + 16 * c;      // this lane's part of Q
-  uint4 qraw[4];
+  int to_load = f1 - f0, left = to_load;
+  uint4 qraw[4];                                          // this lane's part of Q
   auto load_q = [&]() {
-    const __nv_bfloat16* qp = q0 + ((size_t)k.tok * a.q_heads + k.g * HY_GROUP) * HY_HEAD_DIM;
+    const __nv_bfloat16* qp =
+        a.q + ((size_t)k.tok * a.q_heads + k.g * HY_GROUP + r) * HY_HEAD_DIM + 16 * c;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       qraw[i] = r < HY_GROUP ? *reinterpret_cast<const uint4*>(qp + 64 * (i >> 1) + 8 * (i & 1))
@@ -206,35 +207,37 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, long f0, l
     if (run == 0) {
       if (ld.b == ld.nb) cursor_next_pair(a, v, ld);
       turn = 0;
-      run = min(32, ld.nb - ld.b);
+      run = min(min(32, to_load), ld.nb - ld.b);
       int blk = lane < run && ld.b + lane < a.bt_pitch ? __ldg(ld.bt + ld.b + lane) : -1;
       if (blk < 0 || blk >= a.num_blocks) {
-        if (lane < min(run, to_load)) hy_flag(a.err, HY_ERR_BOUNDS);
+        if (lane < run) hy_flag(a.err, HY_ERR_BOUNDS);
         blk = 0;
       }
       src = a.cache + q4_tile(blk, ld.g, 0, a.kv_heads);
       ld.b += run;
     }
-    if (lane == turn) {
+    const int n = min(2, run);
+    if (lane == turn) mbar_arrive_expect_tx(&bars[put], n * BLK_BYTES);
+    __syncwarp();
+    if ((unsigned)(lane - turn) < (unsigned)n) {
       fence_proxy_async();
-      mbar_arrive_expect_tx(&bars[put], BLK_BYTES);
-      bulk_load(ring_ptr + put * BLK_BYTES, src, BLK_BYTES, &bars[put]);
+      bulk_load(ring_ptr + put * STAGE_BYTES + (lane - turn) * BLK_BYTES, src, BLK_BYTES, &bars[put]);
     }
-    ++turn;
-    --run;
-    --to_load;
+    turn += n;
+    run -= n;
+    to_load -= n;
     put = put + 1 == NS ? 0 : put + 1;
   };
 #pragma unroll 1
   for (int j = 0; j < NS; ++j) issue();
 
-  // shared-memory offsets of this lane inside a block's tiles: its two K rows (keyB is
-  // keyA + 4) and the first of its four V keys of either kind
+  // shared-memory offsets of this lane inside a block's tiles: its two K rows (the second
+  // four keys on) and the first of its four V keys of either kind
   const int keyA = key_of(r >> 1, r & 1, 0);
   const uint32_t k_off = keyA * Q4_ROW_BYTES + 8 * c, p_off = Q4_PARAM_OFF + keyA * Q4_PARAM_BYTES;
   const uint32_t v_off0 = Q4_TILE_BYTES + key_of(c, 0, 0) * Q4_ROW_BYTES + 4 * r;
   const uint32_t v_off1 = Q4_TILE_BYTES + key_of(c, 1, 0) * Q4_ROW_BYTES + 4 * r;
-  constexpr uint32_t ROW4 = 4 * Q4_ROW_BYTES, PAR4 = 4 * Q4_PARAM_BYTES;  // four keys on
+  constexpr uint32_t ROW4 = 4 * Q4_ROW_BYTES, PAR4 = 4 * Q4_PARAM_BYTES;
   uint32_t get = ring_pos, par = ring_par;
   bool ok = true, first_pair = true;
   int pending = 0;
@@ -242,14 +245,14 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, long f0, l
   while (left > 0) {
     const int n = min(left, k.nb - k.b), b_first = k.b;   // this pair's blocks in the range
     left -= n;
-    // the last block, if it is here and partial, and its keys
-    const int tail = b_first + n == k.nb && (k.kv_len & (HY_BLOCK - 1)) ? n - 1 : -1;
-    const int rest = k.kv_len & (HY_BLOCK - 1);
+    // whole blocks here, and the keys of the last one if it is here and partial
+    const int rest = b_first + n == k.nb ? k.kv_len & (HY_BLOCK - 1) : 0;
+    const int full = rest ? n - 1 : n;
     // Q in fp16 (q4_query_scale): lane (r, c) holds head r's words 2 c, 2 c + 1 (dimensions
     // 16 c ..) of both halves; rows 4-7 are zero.  Codes in bits 0-3 meet 2^14 q, codes
     // in bits 4-7 2^10 q, so that a score comes out as 2^-10 code . q.
-    uint32_t qb[2][2][4];
-    float qs[2][2], mult[2];                              // sums of q of heads 2 c + k, scale
+    uint32_t qb[2][2][4], qs = 0u;                        // qs: the operand of the sums of q
+    float mult[2];                                        // scale to log2 units of heads 2 c + k
     {
       float x[32], amax = 0.f, down, up;
 #pragma unroll
@@ -281,87 +284,104 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, long f0, l
       for (int hf = 0; hf < 2; ++hf) {
         sum[hf] += __shfl_xor_sync(0xffffffffu, sum[hf], 1);
         sum[hf] += __shfl_xor_sync(0xffffffffu, sum[hf], 2);
-        qs[hf][0] = __shfl_sync(0xffffffffu, sum[hf], 8 * c);            // head 2 c: lanes of row 2 c
-        qs[hf][1] = __shfl_sync(0xffffffffu, sum[hf], 8 * c + 4);
       }
-      mult[0] = a.scale_log2 * (1024.f * __shfl_sync(0xffffffffu, up, 8 * c));
-      mult[1] = a.scale_log2 * (1024.f * __shfl_sync(0xffffffffu, up, 8 * c + 4));
+      // times 2^8, the rest of what their 2^-10 is short of fp16's normal range: the minima
+      // meet (hi, hi) in lanes c = 0 and (lo, lo) in lanes c = 1, and the result is taken
+      // times 2^-8
+      const __half2 hi = __floats2half2_rn(sum[0] * 256.f, sum[1] * 256.f);
+      const float2 back = __half22float2(hi);
+      const __half2 lo = __floats2half2_rn(sum[0] * 256.f - back.x, sum[1] * 256.f - back.y);
+      qs = c == 0 ? q4_as_u32(hi) : c == 1 ? q4_as_u32(lo) : 0u;
+      // not 0 (a scale of 0, a row of tiny elements): masked scores are -inf times it
+      mult[0] = fmaxf(a.scale_log2 * (1024.f * __shfl_sync(0xffffffffu, up, 8 * c)), 1e-30f);
+      mult[1] = fmaxf(a.scale_log2 * (1024.f * __shfl_sync(0xffffffffu, up, 8 * c + 4)), 1e-30f);
     }
-    float o[8][4];                                        // O^T, in 2^-24 vs (odd m-tiles 2^-20 vs)
+    float o[8][4];                                        // O^T, in 2^-24 / vs (odd m-tiles 2^-20 / vs)
     float z[2][2] = {{0.f, 0.f}, {0.f, 0.f}};             // [half][k]: sum of p times V's minimum
     float m[2] = {-INFINITY, -INFINITY};                  // running maximum (log2 units)
-    float ms[2] = {0.f, 0.f};                             // the same, 0 while it is -inf
+    float thr[2] = {-INFINITY, -INFINITY};                // score at which it is raised
     float l[2] = {0.f, 0.f};                              // this lane's part of the sum
-    float vs = 1.f, vcap = -1.f;                          // 2^k, the largest scale that it fits
+    __half2 vs1 = q4_as_half2(0x3c003c00u);               // (vs, 1)
+    __half vcap = __ushort_as_half(0xbc00);               // the largest scale that vs fits: -1, none yet
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
 #pragma unroll 1
-    for (int i = 0; i < n; ++i) {
+    for (int i = 0; i < n; i += 2) {
       if (!__all_sync(0xffffffffu, mbar_try_wait(&bars[get], par)) &&
           !__all_sync(0xffffffffu, mbar_wait(&bars[get], par, a.err))) {
         ok = false;
-        pending = left + n - i - to_load;                 // copies not waited for
+        pending = left + n - i - to_load;                 // blocks not waited for
         break;
       }
-      const uint32_t st = ring + get * BLK_BYTES;
-
-      // S^T = K Q^T, one accumulator per half of the dimensions
-      float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      const uint32_t st = ring + get * STAGE_BYTES;
+      const uint32_t k_at = st + k_off, p_at = st + p_off, v_at0 = st + v_off0, v_at1 = st + v_off1;
+      float x[2][4];                                      // scores of (keyA, keyB) x 2 heads, per block
+      uint2 va[2], vb[2];                                 // V's parameters of keyA, keyB
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const uint2 wa = lds64(st + k_off + 32 * hf), wb = lds64(st + k_off + 32 * hf + ROW4);
-        uint32_t xa[4], xb[4];
-        q4_bits(wa.x, xa);
-        q4_bits(wb.x, xb);
-        mma_f16_16816(sc[hf], xa[0], xb[0], xa[1], xb[1], qb[hf][0][0], qb[hf][0][1]);
-        mma_f16_16816(sc[hf], xa[2], xb[2], xa[3], xb[3], qb[hf][0][2], qb[hf][0][3]);
-        q4_bits(wa.y, xa);
-        q4_bits(wb.y, xb);
-        mma_f16_16816(sc[hf], xa[0], xb[0], xa[1], xb[1], qb[hf][1][0], qb[hf][1][1]);
-        mma_f16_16816(sc[hf], xa[2], xb[2], xa[3], xb[3], qb[hf][1][2], qb[hf][1][3]);
-      }
-      float x[4];                                         // scores of (keyA, keyB) x 2 heads
-      {
-        const uint2 pa = lds64(st + p_off), pb = lds64(st + p_off + PAR4);
-        const float2 a0 = __half22float2(q4_as_half2(pa.x)), a1 = __half22float2(q4_as_half2(pa.y));
-        const float2 b0 = __half22float2(q4_as_half2(pb.x)), b1 = __half22float2(q4_as_half2(pb.y));
+      for (int b = 0; b < 2; ++b) {
+        // S^T = K Q^T, one accumulator per half of the dimensions
+        const uint32_t kb = k_at + b * BLK_BYTES, pb = p_at + b * BLK_BYTES;
+        float sc[3][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const uint2 wa = lds64(kb + 32 * hf), wb = lds64(kb + 32 * hf + ROW4);
+          uint32_t xa[4], xb[4];
+          q4_bits(wa.x, xa);
+          q4_bits(wb.x, xb);
+          mma_f16_16816(sc[hf], xa[0], xb[0], xa[1], xb[1], qb[hf][0][0], qb[hf][0][1]);
+          mma_f16_16816(sc[hf], xa[2], xb[2], xa[3], xb[3], qb[hf][0][2], qb[hf][0][3]);
+          q4_bits(wa.y, xa);
+          q4_bits(wb.y, xb);
+          mma_f16_16816(sc[hf], xa[0], xb[0], xa[1], xb[1], qb[hf][1][0], qb[hf][1][1]);
+          mma_f16_16816(sc[hf], xa[2], xb[2], xa[3], xb[3], qb[hf][1][2], qb[hf][1][3]);
+        }
+        const uint2 pa = lds64(pb), pc = lds64(pb + PAR4);
+        mma_f16_16816(sc[2], __byte_perm(pa.x, pa.y, 0x7632), __byte_perm(pc.x, pc.y, 0x7632), 0u, 0u, qs, 0u);
+        const float a0 = __low2float(q4_as_half2(pa.x)), a1 = __low2float(q4_as_half2(pa.y));
+        const float c0 = __low2float(q4_as_half2(pc.x)), c1 = __low2float(q4_as_half2(pc.y));
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          x[e] = mult[e] * fmaf(a0.x, sc[0][e], fmaf(a1.x, sc[1][e], fmaf(a0.y, qs[0][e], a1.y * qs[1][e])));
-          x[2 + e] = mult[e] * fmaf(b0.x, sc[0][2 + e], fmaf(b1.x, sc[1][2 + e], fmaf(b0.y, qs[0][e], b1.y * qs[1][e])));
+          x[b][e] = fmaf(a0, sc[0][e], fmaf(a1, sc[1][e], 0x1p-8f * sc[2][e]));
+          x[b][2 + e] = fmaf(c0, sc[0][2 + e], fmaf(c1, sc[1][2 + e], 0x1p-8f * sc[2][2 + e]));
+        }
+        va[b] = lds64(pb + Q4_TILE_BYTES);
+        vb[b] = lds64(pb + Q4_TILE_BYTES + PAR4);
+      }
+      if (i + 2 > full) {                                 // keys past the end: their rows hold anything
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int keys = i + b < full ? HY_BLOCK : i + b < n ? rest : 0;
+          if (keyA >= keys) { x[b][0] = x[b][1] = -INFINITY; va[b] = make_uint2(0u, 0u); }
+          if (keyA + 4 >= keys) { x[b][2] = x[b][3] = -INFINITY; vb[b] = make_uint2(0u, 0u); }
         }
       }
-      uint2 va = lds64(st + p_off + Q4_TILE_BYTES), vb = lds64(st + p_off + Q4_TILE_BYTES + PAR4);
-      if (i == tail) {                                    // rows past the end hold anything
-        if (keyA >= rest) { x[0] = x[1] = -INFINITY; va = make_uint2(0u, 0u); }
-        if (keyA + 4 >= rest) { x[2] = x[3] = -INFINITY; vb = make_uint2(0u, 0u); }
-      }
-      // V's (scale, minimum) of (keyA, keyB) x half
-      const float2 va0 = __half22float2(q4_as_half2(va.x)), va1 = __half22float2(q4_as_half2(va.y));
-      const float2 vb0 = __half22float2(q4_as_half2(vb.x)), vb1 = __half22float2(q4_as_half2(vb.y));
-      float mx[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
-      float smax = fmaxf(fmax3f(va0.x, va1.x, vb0.x), vb1.x);
-      const bool grow = mx[0] > m[0] + RESCALE_LOG2 || mx[1] > m[1] + RESCALE_LOG2 || smax > vcap;
+      float mx[2] = {fmax3f(x[0][0], x[0][2], fmaxf(x[1][0], x[1][2])),
+                     fmax3f(x[0][1], x[0][3], fmaxf(x[1][1], x[1][3]))};
+      const __half2 smax2 = __hmax2(
+          __hmax2(__hmax2(q4_as_half2(va[0].x), q4_as_half2(va[0].y)), __hmax2(q4_as_half2(vb[0].x), q4_as_half2(vb[0].y))),
+          __hmax2(__hmax2(q4_as_half2(va[1].x), q4_as_half2(va[1].y)), __hmax2(q4_as_half2(vb[1].x), q4_as_half2(vb[1].y))));
+      const bool grow = mx[0] > thr[0] || mx[1] > thr[1] || __hgt(__low2half(smax2), vcap);
       if (__any_sync(0xffffffffu, grow)) {
+        float smax = __low2float(smax2);
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, d));
         float vr = 1.f;                                   // change of vs
-        if (smax > vcap) {                                // 2^(6 - exponent), for scales of 2^-24 and up
-          const int e = min(max((__float_as_int(smax) >> 23) & 255, 103), 254) - 127;
-          const float vs_new = __int_as_float((6 - e + 127) << 23);
-          vr = vcap < 0.f ? 1.f : vs_new / vs;
-          vs = vs_new;
-          vcap = __int_as_float((e + 127) << 23) * 1.9990234375f;       // the largest fp16 below 2^(e + 1)
+        if (smax > __half2float(vcap)) {                  // vs = 2^(6 - exponent), at most 2^15
+          const int e = min(max((__float_as_int(smax) >> 23) & 255, 118), 254) - 127;
+          const float vs = __int_as_float((6 - e + 127) << 23);
+          vr = __half2float(vcap) < 0.f ? 1.f : vs / __low2float(vs1);
+          vs1 = __floats2half2_rn(vs, 1.f);
+          vcap = __float2half_rn(__int_as_float((e + 127) << 23) * 1.9990234375f);   // the last below 2^(e + 1)
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], d));
-          const float m_new = fmaxf(m[e], mx[e]);
+          const float m_new = fmaxf(m[e], mx[e] * mult[e]);
           const float alpha = m_new == -INFINITY ? 1.f : ex2_ftz(m[e] - m_new);
           m[e] = m_new;
-          ms[e] = m_new == -INFINITY ? 0.f : m_new;
+          thr[e] = (m_new + RESCALE_LOG2) / mult[e];
           l[e] *= alpha;
           z[0][e] *= alpha;
           z[1][e] *= alpha;
@@ -370,38 +390,44 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, long f0, l
           for (int j = 0; j < 8; ++j) { o[j][e] *= ao; o[j][2 + e] *= ao; }
         }
       }
+      const float ms[2] = {m[0] == -INFINITY ? 0.f : -m[0], m[1] == -INFINITY ? 0.f : -m[1]};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = ex2_ftz(x[e] - ms[e & 1]);
-      l[0] += x[0] + x[2];
-      l[1] += x[1] + x[3];
-      uint32_t pt[2][2];                                  // P^T operands [half][keys 0-7, 8-15]
+      for (int b = 0; b < 2; ++b) {
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const float2 ua = hf ? va1 : va0, ub = hf ? vb1 : vb0;
-        const float wa = ua.x * vs, wb = ub.x * vs;
-        pt[hf][0] = movmatrix_trans(q4_as_u32(__floats2half2_rn(x[0] * wa, x[1] * wa)));
-        pt[hf][1] = movmatrix_trans(q4_as_u32(__floats2half2_rn(x[2] * wb, x[3] * wb)));
-        z[hf][0] = fmaf(x[0], ua.y, fmaf(x[2], ub.y, z[hf][0]));
-        z[hf][1] = fmaf(x[1], ua.y, fmaf(x[3], ub.y, z[hf][1]));
-      }
-      // O^T += V^T (scale P)^T, a half of the dimensions per product: the lane's word r of
-      // four keys holds dimensions 8 r .. 8 r + 7; nibbles of equal weight share an m-tile
-      // (rows 0-7 nibble j, rows 8-15 nibble j + 2)
+        for (int e = 0; e < 4; ++e) x[b][e] = ex2_ftz(fmaf(x[b][e], mult[e & 1], ms[e & 1]));
+        l[0] += x[b][0] + x[b][2];
+        l[1] += x[b][1] + x[b][3];
+        const __half2 pa = __floats2half2_rn(x[b][0], x[b][1]), pc = __floats2half2_rn(x[b][2], x[b][3]);
+        uint32_t pt[2][2];                                // P^T operands [half][keys 0-7, 8-15]
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        uint32_t y[2][2][4];                              // [keys 0-7, 8-15][low, high nibbles]
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t w0 = lds32(st + v_off0 + 32 * hf + ROW4 * h), w1 = lds32(st + v_off1 + 32 * hf + ROW4 * h);
-          q4_bits(__byte_perm(w0, w1, 0x5410), y[h][0]);
-          q4_bits(__byte_perm(w0, w1, 0x7632), y[h][1]);
+        for (int hf = 0; hf < 2; ++hf) {
+          const __half2 ua = q4_as_half2(hf ? va[b].y : va[b].x), uc = q4_as_half2(hf ? vb[b].y : vb[b].x);
+          pt[hf][0] = movmatrix_trans(q4_as_u32(__hmul2(pa, __low2half2(__hmul2(ua, vs1)))));
+          pt[hf][1] = movmatrix_trans(q4_as_u32(__hmul2(pc, __low2half2(__hmul2(uc, vs1)))));
+          const float na = __high2float(ua), nc = __high2float(uc);
+          z[hf][0] = fmaf(x[b][0], na, fmaf(x[b][2], nc, z[hf][0]));
+          z[hf][1] = fmaf(x[b][1], na, fmaf(x[b][3], nc, z[hf][1]));
         }
+        // O^T += V^T (scale P)^T, a half of the dimensions per product: the lane's word r of
+        // four keys holds dimensions 8 r .. 8 r + 7; nibbles of equal weight share an m-tile
+        // (rows 0-7 nibble j, rows 8-15 nibble j + 2)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t y[2][2][4];                            // [keys 0-7, 8-15][low, high nibbles]
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            mma_f16_16816(o[4 * hf + 2 * e + j], y[0][e][j], y[0][e][j + 2], y[1][e][j], y[1][e][j + 2],
-                          pt[hf][0], pt[hf][1]);
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t w0 = lds32(v_at0 + b * BLK_BYTES + 32 * hf + ROW4 * h);
+            const uint32_t w1 = lds32(v_at1 + b * BLK_BYTES + 32 * hf + ROW4 * h);
+            q4_bits(__byte_perm(w0, w1, 0x5410), y[h][0]);
+            q4_bits(__byte_perm(w0, w1, 0x7632), y[h][1]);
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              mma_f16_16816(o[4 * hf + 2 * e + j], y[0][e][j], y[0][e][j + 2], y[1][e][j], y[1][e][j + 2],
+                            pt[hf][0], pt[hf][1]);
+        }
       }
       if (++get == NS) {
         get = 0;
@@ -426,6 +452,7 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, long f0, l
       }
       inv[e] = whole ? 1.f / l[e] : 1.f;
     }
+    const float vs = __low2float(vs1);
     const float unit0 = 0x1p24f / vs, unit1 = 0x1p20f / vs;       // m-tiles of bits 0-3, 4-7
     if (c < 2) {
 #pragma unroll
@@ -464,14 +491,14 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, long f0, l
       load_q();
     }
   }
-  if (!ok) {                                              // copies in flight land before the CTA exits
-    for (; pending > 0; --pending) {
+  if (!ok && pending > 0) {                               // copies in flight land before the CTA exits
+    do {
       mbar_wait(&bars[get], par, nullptr);
       if (++get == NS) {
         get = 0;
         par ^= 1u;
       }
-    }
+    } while (get != put);
   }
   ring_pos = get;
   ring_par = par;
@@ -485,73 +512,79 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, long f0, l
 // range), and the CTA whose count of blocks completes a pair joins its partials.
 // Returns false if a wait ran out.
 struct Units {            // `total` blocks in n units whose sizes differ by at most one
-  long total;
-  int n;
-  long size, more;        // the first `more` units have size + 1 blocks
-  HY_DEVICE Units(long t, int units) : total(t), n(units), size(t / units), more(t - size * units) {}
-  HY_DEVICE long start(int u) const { return u * size + min((long)u, more); }
-  HY_DEVICE int of(long f) const {                        // the unit that holds block f
-    return (int)(f < more * (size + 1) ? f / (size + 1) : more + (f - more * (size + 1)) / size);
+  int n, size, more;      // the first `more` units have size + 1 blocks
+  HY_DEVICE Units(int total, int units) : n(units), size(total / units), more(total - size * units) {}
+  HY_DEVICE int start(int u) const { return u * size + min(u, more); }
+  HY_DEVICE int of(int f) const {                         // the unit that holds block f
+    return f < more * (size + 1) ? f / (size + 1) : more + (f - more * (size + 1)) / size;
   }
 };
 
 HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units, int unit,
-                           int only_seq, long f0, long f1, uint8_t* payload, Shared& sh,
+                           int only_seq, int f0, int f1, uint8_t* payload, Shared& sh,
                            uint32_t& ring_pos, uint32_t& ring_par) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const float* parts = reinterpret_cast<const float*>(payload + NW * RING_BYTES);
+  float* parts = reinterpret_cast<float*>(payload + NW * RING_BYTES);
   if (lane < 2) sh.part[2 * warp + lane].pair = -1;
   __syncwarp();
-  const int n = (int)(f1 - f0);
-  const bool ok = decode_warp(a, v, only_seq, f0 + (long)n * warp / NW, f0 + (long)n * (warp + 1) / NW,
-                              payload + warp * RING_BYTES,
-                              const_cast<float*>(parts) + warp * 2 * PART_FLOATS,
-                              sh.part + 2 * warp, sh.bar[warp], ring_pos, ring_par);
+  const int n = f1 - f0, per = n / NW, more = n - per * NW;       // the first `more` warps take one more
+  const int w0 = f0 + warp * per + min(warp, more);
+  const bool ok = decode_warp(a, v, only_seq, w0, w0 + per + (warp < more), payload + warp * RING_BYTES,
+                              parts + warp * 2 * PART_FLOATS, sh.part + 2 * warp, sh.bar[warp],
+                              ring_pos, ring_par);
   if (__syncthreads_or(!ok)) return false;
 
   // Lane j of every warp looks after part j: parts of one pair are neighbours (but for
-  // empty ones between them), so the first lane of each run leads it.
-  static_assert(2 * NW == 32, "one part per lane");
-  const int head = warp >> 2, d = tid & 127;              // a warp has one head
+  // empty ones between them).  Warps 4 i + h, i = 0..3, take head h of every fourth pair.
+  static_assert(2 * NW == 32 && NW == 4 * HY_GROUP, "one part per lane, four warps per head");
+  const int head = warp & 3;
   const Part mine = sh.part[lane];
   const float2 ml = mine.pair < 0 ? make_float2(-INFINITY, 0.f)
                                   : *reinterpret_cast<const float2*>(
                                         parts + lane * PART_FLOATS + HY_GROUP * HY_HEAD_DIM + 2 * head);
   unsigned todo = __ballot_sync(0xffffffffu, mine.pair >= 0);
   int open_at[2], open_blocks[2], n_open = 0;             // pairs that reach out: first part, blocks here
-  while (todo) {
+  for (int turn = 0; todo; ++turn) {
     const int i = __ffs(todo) - 1;
     const int pair = __shfl_sync(0xffffffffu, mine.pair, i);
     const bool in = mine.pair == pair;
     const unsigned group = __ballot_sync(0xffffffffu, in);
     todo &= ~group;
-    float M = in ? ml.x : -INFINITY, L;
-    int blocks = in ? mine.blocks : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-      blocks += __shfl_xor_sync(0xffffffffu, blocks, o);
-    }
-    const float wt = in ? ex2_ftz(ml.x - (M == -INFINITY ? 0.f : M)) : 0.f;
-    L = wt * ml.y;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    float acc = 0.f;
-    for (unsigned g = group; g; g &= g - 1) {
-      const int j = __ffs(g) - 1;
-      acc = fmaf(__shfl_sync(0xffffffffu, wt, j), parts[j * PART_FLOATS + tid], acc);
-    }
-    const int nb = __shfl_sync(0xffffffffu, mine.nb, i), tok = __shfl_sync(0xffffffffu, mine.tok, i);
-    const int seq = pair / a.kv_heads, g = pair - seq * a.kv_heads;
-    if (blocks == nb) {
-      a.out[((size_t)tok * a.q_heads + g * HY_GROUP) * HY_HEAD_DIM + tid] = __float2bfloat16_rn(acc / L);
-    } else {
-      const size_t slot = 2 * unit + ((long)v.dec_blocks[seq] * a.kv_heads + (long)g * nb > f0);
-      __stcg(v.part_o + slot * (HY_GROUP * HY_HEAD_DIM) + tid, acc);
-      if (d == 0) __stcg(v.part_ml + slot * HY_GROUP + head, make_float2(M, L));
+    const int blocks = __reduce_add_sync(0xffffffffu, in ? mine.blocks : 0);
+    const int nb = __shfl_sync(0xffffffffu, mine.nb, i);
+    if (blocks != nb) {
       open_at[n_open & 1] = i;
       open_blocks[n_open & 1] = blocks;
       ++n_open;
+    }
+    if ((turn & 3) != (warp >> 2)) continue;              // warp-uniform
+    const int tok = __shfl_sync(0xffffffffu, mine.tok, i);
+    float M = in ? ml.x : -INFINITY;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float wt = in ? ex2_ftz(ml.x - (M == -INFINITY ? 0.f : M)) : 0.f;
+    float L = wt * ml.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (unsigned g = group; g; g &= g - 1) {
+      const int j = __ffs(g) - 1;
+      const float w = __shfl_sync(0xffffffffu, wt, j);
+      const float4 p = *reinterpret_cast<const float4*>(parts + j * PART_FLOATS + head * HY_HEAD_DIM + 4 * lane);
+      acc.x = fmaf(w, p.x, acc.x);
+      acc.y = fmaf(w, p.y, acc.y);
+      acc.z = fmaf(w, p.z, acc.z);
+      acc.w = fmaf(w, p.w, acc.w);
+    }
+    const int seq = pair / a.kv_heads, g = pair - seq * a.kv_heads;
+    if (blocks == nb) {
+      const float inv = 1.f / L;
+      *reinterpret_cast<uint2*>(a.out + ((size_t)tok * a.q_heads + g * HY_GROUP + head) * HY_HEAD_DIM + 4 * lane) =
+          make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    } else {
+      const size_t slot = 2 * unit + (v.dec_blocks[seq] * a.kv_heads + g * nb > f0);
+      __stcg(reinterpret_cast<float4*>(v.part_o + (slot * HY_GROUP + head) * HY_HEAD_DIM) + lane, acc);
+      if (lane == 0) __stcg(v.part_ml + slot * HY_GROUP + head, make_float2(M, L));
     }
   }
   if (n_open == 0) {
@@ -574,24 +607,26 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
   }
   __syncthreads();
   const int last = sh.last;
+  if (last == 0) return true;
   __threadfence();                                        // the others' partials, after the count
   for (int j = 0; j < n_open; ++j) {
     if (!((last >> j) & 1)) continue;
     const Part p = sh.part[open_at[j]];
     const int seq = p.pair / a.kv_heads, g = p.pair - seq * a.kv_heads;
-    const long F0 = (long)v.dec_blocks[seq] * a.kv_heads + (long)g * p.nb, F1 = F0 + p.nb;
-    const int u0 = units.of(F0), u1 = units.of(F1 - 1);
+    const int F0 = v.dec_blocks[seq] * a.kv_heads + g * p.nb;
+    const int u0 = units.of(F0), u1 = units.of(F0 + p.nb - 1);
+    const int inside = F0 > units.start(u0), h = tid >> 7;
     float M = -INFINITY, L = 0.f, acc = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int u = u0; u <= u1; ++u) {                      // none of them is empty
-      const size_t slot = 2 * u + (u == u0 && F0 > units.start(u));
-      const float2 e = __ldcg(v.part_ml + slot * HY_GROUP + head);
+      const size_t slot = 2 * u + (u == u0 ? inside : 0);
+      const float2 e = __ldcg(v.part_ml + slot * HY_GROUP + h);
       const float po = __ldcg(v.part_o + slot * (HY_GROUP * HY_HEAD_DIM) + tid);
       const float m_new = fmaxf(M, e.x);
-      const float w0 = m_new == -INFINITY ? 1.f : ex2_ftz(M - m_new);
-      const float w1 = m_new == -INFINITY ? 1.f : ex2_ftz(e.x - m_new);
-      L = fmaf(L, w0, e.y * w1);
-      acc = fmaf(acc, w0, po * w1);
+      const float s0 = m_new == -INFINITY ? 1.f : ex2_ftz(M - m_new);
+      const float s1 = m_new == -INFINITY ? 1.f : ex2_ftz(e.x - m_new);
+      L = fmaf(L, s0, e.y * s1);
+      acc = fmaf(acc, s0, po * s1);
       M = m_new;
     }
     a.out[((size_t)p.tok * a.q_heads + g * HY_GROUP) * HY_HEAD_DIM + tid] = __float2bfloat16_rn(acc / L);
@@ -906,10 +941,10 @@ __device__ bool prefill_item(const Args& a, const PlanView& v, int item, uint8_t
 // beside prefill items, whose CTAs come late, CTAs take units of a third of an even
 // share.  Returns false if a wait ran out.
 constexpr int MIXED_UNITS = 3;
-__device__ bool decode_all(const Args& a, const PlanView& v, int n_pre, int n_pairs, long blocks,
+__device__ bool decode_all(const Args& a, const PlanView& v, int n_pre, int n_pairs, int blocks,
                            uint8_t* payload, Shared& sh) {
   uint32_t ring_pos = 0, ring_par = 0;
-  const long total = blocks * a.kv_heads;
+  const int total = blocks * a.kv_heads;                  // below 2^31: the host checks the tables' size
   if (total == 0) return true;
   const Units units(total, n_pairs > 0 ? n_pairs : n_pre > 0 ? MIXED_UNITS * (int)gridDim.x : (int)gridDim.x);
   int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
@@ -923,11 +958,11 @@ __device__ bool decode_all(const Args& a, const PlanView& v, int n_pre, int n_pa
     }
     if (u >= units.n) return true;
     int only_seq = -1;
-    long f0 = units.start(u), f1 = units.start(u + 1);
+    int f0 = units.start(u), f1 = units.start(u + 1);
     if (n_pairs > 0) {
       only_seq = u / a.kv_heads;
       const int p0 = v.dec_blocks[only_seq], nb = v.dec_blocks[only_seq + 1] - p0;
-      f0 = (long)p0 * a.kv_heads + (long)(u - only_seq * a.kv_heads) * nb;
+      f0 = p0 * a.kv_heads + (u - only_seq * a.kv_heads) * nb;
       f1 = f0 + nb;
     }
     if (!decode_unit(a, v, units, u, only_seq, f0, f1, payload, sh, ring_pos, ring_par))

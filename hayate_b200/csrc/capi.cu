@@ -496,6 +496,9 @@ int hy_varlen_attention_q4(int32_t dtype, const void* q, void* out, int32_t num_
     return fail(HY_E_INVALID, "hy_varlen_attention_q4: bf16 needs a planned, 256-byte aligned workspace");
   if (max_seqs <= 0 || max_tokens <= 0 || num_seqs > max_seqs || num_tokens > max_tokens)
     return fail(HY_E_INVALID, "hy_varlen_attention_q4: num_seqs or num_tokens above the workspace's");
+  // the kernel numbers the key blocks of all (sequence, head) pairs in 32 bits
+  if ((int64_t)num_seqs * bt_pitch * kv_heads > INT32_MAX)
+    return fail(HY_E_UNSUPPORTED, "hy_varlen_attention_q4: num_seqs x bt_pitch x kv_heads exceeds 2^31");
   const int dev = current_device();
   const PlanDims d = hy_attn_plan_dims(max_seqs, max_tokens, kv_heads, dev);
   if (workspace_bytes < hy_attn_workspace_bytes(d))
