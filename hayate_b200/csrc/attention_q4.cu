@@ -68,10 +68,19 @@ struct Args {
   int32_t* err;
 };
 
+// A place in the flattened list of key blocks (sequence, head, block) of the step's
+// decode sequences, with what a warp needs of the sequence.  Warps keep theirs in shared
+// memory: it is read once per pair, and the key loop needs the registers.
+struct Cursor {
+  int seq, g, b, nb;                                      // block b of nb
+  int first, tok, kv_len, row;                            // of the sequence, see SeqInfo
+};
+
 // What a warp leaves of a pair that it did not finish alone.
 struct Part {
   int pair;               // sequence * kv_heads + head, -1: none
   int blocks, nb;         // blocks that it covers, blocks of the pair
+  int first;              // the pair's first block in the flattened list
   int tok;                // query row
 };
 
@@ -80,6 +89,7 @@ struct Shared {
   int unit;               // the CTA's next unit of decode work
   int last;               // bit j: this CTA finished pair j of its two open ones
   Part part[2 * NW];      // each warp's two parts, in block order
+  Cursor cur[NW][2];      // each warp's pair computed, and next block to load
   // prefill; ring barriers complete once per use of their slot, the others once
   // per key tile (per use of their S buffer), qfull once per item
   uint64_t full[PS];      // K and V of a tile expanded (one arrival per expanding warp)
@@ -113,37 +123,55 @@ HY_DEVICE void q4_bits(uint32_t w, uint32_t (&x)[4]) {
   x[3] = w8 & 0x00f000f0u;
 }
 
-// A place in the flattened list of key blocks (sequence, head, block) of the step's
-// decode sequences, with what a warp needs of the sequence.
-struct Cursor {
-  int seq, g, b, nb;                                      // block b of nb
-  int tok, kv_len;                                        // query row, key length
-  const int32_t* bt;
+// What a sequence is to the decode: its first block in the list of all sequences' key
+// blocks, query row, key length and block-table row.
+struct SeqInfo {
+  int first, tok, kv_len, row;
 };
-HY_DEVICE void cursor_sequence(const Args& a, const PlanView& v, Cursor& k) {
-  k.tok = a.cu_q[k.seq];
-  k.kv_len = a.seq_lens_k[k.seq];
-  k.nb = (k.kv_len + HY_BLOCK - 1) / HY_BLOCK;            // as the plan counts them
-  k.bt = a.block_tables + (size_t)(a.seq_bt_row ? a.seq_bt_row[k.seq] : k.seq) * a.bt_pitch;
+HY_DEVICE SeqInfo seq_info(const Args& a, const PlanView& v, int seq) {
+  return SeqInfo{v.dec_blocks[seq], a.cu_q[seq], a.seq_lens_k[seq], a.seq_bt_row ? a.seq_bt_row[seq] : seq};
 }
-// The place of flattened block f: in sequence seq (>= 0), or in the last sequence that
-// starts at or before f, found by the whole warp 32 sequences (or runs of 32^n) at a time.
-HY_DEVICE Cursor cursor_at(const Args& a, const PlanView& v, int seq, int f) {
-  Cursor k;
-  k.seq = seq;
-  if (seq < 0) {
-    const int lane = threadIdx.x & 31;
-    int lo = 0, step = 1;
-    while ((long)step * 32 < a.num_seqs) step *= 32;
-    for (; step >= 1; step >>= 5) {
-      const long i = lo + (long)lane * step;
-      const bool le = i < a.num_seqs && v.dec_blocks[i] * a.kv_heads <= f;
-      lo += (31 - __clz(__ballot_sync(0xffffffffu, le) | 1u)) * step;
+// The search of cursor_at begins with sequences `top_step` apart, one per lane; they are
+// loaded before the kernel knows whether it has decode work.
+HY_DEVICE int top_step(const Args& a) {
+  int step = 1;
+  while ((long)step * 32 < a.num_seqs) step *= 32;
+  return step;
+}
+
+HY_DEVICE SeqInfo seq_top(const Args& a, const PlanView& v) {
+  return seq_info(a, v, (int)min((threadIdx.x & 31) * (long)top_step(a), a.num_seqs - 1L));
+}
+
+HY_DEVICE void cursor_sequence(const Args& a, Cursor& k, const SeqInfo& s) {
+  k.first = s.first;
+  k.tok = s.tok;
+  k.kv_len = s.kv_len;
+  k.nb = (s.kv_len + HY_BLOCK - 1) / HY_BLOCK;            // as the plan counts them
+  k.row = s.row;
+}
+// The place of flattened block f: the last sequence that starts at or before it, found
+// by the whole warp 32 sequences (or runs of 32^n) at a time.
+HY_DEVICE Cursor cursor_at(const Args& a, const PlanView& v, const SeqInfo& top, int f) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0;
+  SeqInfo s = top;
+  for (int step = top_step(a);; step >>= 5) {
+    const long i = lo + (long)lane * step;
+    const bool le = i < a.num_seqs && s.first * a.kv_heads <= f;
+    const int at = 31 - __clz(__ballot_sync(0xffffffffu, le) | 1u);
+    lo += at * step;
+    if (step == 1) {
+      s = SeqInfo{__shfl_sync(0xffffffffu, s.first, at), __shfl_sync(0xffffffffu, s.tok, at),
+                  __shfl_sync(0xffffffffu, s.kv_len, at), __shfl_sync(0xffffffffu, s.row, at)};
+      break;
     }
-    k.seq = lo;
+    s = seq_info(a, v, (int)min(lo + (long)lane * (step >> 5), a.num_seqs - 1L));
   }
-  cursor_sequence(a, v, k);
-  const int in = f - v.dec_blocks[k.seq] * a.kv_heads;
+  Cursor k;
+  k.seq = lo;
+  cursor_sequence(a, k, s);
+  const int in = f - s.first * a.kv_heads;
   k.g = in / k.nb;
   k.b = in - k.g * k.nb;
   return k;
@@ -156,11 +184,11 @@ HY_DEVICE void cursor_next_pair(const Args& a, const PlanView& v, Cursor& k) {
   do {
     ++k.seq;
   } while (v.dec_blocks[k.seq + 1] == v.dec_blocks[k.seq]);
-  cursor_sequence(a, v, k);
+  cursor_sequence(a, k, seq_info(a, v, k.seq));
 }
 
-// One warp: key blocks [f0, f1) of the flattened list, pair by pair, two blocks (32 keys)
-// at a time.
+// One warp: n_blocks key blocks of the flattened list from cur[0] (= cur[1]) on, pair by pair, two blocks
+// (32 keys) at a time.
 //
 // Scores are computed transposed, S^T = K Q^T (16 keys x 8 columns, 4 of them heads),
 // and so is the output, O^T = V^T P^T: the codes then fill the 16-row operand of
@@ -177,19 +205,17 @@ HY_DEVICE void cursor_next_pair(const Args& a, const PlanView& v, Cursor& k) {
 // Lane (r, c) = (lane / 4, lane % 4) with c < 2 ends with heads 2 c + k (k = 0, 1) at
 // dimensions 8 r + i and 64 + 8 r + i.  ring_pos: the ring's next stage, ring_par the
 // parity of its next pass.  Returns false if a wait ran out.
-HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, int f0, int f1,
-                           uint8_t* ring_ptr, float* part, Part* parts, uint64_t* bars,
+HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], int n_blocks, uint8_t* ring_ptr,
+                           float* part, Part* parts, uint64_t* bars,
                            uint32_t& ring_pos, uint32_t& ring_par) {
   const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  if (f0 >= f1) return true;
+  if (n_blocks == 0) return true;
   const uint32_t ring = smem_u32(ring_ptr);
-  Cursor k = cursor_at(a, v, seq, f0);                    // the pair being computed
-  Cursor ld = k;                                          // the next block to load
-  int to_load = f1 - f0, left = to_load;
+  int to_load = n_blocks, left = n_blocks;
   uint4 qraw[4];                                          // this lane's part of Q
   auto load_q = [&]() {
     const __nv_bfloat16* qp =
-        a.q + ((size_t)k.tok * a.q_heads + k.g * HY_GROUP + r) * HY_HEAD_DIM + 16 * c;
+        a.q + ((size_t)cur[0].tok * a.q_heads + cur[0].g * HY_GROUP + r) * HY_HEAD_DIM + 16 * c;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       qraw[i] = r < HY_GROUP ? *reinterpret_cast<const uint4*>(qp + 64 * (i >> 1) + 8 * (i & 1))
@@ -205,16 +231,21 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, int f0, in
   auto issue = [&]() {
     if (to_load == 0) return;
     if (run == 0) {
+      Cursor ld = cur[1];
       if (ld.b == ld.nb) cursor_next_pair(a, v, ld);
       turn = 0;
       run = min(min(32, to_load), ld.nb - ld.b);
-      int blk = lane < run && ld.b + lane < a.bt_pitch ? __ldg(ld.bt + ld.b + lane) : -1;
+      int blk = lane < run && ld.b + lane < a.bt_pitch
+                    ? __ldg(a.block_tables + (size_t)ld.row * a.bt_pitch + ld.b + lane) : -1;
       if (blk < 0 || blk >= a.num_blocks) {
         if (lane < run) hy_flag(a.err, HY_ERR_BOUNDS);
         blk = 0;
       }
       src = a.cache + q4_tile(blk, ld.g, 0, a.kv_heads);
       ld.b += run;
+      __syncwarp();                                       // cur[1] is read
+      if (lane == 0) cur[1] = ld;
+      __syncwarp();
     }
     const int n = min(2, run);
     if (lane == turn) mbar_arrive_expect_tx(&bars[put], n * BLK_BYTES);
@@ -243,11 +274,10 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, int f0, in
   int pending = 0;
 #pragma unroll 1
   while (left > 0) {
-    const int n = min(left, k.nb - k.b), b_first = k.b;   // this pair's blocks in the range
+    const int n = min(left, cur[0].nb - cur[0].b);        // this pair's blocks in the range
     left -= n;
-    // whole blocks here, and the keys of the last one if it is here and partial
-    const int rest = b_first + n == k.nb ? k.kv_len & (HY_BLOCK - 1) : 0;
-    const int full = rest ? n - 1 : n;
+    // those that are full: the pair's last one may not be
+    const int full = cur[0].b + n == cur[0].nb && (cur[0].kv_len & (HY_BLOCK - 1)) ? n - 1 : n;
     // Q in fp16 (q4_query_scale): lane (r, c) holds head r's words 2 c, 2 c + 1 (dimensions
     // 16 c ..) of both halves; rows 4-7 are zero.  Codes in bits 0-3 meet 2^14 q, codes
     // in bits 4-7 2^10 q, so that a score comes out as 2^-10 code . q.
@@ -351,7 +381,7 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, int f0, in
       if (i + 2 > full) {                                 // keys past the end: their rows hold anything
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const int keys = i + b < full ? HY_BLOCK : i + b < n ? rest : 0;
+          const int keys = i + b < full ? HY_BLOCK : i + b < n ? cur[0].kv_len & (HY_BLOCK - 1) : 0;
           if (keyA >= keys) { x[b][0] = x[b][1] = -INFINITY; va[b] = make_uint2(0u, 0u); }
           if (keyA + 4 >= keys) { x[b][2] = x[b][3] = -INFINITY; vb[b] = make_uint2(0u, 0u); }
         }
@@ -439,7 +469,8 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, int f0, in
     if (!ok) break;
 
     // the pair's result, or a partial of it
-    const bool whole = b_first == 0 && n == k.nb;
+    Cursor k = cur[0];
+    const bool whole = n == k.nb;
     const int slot = first_pair ? 0 : 1;
     float inv[2];
 #pragma unroll
@@ -483,11 +514,14 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, int seq, int f0, in
           *reinterpret_cast<float2*>(part + slot * PART_FLOATS + HY_GROUP * HY_HEAD_DIM + 2 * (2 * c + e)) =
               make_float2(m[e], l[e]);
     }
-    if (!whole && lane == 0) parts[slot] = Part{k.seq * a.kv_heads + k.g, n, k.nb, k.tok};
+    if (!whole && lane == 0) 
+      parts[slot] = Part{k.seq * a.kv_heads + k.g, n, k.nb, k.first * a.kv_heads + k.g * k.nb, k.tok};
     first_pair = false;
-    k.b += n;
     if (left > 0) {
       cursor_next_pair(a, v, k);
+      __syncwarp();                                       // cur[0] is read
+      if (lane == 0) cur[0] = k;
+      __syncwarp();
       load_q();
     }
   }
@@ -520,16 +554,31 @@ struct Units {            // `total` blocks in n units whose sizes differ by at 
   }
 };
 
-HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units, int unit,
-                           int only_seq, int f0, int f1, uint8_t* payload, Shared& sh,
-                           uint32_t& ring_pos, uint32_t& ring_par) {
+// (small: a unit is the pair `unit` / `unit` % kv_heads alone)
+HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units, int unit, bool small,
+                           const SeqInfo& top, uint8_t* payload, Shared& sh, uint32_t& ring_pos,
+                           uint32_t& ring_par) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   float* parts = reinterpret_cast<float*>(payload + NW * RING_BYTES);
   if (lane < 2) sh.part[2 * warp + lane].pair = -1;
+  const int f0 = small ? 0 : units.start(unit);
+  Cursor k;
+  int n;
+  if (small) {
+    k.seq = unit / a.kv_heads;
+    k.g = unit - k.seq * a.kv_heads;
+    cursor_sequence(a, k, seq_info(a, v, k.seq));
+    n = a.cu_q[k.seq + 1] - k.tok == 1 ? k.nb : 0;        // no decode token: no blocks
+  } else {
+    n = units.start(unit + 1) - f0;
+  }
+  const int per = n / NW, more = n - per * NW;            // the first `more` warps take one more
+  const int at = warp * per + min(warp, more), count = per + (warp < more);
+  if (small) k.b = at;
+  else if (count > 0) k = cursor_at(a, v, top, f0 + at);
+  if (lane < 2) sh.cur[warp][lane] = k;
   __syncwarp();
-  const int n = f1 - f0, per = n / NW, more = n - per * NW;       // the first `more` warps take one more
-  const int w0 = f0 + warp * per + min(warp, more);
-  const bool ok = decode_warp(a, v, only_seq, w0, w0 + per + (warp < more), payload + warp * RING_BYTES,
+  const bool ok = decode_warp(a, v, sh.cur[warp], count, payload + warp * RING_BYTES,
                               parts + warp * 2 * PART_FLOATS, sh.part + 2 * warp, sh.bar[warp],
                               ring_pos, ring_par);
   if (__syncthreads_or(!ok)) return false;
@@ -582,7 +631,7 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
       *reinterpret_cast<uint2*>(a.out + ((size_t)tok * a.q_heads + g * HY_GROUP + head) * HY_HEAD_DIM + 4 * lane) =
           make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
     } else {
-      const size_t slot = 2 * unit + (v.dec_blocks[seq] * a.kv_heads + g * nb > f0);
+      const size_t slot = 2 * unit + (__shfl_sync(0xffffffffu, mine.first, i) > f0);
       __stcg(reinterpret_cast<float4*>(v.part_o + (slot * HY_GROUP + head) * HY_HEAD_DIM) + lane, acc);
       if (lane == 0) __stcg(v.part_ml + slot * HY_GROUP + head, make_float2(M, L));
     }
@@ -612,21 +661,32 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
   for (int j = 0; j < n_open; ++j) {
     if (!((last >> j) & 1)) continue;
     const Part p = sh.part[open_at[j]];
-    const int seq = p.pair / a.kv_heads, g = p.pair - seq * a.kv_heads;
-    const int F0 = v.dec_blocks[seq] * a.kv_heads + g * p.nb;
-    const int u0 = units.of(F0), u1 = units.of(F0 + p.nb - 1);
-    const int inside = F0 > units.start(u0), h = tid >> 7;
+    const int g = p.pair % a.kv_heads, h = tid >> 7;
+    const int u0 = units.of(p.first), u1 = units.of(p.first + p.nb - 1);
+    const int inside = p.first > units.start(u0);
+    auto slot = [&](int u) { return (size_t)(2 * u + (u == u0 ? inside : 0)); };
     float M = -INFINITY, L = 0.f, acc = 0.f;
-#pragma unroll 8
-    for (int u = u0; u <= u1; ++u) {                      // none of them is empty
-      const size_t slot = 2 * u + (u == u0 ? inside : 0);
-      const float2 e = __ldcg(v.part_ml + slot * HY_GROUP + h);
-      const float po = __ldcg(v.part_o + slot * (HY_GROUP * HY_HEAD_DIM) + tid);
-      const float m_new = fmaxf(M, e.x);
-      const float s0 = m_new == -INFINITY ? 1.f : ex2_ftz(M - m_new);
-      const float s1 = m_new == -INFINITY ? 1.f : ex2_ftz(e.x - m_new);
-      L = fmaf(L, s0, e.y * s1);
-      acc = fmaf(acc, s0, po * s1);
+    for (int c0 = u0; c0 <= u1; c0 += 32) {               // 32 partials (none is empty), one weight per lane
+      const int cnt = min(32, u1 - c0 + 1);
+      const float2 e = lane < cnt ? __ldcg(v.part_ml + slot(c0 + lane) * HY_GROUP + h) : make_float2(-INFINITY, 0.f);
+      float m_new = fmaxf(M, e.x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, o));
+      const float mu = m_new == -INFINITY ? 0.f : m_new, old = ex2_ftz(M - mu);
+      const float w = ex2_ftz(e.x - mu);
+      float lw = w * e.y;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, o);
+      L = fmaf(L, old, lw);
+      acc *= old;
+      for (int i = 0; i < cnt; i += 8) {                  // 8 loads in flight
+        float po[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          po[t] = i + t < cnt ? __ldcg(v.part_o + slot(c0 + i + t) * (HY_GROUP * HY_HEAD_DIM) + tid) : 0.f;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) acc = fmaf(__shfl_sync(0xffffffffu, w, (i + t) & 31), po[t], acc);
+      }
       M = m_new;
     }
     a.out[((size_t)p.tok * a.q_heads + g * HY_GROUP) * HY_HEAD_DIM + tid] = __float2bfloat16_rn(acc / L);
@@ -942,11 +1002,11 @@ __device__ bool prefill_item(const Args& a, const PlanView& v, int item, uint8_t
 // share.  Returns false if a wait ran out.
 constexpr int MIXED_UNITS = 3;
 __device__ bool decode_all(const Args& a, const PlanView& v, int n_pre, int n_pairs, int blocks,
-                           uint8_t* payload, Shared& sh) {
+                           SeqInfo top, uint8_t* payload, Shared& sh) {
   uint32_t ring_pos = 0, ring_par = 0;
   const int total = blocks * a.kv_heads;                  // below 2^31: the host checks the tables' size
   if (total == 0) return true;
-  const Units units(total, n_pairs > 0 ? n_pairs : n_pre > 0 ? MIXED_UNITS * (int)gridDim.x : (int)gridDim.x);
+  const Units units(total, n_pre > 0 ? MIXED_UNITS * (int)gridDim.x : (int)gridDim.x);
   int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
   int u = blockIdx.x;
   for (;;) {
@@ -955,18 +1015,10 @@ __device__ bool decode_all(const Args& a, const PlanView& v, int n_pre, int n_pa
       __syncthreads();
       u = sh.unit;
       __syncthreads();
+      top = seq_top(a, v);
     }
-    if (u >= units.n) return true;
-    int only_seq = -1;
-    int f0 = units.start(u), f1 = units.start(u + 1);
-    if (n_pairs > 0) {
-      only_seq = u / a.kv_heads;
-      const int p0 = v.dec_blocks[only_seq], nb = v.dec_blocks[only_seq + 1] - p0;
-      f0 = p0 * a.kv_heads + (u - only_seq * a.kv_heads) * nb;
-      f1 = f0 + nb;
-    }
-    if (!decode_unit(a, v, units, u, only_seq, f0, f1, payload, sh, ring_pos, ring_par))
-      return false;
+    if (u >= (n_pairs > 0 ? n_pairs : units.n)) return true;
+    if (!decode_unit(a, v, units, u, n_pairs > 0, top, payload, sh, ring_pos, ring_par)) return false;
     if (n_pre == 0) return true;
   }
 }
@@ -998,6 +1050,7 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(Args a, PlanView v) {
   hy_grid_wait();
   hy_grid_trigger();
   const uint64_t keep = l2_keep_policy();
+  const SeqInfo top = seq_top(a, v);
   const int n_pre = ld_keep(v.header, keep), n_pairs = ld_keep(v.header + 4, keep);
   const int blocks = ld_keep(v.header + 5, keep);         // key blocks of the decode sequences
   int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
@@ -1027,7 +1080,7 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(Args a, PlanView v) {
       tmem_dealloc(tmem, TMEM_COLS);
     }
   }
-  if (ok) decode_all(a, v, n_pre, n_pairs, blocks, payload, sh);
+  if (ok) decode_all(a, v, n_pre, n_pairs, blocks, top, payload, sh);
   __syncthreads();
   if (n_pre > 0 && threadIdx.x == 0) {
     __threadfence();                                      // the last CTA out resets the counters
