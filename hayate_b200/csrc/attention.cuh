@@ -95,7 +95,7 @@ cudaError_t hy_launch_attn_fp32(const float* q, float* out, int T, int q_heads, 
                                 cudaStream_t st);
 
 // The 4-bit cache (attention_q4.cu); cache_layer: the layer's first tile.
-cudaError_t hy_launch_attn_q4_bf16(const void* q, void* out, int q_heads, int kv_heads,
+cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap& q_map, const void* q, void* out, int q_heads, int kv_heads,
                                    const void* cache_layer, int num_blocks, int layer,
                                    const int32_t* block_tables, int bt_pitch,
                                    const int32_t* seq_bt_row, const int32_t* cu_q,

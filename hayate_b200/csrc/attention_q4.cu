@@ -38,11 +38,12 @@ constexpr int DEC_SMEM = NW * (RING_BYTES + 2 * PART_FLOATS * 4);
 constexpr float RESCALE_LOG2 = 8.0f;                      // see decode_warp
 
 // Prefill: warps 0-3 / 4-7 softmax of sub-tile 0 / 1, 8-11 expand, 12 / 13 issue the
-// products of sub-tile 0 / 1.  Sub-tile X, row r: query head 4 g + 2 X + r / 64, token
+// products of sub-tile 0 / 1, 14 deals out items and loads Q.  Sub-tile X, row r: query head 4 g + 2 X + r / 64, token
 // t0 + r % 64.  Q is [column half][128 rows][64] per sub-tile, a K or V ring slot [column
 // half][64 keys][64], rows of 128 bytes with the 128-byte swizzle: the K-major operand
 // of S = Q K^T and the MN-major operand of P V.
-constexpr int EXP_WARP = 8, MMA_WARP = 12;
+constexpr int EXP_WARP = 8, MMA_WARP = 12, ITEM_WARP = 14;
+constexpr int ITEM_READERS = 14;                          // the warps before ITEM_WARP
 constexpr int PS = 4;                                     // K and V ring slots
 constexpr int Q_BYTES = 128 * HY_HEAD_DIM * 2;            // Q of one sub-tile: 32 KB
 constexpr int KV_BYTES = PRE_KEYS * HY_HEAD_DIM * 2;      // K or V of one tile: 16 KB
@@ -68,6 +69,12 @@ struct Args {
   int32_t* err;
 };
 
+// A prefill item (or a key-range piece of one): query tokens t0 .. t0 + nrows - 1 of a
+// sequence, KV head g, key tiles [tlo, thi).
+struct PreItem {
+  int seq, g, t0, row0, nrows, prefix, kv_end, tlo, thi, w;   // seq -1: no more items
+};
+
 // A place in the flattened list of key blocks (sequence, head, block) of the step's
 // decode sequences, with what a warp needs of the sequence.  Warps keep theirs in shared
 // memory: it is read once per pair, and the key loop needs the registers.
@@ -90,17 +97,23 @@ struct Shared {
   int last;               // bit j: this CTA finished pair j of its two open ones
   Part part[2 * NW];      // each warp's two parts, in block order
   Cursor cur[NW][2];      // each warp's pair computed, and next block to load
-  // prefill; ring barriers complete once per use of their slot, the others once
-  // per key tile (per use of their S buffer), qfull once per item
+  // prefill; ring barriers complete once per use of their slot, sfull, pfull and odone
+  // once per use of their S buffer, the others once per item
   uint64_t full[PS];      // K and V of a tile expanded (one arrival per expanding warp)
   uint64_t free_[PS];     // both P V products of the slot's tile are done
   uint64_t sfull[2][2];   // S_X[b] complete
   uint64_t pfull[2][2];   // P_X[b] written (one arrival per softmax warp)
   uint64_t odone[2][2];   // O_X += P_X[b] V complete
   uint64_t drain[2];      // error path: everything an issuing warp issued is complete
-  uint64_t qfull;         // Q written (one arrival per softmax warp)
+  uint64_t qraw;          // Q landed as bf16 (TMA transaction bytes)
+  uint64_t qfull;         // Q is fp16 (one arrival per softmax warp)
+  uint64_t ofree[2];      // O_X is read out (one arrival per softmax warp)
+  uint64_t qfree;         // both sub-tiles' last S is done (one commit each)
+  uint64_t itemfull;      // item[n % 2] is the CTA's item n
+  uint64_t itemfree;      // every warp has read it (one arrival each)
+  PreItem item[2];
   uint32_t tmem_base;
-  int pre_item, pre_last;
+  int pre_last;
 };
 
 // Row of the score matrix S^T (row r or r + 8 of the 16-key block) -> key of the
@@ -696,9 +709,6 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
 }
 
 // ------------------------------------------------------------------ prefill item
-struct PreItem {
-  int seq, g, t0, row0, nrows, prefix, kv_len, kv_end, tlo, thi, w;
-};
 HY_DEVICE PreItem pre_item_geom(const Args& a, const PlanView& v, int item) {
   const int4 it = v.pre_sorted[item];
   PreItem p;
@@ -708,8 +718,7 @@ HY_DEVICE PreItem pre_item_geom(const Args& a, const PlanView& v, int item) {
   p.w = it.w;
   p.row0 = a.cu_q[p.seq];
   const int q_len = a.cu_q[p.seq + 1] - p.row0;
-  p.kv_len = a.seq_lens_k[p.seq];
-  p.prefix = p.kv_len - q_len;
+  p.prefix = a.seq_lens_k[p.seq] - q_len;
   p.nrows = min(PRE_QROWS, q_len - p.t0);
   p.kv_end = p.prefix + p.t0 + p.nrows;                   // keys its last row sees
   pre_piece_range(p.w, (p.kv_end + PRE_KEYS - 1) / PRE_KEYS, p.tlo, p.thi);
@@ -763,237 +772,289 @@ HY_DEVICE void expand_row(const RowCodes& x, uint8_t* slot, int key) {
   }
 }
 
-// One prefill item, all warps of the CTA (roles as above).  The products, barriers
-// and softmax follow attention.cu's prefill: S(t + 1) is issued while the softmax
-// works on S(t); the softmax writes P(t) over S(t) and waits for P V(t - 1) only to
-// rescale O.  c = c0 + t counts key tiles over all items of the launch.
+// The CTA's prefill items, taken from the counter `next` until there are no more.  Each
+// role runs through the items at its own pace, ahead of the others as far as the
+// barriers let it: the expanding warps fill the ring for the next item, whose Q is
+// loaded as soon as the last score tile of this one is done, while the softmax warps
+// write this one's output.
+// The products, barriers and softmax follow attention.cu's prefill: S(t + 1) is issued
+// while the softmax works on S(t); the softmax writes P(t) over S(t) and waits for
+// P V(t - 1) only to rescale O.  c counts key tiles, n items, over the launch.
 // Returns false if a wait ran out; the roles then drain what they issued.
-__device__ bool prefill_item(const Args& a, const PlanView& v, int item, uint8_t* payload,
-                             Shared& sh, uint32_t tmem, uint32_t& ctr, uint32_t qpar) {
+__device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanView& v, int n_pre,
+                            int* next, uint8_t* payload, Shared& sh, uint32_t tmem) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const PreItem P = pre_item_geom(a, v, item);
-  const int ntiles = P.thi - P.tlo;
   const uint32_t sbase = smem_u32(payload);
-  const uint32_t c0 = ctr;
-  ctr += ntiles;
   bool ok = true;
+  uint32_t c0 = 0;
+  // the CTA's item n, for a whole warp
+  auto item_at = [&](uint32_t n) {
+    PreItem p;
+    ok = __all_sync(0xffffffffu, mbar_wait(&sh.itemfull, n & 1, a.err));
+    p = sh.item[n & 1];
+    if (!ok) p.seq = -1;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.itemfree);
+    return p;
+  };
 
-  if (warp >= EXP_WARP && warp < MMA_WARP) {
-    const int t128 = tid - EXP_WARP * 32, part = t128 >> 6, key = t128 & 63;
-    const int32_t* bt = a.block_tables + (size_t)(a.seq_bt_row ? a.seq_bt_row[P.seq] : P.seq) * a.bt_pitch;
-    uint8_t* ring = payload + (part ? V_OFF : K_OFF);
-    RowCodes cur, nxt;
-    int pos = P.tlo * PRE_KEYS + key;
-    load_row(a, P, part, pos, tile_block(a, P, bt, pos), nxt);
-    int blk = ntiles > 1 ? tile_block(a, P, bt, pos + PRE_KEYS) : -1;
-    for (int t = 0; t < ntiles; ++t) {
-      cur = nxt;
-      pos += PRE_KEYS;
-      if (t + 1 < ntiles) load_row(a, P, part, pos, blk, nxt);
-      if (t + 2 < ntiles) blk = tile_block(a, P, bt, pos + PRE_KEYS);
-      const uint32_t c = c0 + t, slot = c % PS;
-      ok = __all_sync(0xffffffffu, mbar_wait(&sh.free_[slot], ((c / PS) & 1) ^ 1, a.err));
-      if (!ok) break;
-      expand_row(cur, ring + slot * KV_BYTES, key);
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.full[slot]);
-    }
-  } else if (warp == MMA_WARP || warp == MMA_WARP + 1) {
-    const int X = warp - MMA_WARP;
+  if (warp == ITEM_WARP) {
     if (lane == 0) {
-      constexpr uint32_t ID_S = tc_idesc_f16(128, PRE_KEYS, false);
-      constexpr uint32_t ID_O = tc_idesc_f16(128, HY_HEAD_DIM, true);
-      const uint64_t dQ = tc_desc_sw128(sbase + X * Q_BYTES, 16, 1024);
-      ok = mbar_wait(&sh.qfull, qpar, a.err);
-      tc_fence_after();
-      for (int t = 0; t <= ntiles && ok; ++t) {
-        if (t < ntiles) {                                 // S_X(t) = Q_X K_t^T
-          const uint32_t c = c0 + t, slot = c % PS;
-          ok = mbar_wait(&sh.full[slot], (c / PS) & 1, a.err);
-          if (!ok) break;
-          // S(t) goes over P(t - 2): products of different shapes are not ordered among
-          // themselves, so the one that reads it is waited for (it was issued a softmax
-          // tile ago; the wait also tells the softmax, which waits for S(t), that it is done)
-          if (t > 1) ok = mbar_wait(&sh.odone[X][c & 1], ((c - 2) >> 1) & 1, a.err);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t dK = tc_desc_sw128(sbase + K_OFF + slot * KV_BYTES, 16, 1024);
-#pragma unroll
-          for (int kk = 0; kk < HY_HEAD_DIM / 16; ++kk)
-            tc_mma_bf16(tmem + tm_s(X, c & 1),
-                        dQ + (uint64_t)((((kk >> 2) * (Q_BYTES / 2)) + (kk & 3) * 32) >> 4),
-                        dK + (uint64_t)((((kk >> 2) * (KV_BYTES / 2)) + (kk & 3) * 32) >> 4), ID_S,
-                        kk > 0);
-          tc_commit(&sh.sfull[X][c & 1]);
-        }
-        if (t > 0) {                                      // O_X += P_X(t - 1) V_{t-1}
-          const uint32_t c = c0 + t - 1, slot = c % PS;
-          ok = mbar_wait(&sh.pfull[X][c & 1], (c >> 1) & 1, a.err);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t dV = tc_desc_sw128(sbase + V_OFF + slot * KV_BYTES, KV_BYTES / 2, 1024);
-#pragma unroll
-          for (int kk = 0; kk < PRE_KEYS / 16; ++kk)
-            tc_mma_bf16_ta(tmem + TM_O + 128 * X, tmem + tm_s(X, c & 1) + 8 * kk,
-                           dV + (uint64_t)((kk * 2048) >> 4), ID_O, (t > 1 || kk > 0));
-          tc_commit(&sh.odone[X][c & 1]);
-          tc_commit(&sh.free_[slot]);
-        }
-      }
-      if (!ok) {                                          // let every issued product finish
-        tc_commit(&sh.drain[X]);
-        mbar_wait(&sh.drain[X], 0, nullptr);
+      for (uint32_t n = 0; ok; ++n) {
+        const int k = atomicAdd(next, 1);
+        PreItem N;
+        if (k < n_pre) N = pre_item_geom(a, v, k);
+        else N.seq = -1;
+        if (n > 0) ok = mbar_wait(&sh.itemfree, (n - 1) & 1, a.err);
+        if (!ok) break;
+        sh.item[n & 1] = N;
+        mbar_arrive(&sh.itemfull);
+        if (N.seq < 0) break;
+        if (n > 0) ok = mbar_wait(&sh.qfree, (n - 1) & 1, a.err);
+        if (!ok) break;
+        fence_proxy_async();
+        mbar_arrive_expect_tx(&sh.qraw, 2 * Q_BYTES);
+        for (int X = 0; X < 2; ++X)
+          tma_load_4d(payload + X * Q_BYTES, q_map, 0, N.row0 + N.t0, N.g * HY_GROUP + 2 * X, 0, &sh.qraw);
+        ok = mbar_wait(&sh.qraw, n & 1, a.err);           // landed before this warp can leave
       }
     }
     __syncwarp();
+  } else if (warp >= EXP_WARP && warp < MMA_WARP) {
+    const int t128 = tid - EXP_WARP * 32, part = t128 >> 6, key = t128 & 63;
+    uint8_t* ring = payload + (part ? V_OFF : K_OFF);
+    for (uint32_t n = 0; ok; ++n) {
+      const PreItem P = item_at(n);
+      if (P.seq < 0) break;
+      const int ntiles = P.thi - P.tlo;
+      const int32_t* bt = a.block_tables + (size_t)(a.seq_bt_row ? a.seq_bt_row[P.seq] : P.seq) * a.bt_pitch;
+      RowCodes cur, nxt;
+      int pos = P.tlo * PRE_KEYS + key;
+      load_row(a, P, part, pos, tile_block(a, P, bt, pos), nxt);
+      int blk = ntiles > 1 ? tile_block(a, P, bt, pos + PRE_KEYS) : -1;
+      for (int t = 0; t < ntiles; ++t) {
+        cur = nxt;
+        pos += PRE_KEYS;
+        if (t + 1 < ntiles) load_row(a, P, part, pos, blk, nxt);
+        if (t + 2 < ntiles) blk = tile_block(a, P, bt, pos + PRE_KEYS);
+        const uint32_t c = c0 + t, slot = c % PS;
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.free_[slot], ((c / PS) & 1) ^ 1, a.err));
+        if (!ok) break;
+        expand_row(cur, ring + slot * KV_BYTES, key);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.full[slot]);
+      }
+      c0 += ntiles;
+    }
+  } else if (warp == MMA_WARP || warp == MMA_WARP + 1) {
+    const int X = warp - MMA_WARP;
+    constexpr uint32_t ID_S = tc_idesc_f16(128, PRE_KEYS, false);
+    constexpr uint32_t ID_O = tc_idesc_f16(128, HY_HEAD_DIM, true);
+    const uint64_t dQ = tc_desc_sw128(sbase + X * Q_BYTES, 16, 1024);
+    for (uint32_t n = 0; ok; ++n) {
+      const PreItem P = item_at(n);
+      if (P.seq < 0) break;
+      const int ntiles = P.thi - P.tlo;
+      if (lane == 0) {
+        ok = mbar_wait(&sh.qfull, n & 1, a.err);
+        for (int t = 0; t <= ntiles && ok; ++t) {
+          if (t < ntiles) {                               // S_X(t) = Q_X K_t^T
+            const uint32_t c = c0 + t, slot = c % PS;
+            ok = mbar_wait(&sh.full[slot], (c / PS) & 1, a.err);
+            // S(t) goes over P(t - 2): products of different shapes are not ordered among
+            // themselves, so the one that reads it is waited for (it was issued a softmax
+            // tile ago; the wait also tells the softmax, which waits for S(t), that it is done)
+            if (ok && c > 1) ok = mbar_wait(&sh.odone[X][c & 1], ((c - 2) >> 1) & 1, a.err);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t dK = tc_desc_sw128(sbase + K_OFF + slot * KV_BYTES, 16, 1024);
+#pragma unroll
+            for (int kk = 0; kk < HY_HEAD_DIM / 16; ++kk)
+              tc_mma_bf16(tmem + tm_s(X, c & 1),
+                          dQ + (uint64_t)((((kk >> 2) * (Q_BYTES / 2)) + (kk & 3) * 32) >> 4),
+                          dK + (uint64_t)((((kk >> 2) * (KV_BYTES / 2)) + (kk & 3) * 32) >> 4), ID_S,
+                          kk > 0);
+            tc_commit(&sh.sfull[X][c & 1]);
+            if (t == ntiles - 1) tc_commit(&sh.qfree);
+          }
+          if (t > 0) {                                    // O_X += P_X(t - 1) V_{t-1}
+            const uint32_t c = c0 + t - 1, slot = c % PS;
+            ok = mbar_wait(&sh.pfull[X][c & 1], (c >> 1) & 1, a.err);
+            if (ok && t == 1 && n > 0) ok = mbar_wait(&sh.ofree[X], (n - 1) & 1, a.err);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t dV = tc_desc_sw128(sbase + V_OFF + slot * KV_BYTES, KV_BYTES / 2, 1024);
+#pragma unroll
+            for (int kk = 0; kk < PRE_KEYS / 16; ++kk)
+              tc_mma_bf16_ta(tmem + TM_O + 128 * X, tmem + tm_s(X, c & 1) + 8 * kk,
+                             dV + (uint64_t)((kk * 2048) >> 4), ID_O, (t > 1 || kk > 0));
+            tc_commit(&sh.odone[X][c & 1]);
+            tc_commit(&sh.free_[slot]);
+          }
+        }
+        if (!ok) {                                        // let every issued product finish
+          tc_commit(&sh.drain[X]);
+          mbar_wait(&sh.drain[X], 0, nullptr);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      c0 += ntiles;
+    }
   } else if (warp < EXP_WARP) {                           // softmax: thread = row = TMEM lane
     const int X = warp >> 2, r = (warp & 3) * 32 + lane, j = r & 63;
-    const int head = P.g * HY_GROUP + 2 * X + (r >> 6);
-    const size_t at = ((size_t)(P.row0 + P.t0 + j) * a.q_heads + head) * HY_HEAD_DIM;
-    const bool real = j < P.nrows;
-    float sl2;                                            // scale to log2 units of this row
-    {                                                     // Q row r in fp16 (q4_query_scale)
-      uint4 u[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        u[i] = real ? reinterpret_cast<const uint4*>(a.q + at)[i] : make_uint4(0, 0, 0, 0);
-      float amax = 0.f, down, up;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float lo = __uint_as_float(w[k] << 16), hi = __uint_as_float(w[k] & 0xffff0000u);
-          amax = fmax3f(amax, fabsf(lo), fabsf(hi));
-        }
-      }
-      q4_query_scale(amax, down, up);
-      // not 0 (a scale of 0, a row of tiny elements): masked scores are -inf times it,
-      // and the scores it multiplies, at most 2^24, stay 0 to fp32 either way
-      sl2 = fmaxf(a.scale_log2 * up, 1e-30f);
-      uint8_t* row = payload + X * Q_BYTES + r * 128;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-        uint32_t y[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          y[k] = q4_as_u32(__floats2half2_rn(__uint_as_float(w[k] << 16) * down,
-                                             __uint_as_float(w[k] & 0xffff0000u) * down));
-        *reinterpret_cast<uint4*>(row + (i >> 3) * (Q_BYTES / 2) + (((i & 7) ^ (r & 7)) << 4)) =
-            make_uint4(y[0], y[1], y[2], y[3]);
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.qfull);
-    }
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tO = tmem + lane_base + TM_O + 128 * X;
-    const int lim = P.prefix + P.t0 + j;                  // last key row r may see
-    float m = NEG_INF, l = 0.f;                           // m in scaled log2 units
-    for (int t = 0; t < ntiles && ok; ++t) {
-      const uint32_t c = c0 + t;
-      const uint32_t tS = tmem + lane_base + tm_s(X, c & 1);
-      ok = __all_sync(0xffffffffu, mbar_wait(&sh.sfull[X][c & 1], (c >> 1) & 1, a.err));
-      if (!ok) break;
-      tc_fence_after();
-      float s[64];
-      float (&s_lo)[32] = *reinterpret_cast<float(*)[32]>(&s[0]);
-      float (&s_hi)[32] = *reinterpret_cast<float(*)[32]>(&s[32]);
-      tmem_ld32(tS, s_lo);
-      tmem_ld32(tS + 32, s_hi);
-      tmem_wait_ld(s_lo);
-      tmem_wait_ld(s_hi);
-      const int kb = (P.tlo + t) * PRE_KEYS;
-      if (kb + PRE_KEYS - 1 > P.prefix + P.t0) {          // the tile reaches the diagonal or the end
+    uint8_t* q_row = payload + X * Q_BYTES + r * 128;
+    for (uint32_t n = 0;; ++n) {
+      PreItem P = {};
+      if (ok) P = item_at(n);
+      if (ok && P.seq >= 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.qraw, n & 1, a.err));
+      // the softmax warps leave together: pieces of an item meet at a barrier of theirs
+      if (named_sync_or(PRE_PIECE_BAR, PRE_ROWS, !ok)) ok = false;
+      if (!ok || P.seq < 0) break;
+      const int ntiles = P.thi - P.tlo;
+      const bool real = j < P.nrows;                      // rows past the chunk hold other tokens' Q
+      // Q row r to fp16 in place (q4_query_scale)
+      float sl2;                                          // scale to log2 units of this row
+      {
+        float amax = 0.f, down, up;
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (kb + i > lim || kb + i >= P.kv_end) s[i] = NEG_INF;
+        for (int i = 0; i < 16; ++i) {
+          const uint4 u = *reinterpret_cast<const uint4*>(q_row + (i >> 3) * (Q_BYTES / 2) + (((i & 7) ^ (r & 7)) << 4));
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            amax = fmax3f(amax, fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u)));
+        }
+        q4_query_scale(amax, down, up);
+        // not 0 (a scale of 0, a row of tiny elements): masked scores are -inf times it,
+        // and the scores it multiplies, at most 2^24, stay 0 to fp32 either way
+        sl2 = fmaxf(a.scale_log2 * up, 1e-30f);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          uint4* at = reinterpret_cast<uint4*>(q_row + (i >> 3) * (Q_BYTES / 2) + (((i & 7) ^ (r & 7)) << 4));
+          const uint4 u = *at;
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+          uint32_t y[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            y[k] = q4_as_u32(__floats2half2_rn(__uint_as_float(w[k] << 16) * down,
+                                               __uint_as_float(w[k] & 0xffff0000u) * down));
+          *at = make_uint4(y[0], y[1], y[2], y[3]);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.qfull);
       }
-      float mxs[8];                                       // 8 independent chains
+      const int lim = P.prefix + P.t0 + j;                // last key row r may see
+      float m = NEG_INF, l = 0.f;                         // m in scaled log2 units
+      for (int t = 0; t < ntiles; ++t) {
+        const uint32_t c = c0 + t;
+        const uint32_t tS = tmem + lane_base + tm_s(X, c & 1);
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.sfull[X][c & 1], (c >> 1) & 1, a.err));
+        if (!ok) break;
+        tc_fence_after();
+        float s[64];
+        float (&s_lo)[32] = *reinterpret_cast<float(*)[32]>(&s[0]);
+        float (&s_hi)[32] = *reinterpret_cast<float(*)[32]>(&s[32]);
+        tmem_ld32(tS, s_lo);
+        tmem_ld32(tS + 32, s_hi);
+        tmem_wait_ld(s_lo);
+        tmem_wait_ld(s_hi);
+        const int kb = (P.tlo + t) * PRE_KEYS;
+        if (kb + PRE_KEYS - 1 > P.prefix + P.t0) {        // the tile reaches the diagonal or the end
 #pragma unroll
-      for (int k = 0; k < 8; ++k) mxs[k] = fmax3f(s[k], s[8 + k], s[16 + k]);
+          for (int i = 0; i < 64; ++i)
+            if (kb + i > lim || kb + i >= P.kv_end) s[i] = NEG_INF;
+        }
+        float mxs[8];                                     // 8 independent chains
 #pragma unroll
-      for (int i = 24; i < 56; i += 16)
+        for (int k = 0; k < 8; ++k) mxs[k] = fmax3f(s[k], s[8 + k], s[16 + k]);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) mxs[k] = fmax3f(mxs[k], s[i + k], s[i + 8 + k]);
+        for (int i = 24; i < 56; i += 16)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) mxs[k] = fmaxf(mxs[k], s[56 + k]);
-      const float mx = sl2 * fmax3f(fmax3f(mxs[0], mxs[1], mxs[2]), fmax3f(mxs[3], mxs[4], mxs[5]),
-                                    fmaxf(mxs[6], mxs[7]));
-      const bool grow = mx > m + RESCALE_LOG2;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float mnew = grow ? mx : m;
-        const float alpha = mnew == NEG_INF ? 1.f : ex2_ftz(m - mnew);
-        l *= alpha;
-        m = mnew;
-        if (t > 0) {                                      // O holds tiles < t: wait for P V(t - 1)
-          ok = __all_sync(0xffffffffu, mbar_wait(&sh.odone[X][(c & 1) ^ 1], ((c - 1) >> 1) & 1, a.err));
-          tc_fence_after();
+          for (int k = 0; k < 8; ++k) mxs[k] = fmax3f(mxs[k], s[i + k], s[i + 8 + k]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mxs[k] = fmaxf(mxs[k], s[56 + k]);
+        const float mx = sl2 * fmax3f(fmax3f(mxs[0], mxs[1], mxs[2]), fmax3f(mxs[3], mxs[4], mxs[5]),
+                                      fmaxf(mxs[6], mxs[7]));
+        const bool grow = mx > m + RESCALE_LOG2;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float mnew = grow ? mx : m;
+          const float alpha = mnew == NEG_INF ? 1.f : ex2_ftz(m - mnew);
+          l *= alpha;
+          m = mnew;
+          if (t > 0) {                                    // O holds tiles < t: wait for P V(t - 1)
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.odone[X][(c & 1) ^ 1], ((c - 1) >> 1) & 1, a.err));
+            tc_fence_after();
 #pragma unroll 1
-          for (int cc = 0; cc < 4; ++cc) {
-            float o[32];
-            tmem_ld32(tO + 32 * cc, o);
-            tmem_wait_ld(o);
+            for (int cc = 0; cc < 8; ++cc) {
+              float o[16];
+              tmem_ld16(tO + 16 * cc, o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= alpha;
-            tmem_st32(tO + 32 * cc, o);
+              for (int i = 0; i < 16; ++i) o[i] *= alpha;
+              tmem_st16(tO + 16 * cc, o);
+            }
+            tmem_wait_st();
+            if (!ok) break;
           }
-          tmem_wait_st();
+        }
+        const float mneg = (m == NEG_INF) ? 0.f : -m;
+        const float2 sl2v = make_float2(sl2, sl2), mnegv = make_float2(mneg, mneg);
+        uint32_t pk[32];
+        float2 ls[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
+                        make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), sl2v, mnegv);
+          const float p0 = ex2_ftz(x.x), p1 = ex2_ftz(x.y);
+          ls[i & 3] = __fadd2_rn(ls[i & 3], make_float2(p0, p1));
+          pk[i] = q4_as_u32(__floats2half2_rn(p0, p1));
+        }
+        l += ((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y)) + ((ls[2].x + ls[2].y) + (ls[3].x + ls[3].y));
+        tmem_st32u(tS, pk);                               // P(t) over the first 32 columns of S(t)
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.pfull[X][c & 1]);
+      }
+      c0 += ntiles;
+      if (ok) {                                           // epilogue: O_X complete
+        const uint32_t c = c0 - 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.odone[X][c & 1], (c >> 1) & 1, a.err));
+        tc_fence_after();
+      }
+      const bool store = ok && real;
+      __nv_bfloat16* op = a.out + ((size_t)(P.row0 + P.t0 + j) * a.q_heads + P.g * HY_GROUP + 2 * X + (r >> 6)) *
+                                      HY_HEAD_DIM;
+      if (P.w != 0) {                                     // a piece: every softmax thread takes part
+        ok = prefill_piece_finish(v, P.w, X * 128 + r, tO, m, l, ok, store ? op : nullptr, sh.pre_last);
+      } else if (ok) {
+        const float inv = 1.f / l;
+#pragma unroll 1
+        for (int cc = 0; cc < 4; ++cc) {
+          float o[32];
+          tmem_ld32(tO + 32 * cc, o);                     // warp-collective: every lane loads
+          tmem_wait_ld(o);
+          if (store) {
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+              *reinterpret_cast<uint4*>(op + 32 * cc + 8 * q4) =
+                  make_uint4(pack_bf16(o[8 * q4 + 0] * inv, o[8 * q4 + 1] * inv),
+                             pack_bf16(o[8 * q4 + 2] * inv, o[8 * q4 + 3] * inv),
+                             pack_bf16(o[8 * q4 + 4] * inv, o[8 * q4 + 5] * inv),
+                             pack_bf16(o[8 * q4 + 6] * inv, o[8 * q4 + 7] * inv));
+          }
         }
       }
-      const float mneg = (m == NEG_INF) ? 0.f : -m;
-      const float2 sl2v = make_float2(sl2, sl2), mnegv = make_float2(mneg, mneg);
-      uint32_t pk[32];
-      float2 ls[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
-                      make_float2(0.f, 0.f)};
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), sl2v, mnegv);
-        const float p0 = ex2_ftz(x.x), p1 = ex2_ftz(x.y);
-        ls[i & 3] = __fadd2_rn(ls[i & 3], make_float2(p0, p1));
-        pk[i] = q4_as_u32(__floats2half2_rn(p0, p1));
-      }
-      l += ((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y)) + ((ls[2].x + ls[2].y) + (ls[3].x + ls[3].y));
-      tmem_st32u(tS, pk);                                 // P(t) over the first 32 columns of S(t)
-      tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.pfull[X][c & 1]);
-    }
-    if (ok) {                                             // epilogue: O_X complete
-      const uint32_t c = c0 + ntiles - 1;
-      ok = __all_sync(0xffffffffu, mbar_wait(&sh.odone[X][c & 1], (c >> 1) & 1, a.err));
-      tc_fence_after();
-    }
-    const bool store = ok && real;
-    __nv_bfloat16* op = a.out + at;
-    if (P.w != 0) {                                       // a piece: every softmax thread takes part
-      ok = prefill_piece_finish(v, P.w, X * 128 + r, tO, m, l, ok, store ? op : nullptr,
-                                sh.pre_last);
-    } else if (ok) {
-      const float inv = 1.f / l;
-#pragma unroll 1
-      for (int cc = 0; cc < 4; ++cc) {
-        float o[32];
-        tmem_ld32(tO + 32 * cc, o);                       // warp-collective: every lane loads
-        tmem_wait_ld(o);
-        if (store) {
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4)
-            *reinterpret_cast<uint4*>(op + 32 * cc + 8 * q4) =
-                make_uint4(pack_bf16(o[8 * q4 + 0] * inv, o[8 * q4 + 1] * inv),
-                           pack_bf16(o[8 * q4 + 2] * inv, o[8 * q4 + 3] * inv),
-                           pack_bf16(o[8 * q4 + 4] * inv, o[8 * q4 + 5] * inv),
-                           pack_bf16(o[8 * q4 + 6] * inv, o[8 * q4 + 7] * inv));
-        }
-      }
+      if (lane == 0) mbar_arrive(&sh.ofree[X]);
     }
   }
   tc_fence_before();
-  if (__syncthreads_or(!ok)) ok = false;
-  return ok;
+  return !__syncthreads_or(!ok);
 }
 
 // The step's decode sequences.  Alone in the launch, their key blocks are dealt evenly
@@ -1023,7 +1084,8 @@ __device__ bool decode_all(const Args& a, const PlanView& v, int n_pre, int n_pa
   }
 }
 
-__global__ void __launch_bounds__(NT, 1) attn_q4_kernel(Args a, PlanView v) {
+__global__ void __launch_bounds__(NT, 1) attn_q4_kernel(const __grid_constant__ CUtensorMap q_map,
+                                                          Args a, PlanView v) {
   __shared__ Shared sh;
   extern __shared__ uint8_t dyn_smem[];
   uint8_t* payload = dyn_smem + ((1024u - (smem_u32(dyn_smem) & 1023u)) & 1023u);
@@ -1042,8 +1104,13 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(Args a, PlanView v) {
         mbar_init(&sh.odone[x][b], 1);
       }
       mbar_init(&sh.drain[x], 1);
+      mbar_init(&sh.ofree[x], EXP_WARP / 2);
     }
+    mbar_init(&sh.qraw, 1);
     mbar_init(&sh.qfull, EXP_WARP);
+    mbar_init(&sh.qfree, 2);
+    mbar_init(&sh.itemfull, 1);
+    mbar_init(&sh.itemfree, ITEM_READERS);
     fence_mbar_init();
   }
   __syncthreads();
@@ -1064,15 +1131,7 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(Args a, PlanView v) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem_base;
-    uint32_t tile_ctr = 0;
-    for (uint32_t n = 0; ok; ++n) {
-      if (threadIdx.x == 0) sh.pre_item = atomicAdd(&grab[2], 1);
-      __syncthreads();
-      const int k = sh.pre_item;
-      __syncthreads();
-      if (k >= n_pre) break;
-      ok = prefill_item(a, v, k, payload, sh, tmem, tile_ctr, n & 1);
-    }
+    ok = prefill_all(&q_map, a, v, n_pre, &grab[2], payload, sh, tmem);
     tc_fence_before();
     __syncthreads();
     if (warp == 0) {
@@ -1209,7 +1268,7 @@ cudaError_t hy_launch_attn_q4_fp32(const void* q, void* out, int tokens, int q_h
                               bt_pitch, seq_bt_row, cu_q, seq_lens_k, S, scale, err, st);
 }
 
-cudaError_t hy_launch_attn_q4_bf16(const void* q, void* out, int q_heads, int kv_heads,
+cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap& q_map, const void* q, void* out, int q_heads, int kv_heads,
                                    const void* cache_layer, int num_blocks, int layer,
                                    const int32_t* block_tables, int bt_pitch,
                                    const int32_t* seq_bt_row, const int32_t* cu_q,
@@ -1235,6 +1294,6 @@ cudaError_t hy_launch_attn_q4_bf16(const void* q, void* out, int q_heads, int kv
   a.seq_lens_k = seq_lens_k;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = err;
-  return hy_launch(attn_q4_kernel, dim3(hy_attn_num_sms(dev)), dim3(NT), SMEM_BYTES, st, a,
-                   hy_attn_plan_view(ws, dims));
+  return hy_launch(attn_q4_kernel, dim3(hy_attn_num_sms(dev)), dim3(NT), SMEM_BYTES, st, q_map,
+                   a, hy_attn_plan_view(ws, dims));
 }
