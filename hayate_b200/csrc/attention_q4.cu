@@ -111,6 +111,7 @@ struct Shared {
   uint64_t qfree;         // both sub-tiles' last S is done (one commit each)
   uint64_t itemfull;      // item[n % 2] is the CTA's item n
   uint64_t itemfree;      // every warp has read it (one arrival each)
+  uint64_t expdone;       // the item's last tile is about to be expanded (one arrival per expanding warp)
   PreItem item[2];
   uint32_t tmem_base;
   int pre_last;
@@ -801,6 +802,10 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
   if (warp == ITEM_WARP) {
     if (lane == 0) {
       for (uint32_t n = 0; ok; ++n) {
+        // an item is taken when the loads of the last one are over, not before: others
+        // may be free for it
+        if (n > 0) ok = mbar_wait(&sh.expdone, (n - 1) & 1, a.err);
+        if (!ok) break;
         const int k = atomicAdd(next, 1);
         PreItem N;
         if (k < n_pre) N = pre_item_geom(a, v, k);
@@ -838,6 +843,7 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
         if (t + 1 < ntiles) load_row(a, P, part, pos, blk, nxt);
         if (t + 2 < ntiles) blk = tile_block(a, P, bt, pos + PRE_KEYS);
         const uint32_t c = c0 + t, slot = c % PS;
+        if (t == ntiles - 1 && lane == 0) mbar_arrive(&sh.expdone);
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.free_[slot], ((c / PS) & 1) ^ 1, a.err));
         if (!ok) break;
         expand_row(cur, ring + slot * KV_BYTES, key);
@@ -1111,6 +1117,7 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(const __grid_constant__ 
     mbar_init(&sh.qfree, 2);
     mbar_init(&sh.itemfull, 1);
     mbar_init(&sh.itemfree, ITEM_READERS);
+    mbar_init(&sh.expdone, MMA_WARP - EXP_WARP);
     fence_mbar_init();
   }
   __syncthreads();
