@@ -14,7 +14,7 @@
 // Prefill items (64 query tokens x one KV head, 256 score rows) run on tcgen05: four
 // warps expand key tiles to fp16 operands in shared memory, one warp per 128-row
 // sub-tile issues the products, two warpgroups run the softmax.
-// fp32 runs a scalar kernel.
+// fp32 runs a kernel of its own on the fp32 units.
 #include "attention.cuh"
 #include "attention_pieces.cuh"
 #include "q4.cuh"
@@ -1158,54 +1158,33 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(const __grid_constant__ 
   }
 }
 
-// ------------------------------------------------------------------ scalar path
-// One warp per (query token, query head), every key visited in order with a
-// running maximum and sum: fp32 throughout, whatever T is.
-template <typename T> HY_DEVICE void load4(const T* p, float (&f)[4]);
-template <> HY_DEVICE void load4<float>(const float* p, float (&f)[4]) {
-  const float4 u = *reinterpret_cast<const float4*>(p);
-  f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
-}
-template <> HY_DEVICE void load4<__nv_bfloat16>(const __nv_bfloat16* p, float (&f)[4]) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  f[0] = __uint_as_float(u.x << 16); f[1] = __uint_as_float(u.x & 0xffff0000u);
-  f[2] = __uint_as_float(u.y << 16); f[3] = __uint_as_float(u.y & 0xffff0000u);
-}
-HY_DEVICE void store4(float* p, const float (&f)[4]) {
-  *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-}
-HY_DEVICE void store4(__nv_bfloat16* p, const float (&f)[4]) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
-}
+// ------------------------------------------------------------------ fp32 path
+// fp32 throughout, for the parity engine.  A CTA takes one (query token, KV head): its
+// four query heads share every key and value read.  The warps take 32 keys at a time in
+// turn: one key per lane for the scores (the whole 128-long product in a lane, no exchange
+// between lanes), four dimensions per lane for the values; each keeps a running maximum
+// and sum, merged at the end.
+constexpr int F_WARPS = 8, F_KEYS = 32;
+struct F32Shared {
+  float q[HY_GROUP][HY_HEAD_DIM];
+  float p[F_WARPS][F_KEYS][HY_GROUP];                     // weights of a warp's 32 keys
+  float o[F_WARPS][HY_GROUP][HY_HEAD_DIM];
+  float2 ml[F_WARPS][HY_GROUP];
+};
 
-// This lane's 4 dimensions (4 lane .. 4 lane + 3) of row `off` of a tile.
-HY_DEVICE void row4(const uint8_t* tile, int off, int lane, float (&f)[4]) {
-  const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + off * Q4_ROW_BYTES + 4 * (lane >> 1));
-  const uint32_t p = *reinterpret_cast<const uint32_t*>(tile + Q4_PARAM_OFF + off * Q4_PARAM_BYTES +
-                                                        4 * (lane >> 4));
-  const float2 sm = __half22float2(q4_as_half2(p));
-  const uint32_t n = w >> (8 * (lane & 1));      // nibbles j, j + 1 and, 16 bits up, their partners
-  f[0] = fmaf((float)(n & 15u), sm.x, sm.y);
-  f[1] = fmaf((float)((n >> 16) & 15u), sm.x, sm.y);
-  f[2] = fmaf((float)((n >> 4) & 15u), sm.x, sm.y);
-  f[3] = fmaf((float)((n >> 20) & 15u), sm.x, sm.y);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) attn_q4_scalar_kernel(
-    const T* __restrict__ q, T* __restrict__ out, int tokens, int q_heads, int kv_heads,
+__global__ void __launch_bounds__(F_WARPS * 32) attn_q4_fp32_kernel(
+    const float* __restrict__ q, float* __restrict__ out, int tokens, int q_heads, int kv_heads,
     const uint8_t* __restrict__ cache_layer, int num_blocks,
     const int32_t* __restrict__ block_tables, int bt_pitch,
     const int32_t* __restrict__ seq_bt_row, const int32_t* __restrict__ cu_q,
     const int32_t* __restrict__ seq_lens_k, int S, float scale, int32_t* err) {
+  __shared__ F32Shared sh;
   hy_grid_wait();
   hy_grid_trigger();
-  const int lane = threadIdx.x & 31;
-  const long total = (long)min(tokens, cu_q[S]) * q_heads;   // rows past the last sequence stay
-  const long nwarps = (long)gridDim.x * (blockDim.x >> 5);
-  for (long w = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w < total; w += nwarps) {
-    const int row = (int)(w / q_heads), hq = (int)(w % q_heads);
-    const int g = hq / HY_GROUP;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const long total = (long)min(tokens, cu_q[S]) * kv_heads;   // rows past the last sequence stay
+  for (long u = blockIdx.x; u < total; u += gridDim.x) {
+    const int row = (int)(u / kv_heads), g = (int)(u % kv_heads);
     int lo = 0, hi = S;                     // seq = last i with cu_q[i] <= row
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -1215,51 +1194,113 @@ __global__ void __launch_bounds__(256) attn_q4_scalar_kernel(
     const int prefix = seq_lens_k[seq] - (cu_q[seq + 1] - cu_q[seq]);
     const int key_end = prefix + (row - cu_q[seq]) + 1;
     if (prefix < 0 || (long)key_end > (long)bt_pitch * HY_BLOCK) {
-      hy_flag(err, HY_ERR_BOUNDS);
+      if (tid == 0) hy_flag(err, HY_ERR_BOUNDS);
       continue;
     }
     const int32_t* bt = block_tables + (size_t)(seq_bt_row ? seq_bt_row[seq] : seq) * bt_pitch;
-    float qv[4];
-    load4(q + ((size_t)row * q_heads + hq) * HY_HEAD_DIM + 4 * lane, qv);
-    float m = -INFINITY, l = 0.f;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int key = 0; key < key_end; ++key) {
-      const int blk = bt[key / HY_BLOCK];
-      if (blk < 0 || blk >= num_blocks) { hy_flag(err, HY_ERR_BOUNDS); break; }
-      const uint8_t* tile = cache_layer + q4_tile(blk, g, 0, kv_heads);
-      float kv[4];
-      row4(tile, key % HY_BLOCK, lane, kv);
-      float s = qv[0] * kv[0] + qv[1] * kv[1] + qv[2] * kv[2] + qv[3] * kv[3];
+    const size_t at = ((size_t)row * q_heads + g * HY_GROUP) * HY_HEAD_DIM;
+    __syncthreads();                        // the last unit's merge is over
+    if (tid < HY_GROUP * HY_HEAD_DIM / 4)
+      reinterpret_cast<float4*>(sh.q)[tid] = reinterpret_cast<const float4*>(q + at)[tid];
+    __syncthreads();
+    float m[HY_GROUP], l[HY_GROUP], acc[HY_GROUP][4];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      s *= scale;
-      const float m_new = fmaxf(m, s);
-      const float alpha = expf(m - m_new);
-      const float p = expf(s - m_new);
-      l = l * alpha + p;
-      row4(tile + Q4_TILE_BYTES, key % HY_BLOCK, lane, kv);
-#pragma unroll
-      for (int d = 0; d < 4; ++d) acc[d] = acc[d] * alpha + p * kv[d];
-      m = m_new;
+    for (int h = 0; h < HY_GROUP; ++h) {
+      m[h] = -INFINITY;
+      l[h] = acc[h][0] = acc[h][1] = acc[h][2] = acc[h][3] = 0.f;
     }
-    const float inv = 1.f / l;
+    for (int k0 = warp * F_KEYS; k0 < key_end; k0 += F_WARPS * F_KEYS) {
+      const int key = k0 + lane, cnt = min(F_KEYS, key_end - k0);
+      int blk = lane < cnt ? bt[key / HY_BLOCK] : 0;
+      if (blk < 0 || blk >= num_blocks) {
+        hy_flag(err, HY_ERR_BOUNDS);
+        blk = 0;
+      }
+      const uint8_t* tile = cache_layer + q4_tile(blk, g, 0, kv_heads);
+      float s[HY_GROUP] = {0.f, 0.f, 0.f, 0.f};
+      {
+        const uint4* codes = reinterpret_cast<const uint4*>(tile + (key % HY_BLOCK) * Q4_ROW_BYTES);
+        const uint2 par = *reinterpret_cast<const uint2*>(tile + Q4_PARAM_OFF + (key % HY_BLOCK) * Q4_PARAM_BYTES);
 #pragma unroll
-    for (int d = 0; d < 4; ++d) acc[d] *= inv;
-    store4(out + ((size_t)row * q_heads + hq) * HY_HEAD_DIM + 4 * lane, acc);
+        for (int i = 0; i < 4; ++i) {
+          const uint4 w4 = codes[i];
+          const float2 sm = __half22float2(q4_as_half2(i < 2 ? par.x : par.y));
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            float x[8];
+            q4_values(w == 0 ? w4.x : w == 1 ? w4.y : w == 2 ? w4.z : w4.w, sm.x, sm.y, x);
+#pragma unroll
+            for (int h = 0; h < HY_GROUP; ++h) {
+              const float4* qp = reinterpret_cast<const float4*>(&sh.q[h][32 * i + 8 * w]);
+              const float4 a = qp[0], b = qp[1];
+              s[h] = fmaf(a.x, x[0], fmaf(a.y, x[1], fmaf(a.z, x[2], fmaf(a.w, x[3], s[h]))));
+              s[h] = fmaf(b.x, x[4], fmaf(b.y, x[5], fmaf(b.z, x[6], fmaf(b.w, x[7], s[h]))));
+            }
+          }
+        }
+      }
+      float p[HY_GROUP];
+#pragma unroll
+      for (int h = 0; h < HY_GROUP; ++h) {
+        s[h] = lane < cnt ? s[h] * scale : -INFINITY;     // rows past the end hold anything
+        float mx = s[h];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float m_new = fmaxf(m[h], mx), mu = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = expf(m[h] - mu);
+        p[h] = expf(s[h] - mu);
+        m[h] = m_new;
+        l[h] = fmaf(l[h], alpha, p[h]);                   // this lane's part of the sum
+#pragma unroll
+        for (int d = 0; d < 4; ++d) acc[h][d] *= alpha;
+      }
+      *reinterpret_cast<float4*>(sh.p[warp][lane]) = make_float4(p[0], p[1], p[2], p[3]);
+      __syncwarp();
+      // this lane's 4 dimensions (4 lane ..) of each key's value: half a code word
+      const uint32_t v_off = Q4_TILE_BYTES + 4 * (lane >> 1), p_off = Q4_TILE_BYTES + Q4_PARAM_OFF + 4 * (lane >> 4);
+      const int sh8 = 8 * (lane & 1);
+#pragma unroll 8
+      for (int j = 0; j < cnt; ++j) {
+        const int b = __shfl_sync(0xffffffffu, blk, j), off = (k0 + j) % HY_BLOCK;
+        const uint8_t* vt = cache_layer + q4_tile(b, g, 0, kv_heads);
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(vt + v_off + off * Q4_ROW_BYTES) >> sh8;
+        const float2 sm = __half22float2(
+            *reinterpret_cast<const __half2*>(vt + p_off + off * Q4_PARAM_BYTES));
+        // nibbles j, j + 1 and, 16 bits up, their partners
+        const float x[4] = {fmaf(q4_nibble(w, 0), sm.x, sm.y), fmaf(q4_nibble(w, 16), sm.x, sm.y),
+                            fmaf(q4_nibble(w, 4), sm.x, sm.y), fmaf(q4_nibble(w, 20), sm.x, sm.y)};
+        const float4 pj = *reinterpret_cast<const float4*>(sh.p[warp][j]);
+        const float ph[HY_GROUP] = {pj.x, pj.y, pj.z, pj.w};
+#pragma unroll
+        for (int h = 0; h < HY_GROUP; ++h)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) acc[h][d] = fmaf(ph[h], x[d], acc[h][d]);
+      }
+      __syncwarp();
+    }
+#pragma unroll
+    for (int h = 0; h < HY_GROUP; ++h) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
+      if (lane == 0) sh.ml[warp][h] = make_float2(m[h], l[h]);
+      *reinterpret_cast<float4*>(&sh.o[warp][h][4 * lane]) = make_float4(acc[h][0], acc[h][1], acc[h][2], acc[h][3]);
+    }
+    __syncthreads();
+    for (int i = tid; i < HY_GROUP * HY_HEAD_DIM; i += F_WARPS * 32) {
+      const int h = i / HY_HEAD_DIM, d = i % HY_HEAD_DIM;
+      float M = -INFINITY, L = 0.f, o = 0.f;
+#pragma unroll
+      for (int w = 0; w < F_WARPS; ++w) M = fmaxf(M, sh.ml[w][h].x);
+      const float mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int w = 0; w < F_WARPS; ++w) {
+        const float wt = expf(sh.ml[w][h].x - mu);
+        L = fmaf(wt, sh.ml[w][h].y, L);
+        o = fmaf(wt, sh.o[w][h][d], o);
+      }
+      out[at + i] = o / L;
+    }
   }
-}
-
-template <typename T>
-cudaError_t launch_scalar(const void* q, void* out, int tokens, int q_heads, int kv_heads,
-                          const uint8_t* cache_layer, int num_blocks,
-                          const int32_t* block_tables, int bt_pitch, const int32_t* seq_bt_row,
-                          const int32_t* cu_q, const int32_t* seq_lens_k, int S, float scale,
-                          int32_t* err, cudaStream_t st) {
-  const long blocks = ((long)tokens * q_heads + 7) / 8;
-  return hy_launch(attn_q4_scalar_kernel<T>, dim3((int)(blocks < 148L * 32 ? blocks : 148L * 32)),
-                   dim3(256), 0, st, static_cast<const T*>(q), static_cast<T*>(out), tokens,
-                   q_heads, kv_heads, cache_layer, num_blocks, block_tables, bt_pitch, seq_bt_row,
-                   cu_q, seq_lens_k, S, scale, err);
 }
 
 }  // namespace
@@ -1270,9 +1311,11 @@ cudaError_t hy_launch_attn_q4_fp32(const void* q, void* out, int tokens, int q_h
                                    const int32_t* seq_bt_row, const int32_t* cu_q,
                                    const int32_t* seq_lens_k, int S, float scale, int32_t* err,
                                    cudaStream_t st) {
-  return launch_scalar<float>(q, out, tokens, q_heads, kv_heads,
-                              static_cast<const uint8_t*>(cache_layer), num_blocks, block_tables,
-                              bt_pitch, seq_bt_row, cu_q, seq_lens_k, S, scale, err, st);
+  const long units = (long)tokens * kv_heads;
+  return hy_launch(attn_q4_fp32_kernel, dim3((int)(units < 148L * 32 ? units : 148L * 32)),
+                   dim3(F_WARPS * 32), 0, st, static_cast<const float*>(q), static_cast<float*>(out),
+                   tokens, q_heads, kv_heads, static_cast<const uint8_t*>(cache_layer), num_blocks,
+                   block_tables, bt_pitch, seq_bt_row, cu_q, seq_lens_k, S, scale, err);
 }
 
 cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap& q_map, const void* q, void* out, int q_heads, int kv_heads,
