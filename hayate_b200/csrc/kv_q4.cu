@@ -1,97 +1,170 @@
 // Writing the 4-bit KV cache and reading it back.
 //
-// Both are one pass over rows of 128 (token, K or V, head): 16 lanes per row, one
-// 32-bit code word (8 dimensions) per lane, the 8 lanes of a half row agreeing on
-// its scale and minimum by three shuffles.  They do what hy_kv_append and a gather
-// of its cache do (hayate/model/attention.py:52-54 keeps the cache in the model
-// dtype; the reference has no quantised one).
+// Both are one pass over rows of 128 (token, K or V, head): 8 lanes per row, 16
+// dimensions (two code words) per lane, the 4 lanes of a half row agreeing on its
+// minimum and maximum by two exchanges.  They do what hy_kv_append and a gather of its
+// cache do (hayate/model/attention.py:52-54 keeps the cache in the model dtype; the
+// reference has no quantised one).
 //
-// Bound by memory: a bf16 row moves 256 + 72 bytes.
+// Bound by memory (a bf16 row moves 256 + 72 bytes) as long as the instructions per
+// element stay few: the codes are rounded and collected by additions instead of
+// conversions (which run at a quarter of the rate), read back by masks, and a thread's
+// row of the token is found once, not per row.
 #include "q4.cuh"
 
 namespace {
 
 constexpr int Q4_THREADS = 256;
-constexpr int Q4_LANES = HY_HEAD_DIM / 8;             // lanes per row
+constexpr int Q4_LANES = HY_HEAD_DIM / 16;            // lanes per row
 constexpr int Q4_ROWS = Q4_THREADS / Q4_LANES;        // rows per CTA pass
 #ifndef HY_Q4_UNROLL
-#define HY_Q4_UNROLL 4
+#define HY_Q4_UNROLL 2
 #endif
 constexpr int Q4_UNROLL = HY_Q4_UNROLL;               // rows in flight per lane
 
-// 8 consecutive elements as loaded, and their values.
-template <typename T> struct Raw8;
-template <> struct Raw8<__nv_bfloat16> {
-  uint4 a;
-  HY_DEVICE void load(const __nv_bfloat16* p) { a = __ldg(reinterpret_cast<const uint4*>(p)); }
-  HY_DEVICE void get(float (&f)[8]) const {
-    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+// min and max that are NaN if either operand is
+HY_DEVICE float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+HY_DEVICE float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 16 consecutive elements as loaded; their values; and over the half row (lanes xor 1,
+// 2) the minimum and maximum, NaN if any element is.
+template <typename T> struct Raw16;
+template <> struct Raw16<__nv_bfloat16> {
+  uint4 a[2];
+  HY_DEVICE void load(const __nv_bfloat16* p) {
+    a[0] = __ldg(reinterpret_cast<const uint4*>(p));
+    a[1] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+  }
+  HY_DEVICE void get(float (&f)[16]) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t u[4] = {a[h].x, a[h].y, a[h].z, a[h].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[8 * h + 2 * i] = __uint_as_float(u[i] << 16);
+        f[8 * h + 2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      }
+    }
+  }
+  HY_DEVICE void range(const float (&)[16], float& lo, float& hi) const {
+    const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(a);
+    __nv_bfloat162 mn = v[0], mx = v[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      mn = __hmin2_nan(mn, v[i]);
+      mx = __hmax2_nan(mx, v[i]);
+    }
+    // (min, -max) of both halves of the registers, exchanged together
+    const __nv_bfloat162 neg = __hneg2(mx);
+    __nv_bfloat162 e = __hmin2_nan(__halves2bfloat162(__low2bfloat16(mn), __low2bfloat16(neg)),
+                                   __halves2bfloat162(__high2bfloat16(mn), __high2bfloat16(neg)));
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) e = __hmin2_nan(e, __shfl_xor_sync(0xffffffffu, e, o));
+    lo = __low2float(e);
+    hi = -__high2float(e);
+  }
+};
+template <> struct Raw16<float> {
+  float4 a[4];
+  HY_DEVICE void load(const float* p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = __ldg(reinterpret_cast<const float4*>(p) + i);
+  }
+  HY_DEVICE void get(float (&f)[16]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(u[i] << 16);
-      f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      f[4 * i] = a[i].x;
+      f[4 * i + 1] = a[i].y;
+      f[4 * i + 2] = a[i].z;
+      f[4 * i + 3] = a[i].w;
+    }
+  }
+  HY_DEVICE void range(const float (&x)[16], float& lo, float& hi) const {
+    lo = hi = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) {
+      lo = min_nan(lo, x[i]);
+      hi = max_nan(hi, x[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
   }
 };
-template <> struct Raw8<float> {
-  float4 a, b;
-  HY_DEVICE void load(const float* p) {
-    a = __ldg(reinterpret_cast<const float4*>(p));
-    b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  }
-  HY_DEVICE void get(float (&f)[8]) const {
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  }
-};
 
-HY_DEVICE void store8(__nv_bfloat16* p, const float (&f)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]),
-                                            pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+HY_DEVICE void store16(__nv_bfloat16* p, const float (&f)[16]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    reinterpret_cast<uint4*>(p)[h] =
+        make_uint4(pack_bf16(f[8 * h], f[8 * h + 1]), pack_bf16(f[8 * h + 2], f[8 * h + 3]),
+                   pack_bf16(f[8 * h + 4], f[8 * h + 5]), pack_bf16(f[8 * h + 6], f[8 * h + 7]));
 }
-HY_DEVICE void store8(float* p, const float (&f)[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+HY_DEVICE void store16(float* p, const float (&f)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    reinterpret_cast<float4*>(p)[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
 }
 
-// Code word of this lane's 8 values and its half row's (scale, minimum); the 8
-// lanes of a half row call it together (xor 1, 2, 4 stay inside it).  Every step is
-// an IEEE fp32 operation, so the codes are the same whatever computes them.
-HY_DEVICE uint32_t quantise8(float (&x)[8], __half2& par) {
-  bool nan = false;
-  float lo = INFINITY, hi = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    nan |= x[i] != x[i];
-    x[i] = fminf(fmaxf(x[i], -Q4_LIMIT), Q4_LIMIT);
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-  }
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  // a NaN anywhere in the half row: it reads back as NaN
-  const unsigned votes = __ballot_sync(0xffffffffu, nan);
-  if ((votes >> (threadIdx.x & 24)) & 0xffu) {
+// Code words of this lane's 16 values and its half row's (scale, minimum).  Every step
+// is an IEEE fp32 operation, so the codes are the same whatever computes them.  The
+// clamp of the values to +-Q4_LIMIT is the clamp of their range: beyond it a code is 0
+// or 15 either way.
+template <typename T>
+HY_DEVICE uint2 quantise16(const Raw16<T>& raw, __half2& par) {
+  float x[16], lo, hi;
+  raw.get(x);
+  raw.range(x, lo, hi);
+  if (lo != lo) {                                       // a NaN somewhere: it reads back as NaN
     par = __half2half2(__ushort_as_half(0x7fff));
-    return 0u;
+    return make_uint2(0u, 0u);
   }
+  lo = fminf(fmaxf(lo, -Q4_LIMIT), Q4_LIMIT);
+  hi = fminf(fmaxf(hi, -Q4_LIMIT), Q4_LIMIT);
   const __half scale = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
   const __half low = __float2half_rn(lo);
   par = __halves2half2(scale, low);
   const float s = __half2float(scale), m = __half2float(low);
-  const float inv = s > 0.f ? __fdiv_rn(1.0f, s) : 0.f;   // a constant half row: codes 0
-  uint32_t w = 0;
+  const float inv = s > 0.f ? __fdiv_rn(1.0f, s) : 0.f; // a constant half row: codes 0
+  uint32_t w[2] = {0u, 0u};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = rintf(__fmul_rn(__fsub_rn(x[i], m), inv));
-    const uint32_t code = (uint32_t)fminf(fmaxf(c, 0.f), 15.f);
-    w |= code << (4 * (i >> 1) + 16 * (i & 1));
+  for (int h = 0; h < 2; ++h) {
+    // c + 2^23 rounds c to an integer, half to even, in the low bits; the words collect
+    // 16 u + u' from nibble 7 down, and the exponents' multiples are taken off at the end
+#pragma unroll
+    for (int n = 7; n >= 0; --n) {
+      const int i = 8 * h + (n < 4 ? 2 * n : 2 * (n - 4) + 1);
+      const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(x[i], m), inv), 0.f), 15.f);
+      w[h] = w[h] * 16u + __float_as_uint(__fadd_rn(c, 8388608.0f));
+    }
+    w[h] -= 0x4b000000u;       // times 1 + 16 + .. + 16^7, of which all but 1 and 16 leave 32 bits
+    w[h] -= 0xb0000000u;       // 16 x 0x4b000000
   }
-  return w;
+  return make_uint2(w[0], w[1]);
 }
+
+// Rows of a CTA pass: 8 lanes each, `per` rows of a token (all its 2 kv_heads rows, or
+// 32 at a time), as many tokens as fit.
+struct RowMap {
+  int per, tokens, t, r;                                // this thread's token of the pass and row
+  HY_DEVICE RowMap(int kv_heads) {
+    const int row = threadIdx.x / Q4_LANES;
+    per = min(2 * kv_heads, Q4_ROWS);
+    tokens = Q4_ROWS / per;
+    t = row / per;
+    r = row - t * per;
+    if (t >= tokens) r = 1 << 30;                       // a spare row of the pass
+  }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(Q4_THREADS) kv_append_q4_kernel(
@@ -100,46 +173,56 @@ __global__ void __launch_bounds__(Q4_THREADS) kv_append_q4_kernel(
     int32_t* err) {
   hy_grid_wait();
   hy_grid_trigger();
-  const int grp = threadIdx.x / Q4_LANES, l = threadIdx.x % Q4_LANES;
-  const int R = 2 * kv_heads;
-  const int total = tokens * R, stride = (int)gridDim.x * Q4_ROWS;
-  // every lane of a warp makes the same trips: the shuffles below need them all
-  const int first = (int)blockIdx.x * Q4_ROWS;
-  for (int base = first; base < total; base += stride * Q4_UNROLL) {
-    Raw8<T> raw[Q4_UNROLL];
-    uint8_t* dst[Q4_UNROLL];                        // the row's codes
-    int par_at[Q4_UNROLL];                          // its parameters, from there
+  const int l = threadIdx.x % Q4_LANES, R = 2 * kv_heads;
+  const RowMap map(kv_heads);
+  const int stride = (int)gridDim.x * map.tokens;
+  // every lane of a warp makes the same trips: the exchanges need them all
+  for (int rb = 0; rb < R; rb += map.per)
+    for (int tb = (int)blockIdx.x * map.tokens; tb < tokens; tb += stride * Q4_UNROLL) {
+      const int r = rb + map.r, kv = r >= kv_heads, h = kv ? r - kv_heads : r;
+      Raw16<T> raw[Q4_UNROLL];
+      int slot[Q4_UNROLL];
 #pragma unroll
-    for (int u = 0; u < Q4_UNROLL; ++u) {
-      const int i = base + u * stride + grp;
-      dst[u] = nullptr;
-      if (i < total) {
-        const int t = i / R, r = i - t * R;
-        const int kv = r >= kv_heads, h = kv ? r - kv_heads : r;
-        raw[u].load((kv ? v + (size_t)t * ldv : k + (size_t)t * ldk) + h * HY_HEAD_DIM + 8 * l);
-        const int slot = slots[t];
-        const int blk = slot / HY_BLOCK, off = slot % HY_BLOCK;
-        if (slot >= 0 && blk >= num_blocks) hy_flag(err, HY_ERR_BOUNDS);
-        else if (slot >= 0) {
-          dst[u] = cache + q4_tile(blk, h, kv, kv_heads) + off * Q4_ROW_BYTES;
-          par_at[u] = Q4_PARAM_OFF - off * (Q4_ROW_BYTES - Q4_PARAM_BYTES);
+      for (int u = 0; u < Q4_UNROLL; ++u) {
+        const int t = tb + u * stride + map.t;
+        slot[u] = -1;
+        if (r < R && t < tokens) {
+          raw[u].load((kv ? v + (size_t)t * ldv : k + (size_t)t * ldk) + h * HY_HEAD_DIM + 16 * l);
+          slot[u] = slots[t];
+        } else {
+          raw[u] = {};
         }
       }
-    }
 #pragma unroll
-    for (int u = 0; u < Q4_UNROLL; ++u) {
-      if (__any_sync(0xffffffffu, dst[u] != nullptr)) {
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (dst[u]) raw[u].get(x);
+      for (int u = 0; u < Q4_UNROLL; ++u) {
         __half2 par;
-        const uint32_t w = quantise8(x, par);
-        if (dst[u]) {
-          reinterpret_cast<uint32_t*>(dst[u])[l] = w;
-          if ((l & 7) == 0)
-            *reinterpret_cast<uint32_t*>(dst[u] + par_at[u] + 4 * (l >> 3)) = q4_as_u32(par);
+        const uint2 w = quantise16(raw[u], par);
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, q4_as_u32(par), Q4_LANES / 2);
+        if (slot[u] < 0) continue;
+        const int blk = slot[u] / HY_BLOCK, off = slot[u] % HY_BLOCK;
+        if (blk >= num_blocks) {
+          hy_flag(err, HY_ERR_BOUNDS);
+          continue;
         }
+        uint8_t* tile = cache + q4_tile(blk, h, kv, kv_heads);
+        reinterpret_cast<uint2*>(tile + off * Q4_ROW_BYTES)[l] = w;
+        if (l == 0)
+          *reinterpret_cast<uint2*>(tile + Q4_PARAM_OFF + off * Q4_PARAM_BYTES) =
+              make_uint2(q4_as_u32(par), other);
       }
     }
+}
+
+// The 8 values of word i (dimensions 8i.., in order) with the scale times 2^0, 2^-4, ..
+// 2^-16: nibbles 0-4 are taken where they stand, at 16^j times their code, nibbles 5-7
+// after one shift.  The products are exact, so the sum is the only rounding.
+HY_DEVICE void read_word(uint32_t w, const float (&s)[5], float low, float* x) {
+  const uint32_t w12 = w >> 12;
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    const int at = n < 5 ? n : n - 3;                   // nibble position in w or w12
+    const float c = __uint_as_float(((n < 5 ? w : w12) & (15u << (4 * at))) | 0x4b000000u) - 8388608.0f;
+    x[n < 4 ? 2 * n : 2 * (n - 4) + 1] = fmaf(c, s[at], low);
   }
 }
 
@@ -150,52 +233,58 @@ __global__ void __launch_bounds__(Q4_THREADS) kv_read_q4_kernel(
     int32_t* err) {
   hy_grid_wait();
   hy_grid_trigger();
-  const int grp = threadIdx.x / Q4_LANES, l = threadIdx.x % Q4_LANES;
-  const int R = 2 * kv_heads;
-  const int total = tokens * R, stride = (int)gridDim.x * Q4_ROWS;
-  for (int base = (int)blockIdx.x * Q4_ROWS + grp; base < total; base += stride * Q4_UNROLL) {
-    uint32_t w[Q4_UNROLL], par[Q4_UNROLL];
-    T* dst[Q4_UNROLL];
+  const int l = threadIdx.x % Q4_LANES, R = 2 * kv_heads;
+  const RowMap map(kv_heads);
+  const int stride = (int)gridDim.x * map.tokens;
+  for (int rb = 0; rb < R; rb += map.per) {
+    const int r = rb + map.r, kv = r >= kv_heads, h = kv ? r - kv_heads : r;
+    if (r >= R) continue;
+    T* out = (kv ? v_out : k_out) + h * HY_HEAD_DIM + 16 * l;
+    for (int tb = (int)blockIdx.x * map.tokens + map.t; tb < tokens; tb += stride * Q4_UNROLL) {
+      uint2 w[Q4_UNROLL];
+      uint32_t par[Q4_UNROLL];
 #pragma unroll
-    for (int u = 0; u < Q4_UNROLL; ++u) {
-      const int i = base + u * stride;
-      dst[u] = nullptr;
-      w[u] = par[u] = 0u;                           // scale = minimum = 0: a row of zeros
-      if (i < total) {
-        const int t = i / R, r = i - t * R;
-        const int kv = r >= kv_heads, h = kv ? r - kv_heads : r;
-        dst[u] = (kv ? v_out : k_out) + ((size_t)t * kv_heads + h) * HY_HEAD_DIM + 8 * l;
-        const int slot = slots[t];
+      for (int u = 0; u < Q4_UNROLL; ++u) {
+        const int t = tb + u * stride;
+        w[u] = make_uint2(0u, 0u);
+        par[u] = 0u;                                    // scale = minimum = 0: a row of zeros
+        const int slot = t < tokens ? slots[t] : -1;
         const int blk = slot / HY_BLOCK, off = slot % HY_BLOCK;
         if (slot >= 0 && blk >= num_blocks) hy_flag(err, HY_ERR_BOUNDS);
         else if (slot >= 0) {
           const uint8_t* tile = cache + q4_tile(blk, h, kv, kv_heads);
-          w[u] = __ldg(reinterpret_cast<const uint32_t*>(tile + off * Q4_ROW_BYTES) + l);
+          w[u] = __ldg(reinterpret_cast<const uint2*>(tile + off * Q4_ROW_BYTES) + l);
           par[u] = __ldg(reinterpret_cast<const uint32_t*>(tile + Q4_PARAM_OFF + off * Q4_PARAM_BYTES) +
-                         (l >> 3));
+                         l / (Q4_LANES / 2));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < Q4_UNROLL; ++u) {
+        const int t = tb + u * stride;
+        if (t < tokens) {
+          const float2 p = __half22float2(q4_as_half2(par[u]));
+          const float s[5] = {p.x, p.x * 0x1p-4f, p.x * 0x1p-8f, p.x * 0x1p-12f, p.x * 0x1p-16f};
+          float x[16];
+          read_word(w[u].x, s, p.y, x);
+          read_word(w[u].y, s, p.y, x + 8);
+          store16(out + (size_t)t * kv_heads * HY_HEAD_DIM, x);
         }
       }
     }
-#pragma unroll
-    for (int u = 0; u < Q4_UNROLL; ++u)
-      if (dst[u]) {
-        const float2 p = __half22float2(q4_as_half2(par[u]));
-        float x[8];
-        q4_values(w[u], p.x, p.y, x);
-        store8(dst[u], x);
-      }
   }
 }
 
-// CTAs for `rows` rows: one pass of Q4_ROWS x Q4_UNROLL rows each, at most 8
-// resident CTAs on each of 148 SMs (the kernels stride over the rest).
-int q4_grid(long rows) {
-  const long n = (rows + Q4_ROWS - 1) / Q4_ROWS;
+// CTAs for `tokens` tokens: one pass each, at most 8 resident CTAs on each of 148 SMs
+// (the kernels stride over the rest).
+int q4_grid(int tokens, int kv_heads) {
+  const int per = 2 * kv_heads < Q4_ROWS ? 2 * kv_heads : Q4_ROWS, pass = Q4_ROWS / per;
+  const long n = ((long)tokens + pass - 1) / pass;
   return (int)(n < 148 * 8 ? n : 148 * 8);
 }
 
-// The kernels count rows in 32 bits: longer calls go in slices of this many rows.
-constexpr long Q4_SLICE_ROWS = 1L << 29;
+// The kernels count tokens in 32 bits, strides past the end included: longer calls go in
+// slices of this many.
+constexpr int Q4_SLICE = 1 << 28;
 
 }  // namespace
 
@@ -203,14 +292,13 @@ template <typename T>
 static cudaError_t append_q4(const T* k, long ldk, const T* v, long ldv, int T_tokens, int kv_heads,
                              const int32_t* slots, uint8_t* cache, int num_blocks, int32_t* err,
                              cudaStream_t st) {
-  const int step = (int)(Q4_SLICE_ROWS / (2 * kv_heads));
-  for (int t = 0; t < T_tokens; t += step) {
-    const int n = T_tokens - t < step ? T_tokens - t : step;
-    const cudaError_t e = hy_launch(kv_append_q4_kernel<T>, dim3(q4_grid(2L * kv_heads * n)),
+  for (long t = 0; t < T_tokens; t += Q4_SLICE) {
+    const int n = T_tokens - t < Q4_SLICE ? (int)(T_tokens - t) : Q4_SLICE;
+    const cudaError_t e = hy_launch(kv_append_q4_kernel<T>, dim3(q4_grid(n, kv_heads)),
                                     dim3(Q4_THREADS), 0, st, k + (size_t)t * ldk, ldk,
                                     v + (size_t)t * ldv, ldv, n, kv_heads, slots + t, cache,
                                     num_blocks, err);
-    if (e != cudaSuccess || n < step) return e;
+    if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
 }
@@ -230,14 +318,13 @@ template <typename T>
 static cudaError_t read_q4(const uint8_t* cache, int num_blocks, int kv_heads,
                            const int32_t* slots, int T_tokens, T* k_out, T* v_out, int32_t* err,
                            cudaStream_t st) {
-  const int step = (int)(Q4_SLICE_ROWS / (2 * kv_heads));
-  for (int t = 0; t < T_tokens; t += step) {
-    const int n = T_tokens - t < step ? T_tokens - t : step;
+  for (long t = 0; t < T_tokens; t += Q4_SLICE) {
+    const int n = T_tokens - t < Q4_SLICE ? (int)(T_tokens - t) : Q4_SLICE;
     const size_t at = (size_t)t * kv_heads * HY_HEAD_DIM;
-    const cudaError_t e = hy_launch(kv_read_q4_kernel<T>, dim3(q4_grid(2L * kv_heads * n)),
+    const cudaError_t e = hy_launch(kv_read_q4_kernel<T>, dim3(q4_grid(n, kv_heads)),
                                     dim3(Q4_THREADS), 0, st, cache, num_blocks, kv_heads,
                                     slots + t, n, k_out + at, v_out + at, err);
-    if (e != cudaSuccess || n < step) return e;
+    if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
 }
