@@ -19,6 +19,7 @@
 #include "attention_pieces.cuh"
 #include "q4.cuh"
 
+#include <atomic>
 #include <math.h>
 
 namespace {
@@ -1325,9 +1326,13 @@ cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap& q_map, const void* q, void
                                    const int32_t* seq_lens_k, int S, float scale,
                                    const PlanDims& dims, void* ws, int32_t* err, int dev,
                                    cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(attn_q4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       SMEM_BYTES);
-  if (e != cudaSuccess) return e;
+  static std::atomic<bool> attr_set[64];                  // per device, set on its first call
+  if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(attn_q4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               SMEM_BYTES);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
+  }
   Args a;
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.out = static_cast<__nv_bfloat16*>(out);

@@ -28,17 +28,13 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    # the current stream's handle, without building a Stream object around it
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
-def _on(device: torch.device):
+def _on(device: int):
     """Make ``device`` current for a launch (a no-op context when it already is)."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def _pitch(t: torch.Tensor) -> int:
-    """Elements from token to token (a single token's stride says nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return _HERE if device == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _i32(t: torch.Tensor, name: str):
@@ -167,18 +163,18 @@ def kv_cache_q4(layers: int, num_blocks: int, kv_heads: int, device="cuda") -> t
 
 
 def _q4_layer(cache: torch.Tensor, ndim: int):
-    if cache.dtype != torch.uint8 or cache.dim() != ndim or not cache.is_contiguous() or \
-            tuple(cache.shape[-2:]) != (2, Q4_TILE_BYTES):
+    """The shape of a 4-bit cache (or one layer of it), checked."""
+    shape = cache.shape
+    if cache.dtype != torch.uint8 or len(shape) != ndim or not cache.is_contiguous() or \
+            shape[-2] != 2 or shape[-1] != Q4_TILE_BYTES:
         raise ValueError("the 4-bit cache must be contiguous uint8 "
                          f"{'[layers]' * (ndim - 4)}[blocks][kv_heads][2][{Q4_TILE_BYTES}]")
+    return shape
 
 
-def _q4_index(t: torch.Tensor, name: str, n: int, device):
-    _i32(t, name)
-    if t.numel() != n:
-        raise ValueError(f"{name} needs one entry per token")
-    if t.device != device:
-        raise ValueError(f"{name} must be on the cache's device")
+def _q4_index(t: torch.Tensor, name: str, device: int):
+    if t.dtype != torch.int32 or device < 0 or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 CUDA tensor on the cache's device")
 
 
 def kv_append_q4(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
@@ -187,21 +183,25 @@ def kv_append_q4(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
     (``kv_cache_q4``) at ``slot_mapping``; a negative slot skips its token, and
     the other slots of a call are distinct.  The heads of a token are contiguous;
     the tokens may be strided (v as a part of the QKV rows)."""
-    _q4_layer(kv_cache_layer, 4)
-    NB, heads = kv_cache_layer.shape[:2]
-    T = k.shape[0]
-    for name, t in (("k", k), ("v", v)):
-        if tuple(t.shape) != (T, heads, 128) or t.dtype != k.dtype or \
-                t.device != kv_cache_layer.device:
-            raise ValueError(f"{name} must be (tokens, {heads}, 128) on the cache's device, "
-                             "k and v of one dtype")
-        if T and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != 128)):
-            raise ValueError(f"the heads of a token must be contiguous in {name}")
-    _q4_index(slot_mapping, "slot_mapping", T, k.device)
-    with _on(k.device):
+    NB, heads, _, _ = _q4_layer(kv_cache_layer, 4)
+    dev, want, T = kv_cache_layer.get_device(), k.shape, k.shape[0]
+    if want != (T, heads, 128) or v.shape != want or v.dtype != k.dtype or \
+            k.get_device() != dev or v.get_device() != dev:
+        raise ValueError(f"k and v must be (tokens, {heads}, 128) of one dtype on the cache's device")
+    ks, vs = k.stride(), v.stride()
+    if T and (ks[2] != 1 or vs[2] != 1 or (heads > 1 and (ks[1] != 128 or vs[1] != 128))):
+        raise ValueError("the heads of a token must be contiguous in k and v")
+    _q4_index(slot_mapping, "slot_mapping", dev)
+    if slot_mapping.numel() != T:
+        raise ValueError("slot_mapping needs one entry per token")
+    if err is not None:
+        _q4_index(err, "err", dev)
+    row = heads * 128                       # a single token's stride says nothing
+    with _on(dev):
         check(_lib.load().hy_kv_append_q4(
-            _dt(k), _ptr(k), _pitch(k), _ptr(v), _pitch(v), T, heads, _ptr(slot_mapping),
-            _ptr(kv_cache_layer), NB, _ptr(err), _stream()), "hy_kv_append_q4")
+            _dt(k), k.data_ptr(), ks[0] if T > 1 else row, v.data_ptr(), vs[0] if T > 1 else row, T,
+            heads, slot_mapping.data_ptr(), kv_cache_layer.data_ptr(), NB, _ptr(err), _stream()),
+            "hy_kv_append_q4")
 
 
 def kv_read_q4(kv_cache_layer: torch.Tensor, slot_mapping: torch.Tensor, dtype: torch.dtype,
@@ -210,24 +210,25 @@ def kv_read_q4(kv_cache_layer: torch.Tensor, slot_mapping: torch.Tensor, dtype: 
     """(k, v), each (tokens, kv_heads, 128) of ``dtype``: what the rows at
     ``slot_mapping`` of one layer of a 4-bit cache stand for (zeros for a negative
     slot)."""
-    _q4_layer(kv_cache_layer, 4)
-    NB, heads = kv_cache_layer.shape[:2]
-    T, device = slot_mapping.numel(), kv_cache_layer.device
-    _q4_index(slot_mapping, "slot_mapping", T, device)
-    outs = []
+    NB, heads, _, _ = _q4_layer(kv_cache_layer, 4)
+    dev, T = kv_cache_layer.get_device(), slot_mapping.numel()
+    _q4_index(slot_mapping, "slot_mapping", dev)
+    if err is not None:
+        _q4_index(err, "err", dev)
+    want = (T, heads, 128)
+    device = kv_cache_layer.device
+    if k_out is None:
+        k_out = torch.empty(want, dtype=dtype, device=device)
+    if v_out is None:
+        v_out = torch.empty(want, dtype=dtype, device=device)
     for t in (k_out, v_out):
-        if t is None:
-            t = torch.empty(T, heads, 128, dtype=dtype, device=device)
-        elif tuple(t.shape) != (T, heads, 128) or t.dtype != dtype or t.device != device or \
-                not t.is_contiguous():
+        if t.shape != want or t.dtype != dtype or t.get_device() != dev or not t.is_contiguous():
             raise ValueError(f"outputs must be contiguous (tokens, {heads}, 128) {dtype} tensors "
                              "on the cache's device")
-        outs.append(t)
-    k_out, v_out = outs
-    with _on(device):
+    with _on(dev):
         check(_lib.load().hy_kv_read_q4(
-            _dt(k_out), _ptr(kv_cache_layer), NB, heads, _ptr(slot_mapping), T, _ptr(k_out),
-            _ptr(v_out), _ptr(err), _stream()), "hy_kv_read_q4")
+            _dt(k_out), kv_cache_layer.data_ptr(), NB, heads, slot_mapping.data_ptr(), T,
+            k_out.data_ptr(), v_out.data_ptr(), _ptr(err), _stream()), "hy_kv_read_q4")
     return k_out, v_out
 
 
@@ -276,32 +277,39 @@ def varlen_attention_q4(q: torch.Tensor, out: torch.Tensor, kv_cache: torch.Tens
                         err: Optional[torch.Tensor] = None) -> None:
     """``varlen_attention`` over a 4-bit cache (``kv_cache_q4``): the same plan,
     workspace and block tables."""
+    L, NB, kv_heads, _, _ = _q4_layer(kv_cache, 5)
     T, q_heads, D = q.shape
-    _q4_layer(kv_cache, 5)
-    L, NB, kv_heads = kv_cache.shape[:3]
+    dev = kv_cache.get_device()
     if D != 128 or out.shape != q.shape or out.dtype != q.dtype or not q.is_contiguous() or \
-            not out.is_contiguous():
-        raise ValueError("q and out must be contiguous (tokens, q_heads, 128) of one dtype")
-    for name, t, n in (("block_tables", block_tables, 0), ("cu_seqlens_q", cu_seqlens_q, num_seqs + 1),
-                       ("seq_lens_k", seq_lens_k, num_seqs), ("seq_bt_row", seq_bt_row, num_seqs)):
-        if t is None:
-            continue
-        _i32(t, name)
-        if t.numel() < n:
-            raise ValueError(f"{name} is too small for num_seqs")
+            not out.is_contiguous() or q.get_device() != dev or out.get_device() != dev:
+        raise ValueError("q and out must be contiguous (tokens, q_heads, 128) of one dtype on the "
+                         "cache's device")
+    _q4_index(block_tables, "block_tables", dev)
+    _q4_index(cu_seqlens_q, "cu_seqlens_q", dev)
+    _q4_index(seq_lens_k, "seq_lens_k", dev)
     if block_tables.dim() != 2 or (seq_bt_row is None and block_tables.shape[0] < num_seqs):
         raise ValueError("block_tables must be [rows][pitch] with a row per sequence")
-    for t in (q, out, block_tables, cu_seqlens_q, seq_lens_k):
-        if t.device != kv_cache.device:
-            raise ValueError("every tensor must be on the cache's device")
-    scale = (1.0 / D ** 0.5) if scale is None else scale
-    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    with _on(q.device):
+    if cu_seqlens_q.numel() <= num_seqs or seq_lens_k.numel() < num_seqs:
+        raise ValueError("cu_seqlens_q or seq_lens_k is too small for num_seqs")
+    if seq_bt_row is not None:
+        _q4_index(seq_bt_row, "seq_bt_row", dev)
+        if seq_bt_row.numel() < num_seqs:
+            raise ValueError("seq_bt_row is too small for num_seqs")
+    if err is not None:
+        _q4_index(err, "err", dev)
+    if workspace is None:
+        ws_bytes = 0
+    else:
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous and on the cache's device")
+        ws_bytes = workspace.numel() * workspace.element_size()
+    scale = 128 ** -0.5 if scale is None else scale
+    with _on(dev):
         check(_lib.load().hy_varlen_attention_q4(
-            _dt(q), _ptr(q), _ptr(out), T, q_heads, kv_heads, _ptr(kv_cache), L, NB, layer,
-            _ptr(block_tables), block_tables.shape[1], _ptr(seq_bt_row), _ptr(cu_seqlens_q),
-            _ptr(seq_lens_k), num_seqs, float(scale), max_seqs, max_tokens, _ptr(workspace),
-            ws_bytes, _ptr(err), _stream()), "hy_varlen_attention_q4")
+            _dt(q), q.data_ptr(), out.data_ptr(), T, q_heads, kv_heads, kv_cache.data_ptr(), L, NB,
+            layer, block_tables.data_ptr(), block_tables.shape[1], _ptr(seq_bt_row),
+            cu_seqlens_q.data_ptr(), seq_lens_k.data_ptr(), num_seqs, scale, max_seqs, max_tokens,
+            _ptr(workspace), ws_bytes, _ptr(err), _stream()), "hy_varlen_attention_q4")
 
 
 def add_rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float,
