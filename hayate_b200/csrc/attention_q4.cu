@@ -655,9 +655,9 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
     __syncthreads();                                      // parts are read
     return true;
   }
-  __threadfence();                                        // this CTA's partials, before the count
   __syncthreads();
   if (tid == 0) {
+    __threadfence();                                      // this CTA's partials, before the count
     int last = 0;
     for (int j = 0; j < n_open; ++j) {
       const Part& p = sh.part[open_at[j]];
@@ -668,11 +668,11 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
       }
     }
     sh.last = last;
+    __threadfence();                                      // the others' partials, after the count
   }
   __syncthreads();
   const int last = sh.last;
   if (last == 0) return true;
-  __threadfence();                                        // the others' partials, after the count
   for (int j = 0; j < n_open; ++j) {
     if (!((last >> j) & 1)) continue;
     const Part p = sh.part[open_at[j]];
@@ -683,6 +683,13 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
     float M = -INFINITY, L = 0.f, acc = 0.f;
     for (int c0 = u0; c0 <= u1; c0 += 32) {               // 32 partials (none is empty), one weight per lane
       const int cnt = min(32, u1 - c0 + 1);
+      float po[8];                                        // 8 partials in flight, beside the weights
+      auto load8 = [&](int i) {
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          po[t] = i + t < cnt ? __ldcg(v.part_o + slot(c0 + i + t) * (HY_GROUP * HY_HEAD_DIM) + tid) : 0.f;
+      };
+      load8(0);
       const float2 e = lane < cnt ? __ldcg(v.part_ml + slot(c0 + lane) * HY_GROUP + h) : make_float2(-INFINITY, 0.f);
       float m_new = fmaxf(M, e.x);
 #pragma unroll
@@ -694,11 +701,8 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
       for (int o = 16; o > 0; o >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, o);
       L = fmaf(L, old, lw);
       acc *= old;
-      for (int i = 0; i < cnt; i += 8) {                  // 8 loads in flight
-        float po[8];
-#pragma unroll
-        for (int t = 0; t < 8; ++t)
-          po[t] = i + t < cnt ? __ldcg(v.part_o + slot(c0 + i + t) * (HY_GROUP * HY_HEAD_DIM) + tid) : 0.f;
+      for (int i = 0; i < cnt; i += 8) {
+        if (i > 0) load8(i);
 #pragma unroll
         for (int t = 0; t < 8; ++t) acc = fmaf(__shfl_sync(0xffffffffu, w, (i + t) & 31), po[t], acc);
       }
@@ -1066,15 +1070,15 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
 
 // The step's decode sequences.  Alone in the launch, their key blocks are dealt evenly
 // over the CTAs; a small step's pairs go one to a CTA, which merges them in shared memory;
-// beside prefill items, whose CTAs come late, CTAs take units of a third of an even
-// share.  Returns false if a wait ran out.
-constexpr int MIXED_UNITS = 3;
+// beside prefill items, whose CTAs come late, CTAs take the even shares as they become
+// free (a share costs about 10 us beside its blocks: 4 chunks and 128 decodes take 147 us
+// with a share per CTA, 159 with two smaller ones and 169 with three).  Returns false if a wait ran out.
 __device__ bool decode_all(const Args& a, const PlanView& v, int n_pre, int n_pairs, int blocks,
                            SeqInfo top, uint8_t* payload, Shared& sh) {
   uint32_t ring_pos = 0, ring_par = 0;
   const int total = blocks * a.kv_heads;                  // below 2^31: the host checks the tables' size
   if (total == 0) return true;
-  const Units units(total, n_pre > 0 ? MIXED_UNITS * (int)gridDim.x : (int)gridDim.x);
+  const Units units(total, (int)gridDim.x);
   int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
   int u = blockIdx.x;
   for (;;) {
