@@ -298,6 +298,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
   enum { PRE, DEC, PART, BLK, UNIT, SUMS };     // UNIT: (query tile, KV head) pairs
   __shared__ int s_first_dec[PLAN_THREADS], s_first_unit[PLAN_THREADS];
   __shared__ int s_pre0[PLAN_THREADS], s_slot0[PLAN_THREADS];
+  __shared__ int s_row[PLAN_THREADS], s_kv[PLAN_THREADS], s_ns[PLAN_THREADS];
+  __shared__ unsigned s_inv[PLAN_THREADS];      // 2^32 / ns, rounded up
   __shared__ int s_wsn[SUMS][32];
   for (int base = 0; base < S; base += PLAN_THREADS) {
     const int i = base + threadIdx.x;
@@ -305,7 +307,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
     int ph = 0, psl = 0;                        // pieces and partial slots per KV head
     int sums[SUMS] = {0, 0, 0, 0, 0}, total[SUMS];
     if (i < S) {
-      const int q = cu_q[i + 1] - cu_q[i], kv = seq_lens_k[i];
+      const int row = cu_q[i], q = cu_q[i + 1] - row, kv = seq_lens_k[i];
+      s_row[threadIdx.x] = row;
+      s_kv[threadIdx.x] = kv;
       if (q < 0 || kv < q) atomicOr(&s_bad, HY_ERR_BOUNDS);
       else if (q == 1) {
         nblk = (kv + HY_BLOCK - 1) / HY_BLOCK;
@@ -332,6 +336,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
     s_first_unit[threadIdx.x] = sums[UNIT];
     s_pre0[threadIdx.x] = p0;
     s_slot0[threadIdx.x] = s0;
+    s_ns[threadIdx.x] = ns;
+    s_inv[threadIdx.x] = ns > 1 ? 0xffffffffu / (unsigned)ns + 1u : 0u;
     if (i < S) {
       if (p0 + npre > v.max_pre || d0 + ndec > v.max_dec || i >= v.max_seqs ||
           s0 + npart > v.max_pre_part) {
@@ -348,11 +354,15 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
       // by at most one block)
       for (int k = threadIdx.x; k < total[DEC]; k += PLAN_THREADS) {
         const int j = plan_find(s_first_dec, k), ji = base + j, kj = k - s_first_dec[j];
-        const int jrow = cu_q[ji], jkv = seq_lens_k[ji];
+        const int jrow = s_row[j], jkv = s_kv[j], jns = s_ns[j];
         const int jnb = (jkv + HY_BLOCK - 1) / HY_BLOCK;
-        const int jns = group ? max(1, min(ATT_WARPS, jnb)) : (jnb + split - 1) / split;
-        const int g = kj / jns, sp = kj - g * jns;
-        const int lo = mul_div(sp, jnb, jns), hi = mul_div(sp + 1, jnb, jns);
+        // x / jns by its inverse, exact while x times jns stays below 2^32
+        const unsigned inv = s_inv[j];
+        const bool fast = (long long)jns * jns * max(jnb, kv_heads) <= 0xffffffffLL;
+        auto by_ns = [&](int x) { return jns == 1 ? x : (int)__umulhi((unsigned)x, inv); };
+        const int g = fast ? by_ns(kj) : kj / jns, sp = kj - g * jns;
+        const int lo = fast ? by_ns(sp * jnb) : mul_div(sp, jnb, jns);
+        const int hi = fast ? by_ns((sp + 1) * jnb) : mul_div(sp + 1, jnb, jns);
         v.dec[2 * (cdec + k)] = make_int4(ji, g, lo, hi);
         v.dec[2 * (cdec + k) + 1] = make_int4(jrow, jkv, jns, cdec + k - sp);
         v.dec_ids[2 * (cdec + k)] = make_int4(-1, 0, 0, 0);
