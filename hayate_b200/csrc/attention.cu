@@ -144,6 +144,10 @@ HY_DEVICE uint8_t* payload_base(uint8_t* dyn) {
 
 // ------------------------------------------------------------------ plan kernel
 constexpr int PLAN_THREADS = 1024;
+// Every CTA of the plan counts and scans all sequences (a few us, with no exchange
+// between CTAs); the decode items, up to a few thousand, are dealt over the CTAs (3584
+// items: 6 us in one CTA), the rest is CTA 0's.
+constexpr int PLAN_CTAS = 8;
 
 __device__ int plan_scan(int v, int* ws, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -342,7 +346,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
       if (p0 + npre > v.max_pre || d0 + ndec > v.max_dec || i >= v.max_seqs ||
           s0 + npart > v.max_pre_part) {
         atomicOr(&s_bad, HY_ERR_PLAN);
-      } else {
+      } else if (blockIdx.x == 0) {
         v.seqinfo[i] = make_int2(d0, ns);
         v.dec_blocks[i] = s_cblk + sums[BLK];
         for (int g = 0; g < kv_heads; ++g) v.counters[i * kv_heads + g] = 0;
@@ -352,7 +356,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
     if (s_bad == 0) {
       // decode item k: KV head and split of the sequence it falls into (splits differ
       // by at most one block)
-      for (int k = threadIdx.x; k < total[DEC]; k += PLAN_THREADS) {
+      for (int k = blockIdx.x * PLAN_THREADS + threadIdx.x; k < total[DEC];
+           k += gridDim.x * PLAN_THREADS) {
         const int j = plan_find(s_first_dec, k), ji = base + j, kj = k - s_first_dec[j];
         const int jrow = s_row[j], jkv = s_kv[j], jns = s_ns[j];
         const int jnb = (jkv + HY_BLOCK - 1) / HY_BLOCK;
@@ -369,7 +374,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
       }
       // (KV head g, query tile t): its pieces follow those of head g's earlier
       // query tiles; a cut item's pieces take consecutive partial slots
-      for (int k = threadIdx.x; k < total[UNIT]; k += PLAN_THREADS) {
+      for (int k = threadIdx.x; k < total[UNIT] && blockIdx.x == 0; k += PLAN_THREADS) {
         const int j = plan_find(s_first_unit, k), ji = base + j, kj = k - s_first_unit[j];
         const int jq = cu_q[ji + 1] - cu_q[ji], jkv = seq_lens_k[ji];
         const int jnt = (jq + PRE_QROWS - 1) / PRE_QROWS;
@@ -396,6 +401,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
     }
     __syncthreads();
   }
+  if (blockIdx.x != 0) return;
   if (threadIdx.x < 64 * GRAB_INTS) v.grab[threadIdx.x] = 0;
   // Prefill items ordered by their key tiles, most first (a counting sort over
   // PLAN_THREADS cost bins), so that CTAs pulling them in order start the
@@ -1551,7 +1557,7 @@ PlanView hy_attn_plan_view(void* ws, const PlanDims& d) {
 cudaError_t hy_launch_attn_plan(const int32_t* cu_q, const int32_t* seq_lens_k, int S,
                                 int kv_heads, const PlanDims& d, void* ws, int32_t* err,
                                 int dev, cudaStream_t st) {
-  return hy_launch(plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, cu_q, seq_lens_k, S,
+  return hy_launch(plan_kernel, dim3(PLAN_CTAS), dim3(PLAN_THREADS), 0, st, cu_q, seq_lens_k, S,
                    kv_heads, hy_attn_warp_slots(dev), hy_attn_plan_view(ws, d), err);
 }
 
