@@ -229,7 +229,7 @@ HY_DEVICE int mul_div(int a, int b, int c) {
 
 __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ seq_lens_k, int S,
-    int kv_heads, int warp_slots, PlanView v, int32_t* err) {
+    int kv_heads, int warp_slots, int block_cap, PlanView v, int32_t* err) {
   hy_grid_wait();
   hy_grid_trigger();
   __shared__ int ws[32];
@@ -245,13 +245,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
   int part = 0, mxb = 0, pre = 0, ptiles = 0, pitems = 0;
   for (int i = threadIdx.x; i < S; i += PLAN_THREADS) {
     const int q = cu_q[i + 1] - cu_q[i], kv = seq_lens_k[i];
-    if (q == 1) {
+    if (q == 1 && kv <= SEQ_MAX_KEYS) {
       const int nb = (kv + HY_BLOCK - 1) / HY_BLOCK;
       part += nb;
       mxb = max(mxb, nb);
     } else if (q > 1) {
       pre = 1;
-      if (kv >= q)
+      if (seq_fits(q, kv))
         for (int t0 = 0; t0 < q; t0 += PRE_QROWS) {
           ptiles += pre_item_tiles(kv, q, t0);
           ++pitems;
@@ -314,12 +314,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
       const int row = cu_q[i], q = cu_q[i + 1] - row, kv = seq_lens_k[i];
       s_row[threadIdx.x] = row;
       s_kv[threadIdx.x] = kv;
-      if (q < 0 || kv < q) atomicOr(&s_bad, HY_ERR_BOUNDS);
+      if (!seq_fits(q, kv)) atomicOr(&s_bad, HY_ERR_BOUNDS);
       else if (q == 1) {
         nblk = (kv + HY_BLOCK - 1) / HY_BLOCK;
         ns = group ? max(1, min(ATT_WARPS, nblk)) : (nblk + split - 1) / split;
         sums[DEC] = kv_heads * ns;
-        sums[BLK] = nblk;
+        sums[BLK] = min(nblk, block_cap);
       } else if (q > 1) {
         ntile = (q + PRE_QROWS - 1) / PRE_QROWS;
         for (int t = 0; t < ntile; ++t) {
@@ -1558,7 +1558,8 @@ cudaError_t hy_launch_attn_plan(const int32_t* cu_q, const int32_t* seq_lens_k, 
                                 int kv_heads, const PlanDims& d, void* ws, int32_t* err,
                                 int dev, cudaStream_t st) {
   return hy_launch(plan_kernel, dim3(PLAN_CTAS), dim3(PLAN_THREADS), 0, st, cu_q, seq_lens_k, S,
-                   kv_heads, hy_attn_warp_slots(dev), hy_attn_plan_view(ws, d), err);
+                   kv_heads, hy_attn_warp_slots(dev), hy_dec_block_cap(S, kv_heads),
+                   hy_attn_plan_view(ws, d), err);
 }
 
 cudaError_t hy_launch_attn_bf16(const KvMaps& maps, const CUtensorMap& qmap, const void* cache,

@@ -57,10 +57,18 @@ struct PlanView {
   float2* pre_part_ml;// [max_pre_part][256] (running max in log2 units, sum) per row
   int* pre_ctr;       // [max_pre_part] finished pieces, at a split item's first slot
                       // (zeroed by the plan and by the merging piece)
-  int* dec_blocks;    // [max_seqs + 1] key blocks of the decode sequences before each
-                      // sequence (the 4-bit cache's kernel deals blocks, not items)
+  int* dec_blocks;    // [max_seqs + 1] key blocks (as hy_dec_block_cap cuts them) of the
+                      // decode sequences before each sequence (the 4-bit cache's kernel
+                      // deals blocks, not items)
   int max_pre, max_dec, max_seqs, max_pre_part;
 };
+
+// The most key blocks that dec_blocks counts of one sequence, so that those of all S
+// sequences and KV heads stay below 2^31.  hy_varlen_attention_q4 refuses block tables
+// with longer rows: only a sequence longer than its row is cut.
+inline int hy_dec_block_cap(int S, int kv_heads) {
+  return (int)(0x7fffffffLL / ((long long)S * kv_heads));
+}
 
 int hy_attn_warp_slots(int dev);
 // split_prefill false: a plan on these dimensions splits no prefill item over

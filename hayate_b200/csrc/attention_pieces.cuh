@@ -33,6 +33,11 @@ constexpr int PRE_SPLIT_MIN = HY_PRE_SPLIT_MIN;                  // key tiles
 constexpr int PRE_MAX_PIECES = 31;
 constexpr int PRE_PART_F4 = 32 * 256;                            // float4 of O per piece
 
+// A sequence that the plan takes: keys for all its query tokens, and no more of them
+// than any pool holds (2^28; the plan sums the tiles of up to an item per SM in 32 bits).
+constexpr int SEQ_MAX_KEYS = 1 << 28;
+HY_DEVICE bool seq_fits(int q, int kv) { return q >= 0 && kv >= q && kv <= SEQ_MAX_KEYS; }
+
 // key tiles of the prefill item at query offset t0 of a sequence of q query
 // tokens and kv keys
 HY_DEVICE int pre_item_tiles(int kv, int q, int t0) {

@@ -20,6 +20,7 @@
 #include "q4.cuh"
 
 #include <atomic>
+#include <limits.h>
 #include <math.h>
 
 namespace {
@@ -28,10 +29,7 @@ constexpr int NW = 16;                                    // warps per CTA
 constexpr int NT = NW * 32;
 constexpr int BLK_BYTES = 2 * Q4_TILE_BYTES;              // K and V tile of one block and head
 constexpr int STAGE_BYTES = 2 * BLK_BYTES;                // a decode warp takes two blocks at a time
-#ifndef HY_Q4_STAGES
-#define HY_Q4_STAGES 2
-#endif
-constexpr int NS = HY_Q4_STAGES;                          // stages of a decode warp's ring
+constexpr int NS = 2;                                     // stages of a decode warp's ring
 constexpr int RING_BYTES = NS * STAGE_BYTES;
 // a warp's partial result of one (sequence, head): O [4][128], then (m, l) [4]
 constexpr int PART_FLOATS = HY_GROUP * HY_HEAD_DIM + 2 * HY_GROUP;
@@ -61,6 +59,7 @@ struct Args {
   __nv_bfloat16* out;
   const uint8_t* cache;   // this layer's tiles
   int q_heads, kv_heads, num_blocks, layer, num_seqs;
+  int block_cap;          // hy_dec_block_cap
   const int32_t* block_tables;
   int bt_pitch;
   const int32_t* seq_bt_row;
@@ -114,6 +113,7 @@ struct Shared {
   uint64_t itemfree;      // every warp has read it (one arrival each)
   uint64_t expdone;       // the item's last tile is about to be expanded (one arrival per expanding warp)
   PreItem item[2];
+  int nan_at[2][2];       // [item n % 2][half]: the first key whose value is NaN there
   uint32_t tmem_base;
   int pre_last;
 };
@@ -162,7 +162,7 @@ HY_DEVICE void cursor_sequence(const Args& a, Cursor& k, const SeqInfo& s) {
   k.first = s.first;
   k.tok = s.tok;
   k.kv_len = s.kv_len;
-  k.nb = (s.kv_len + HY_BLOCK - 1) / HY_BLOCK;            // as the plan counts them
+  k.nb = min((s.kv_len + HY_BLOCK - 1) / HY_BLOCK, a.block_cap);   // as the plan counts them
   k.row = s.row;
 }
 // The place of flattened block f: the last sequence that starts at or before it, found
@@ -583,7 +583,8 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
     k.seq = unit / a.kv_heads;
     k.g = unit - k.seq * a.kv_heads;
     cursor_sequence(a, k, seq_info(a, v, k.seq));
-    n = a.cu_q[k.seq + 1] - k.tok == 1 ? k.nb : 0;        // no decode token: no blocks
+    const int q_len = a.cu_q[k.seq + 1] - k.tok;          // not a decode sequence: no blocks
+    n = q_len == 1 && seq_fits(q_len, k.kv_len) ? k.nb : 0;
   } else {
     n = units.start(unit + 1) - f0;
   }
@@ -728,13 +729,27 @@ HY_DEVICE PreItem pre_item_geom(const Args& a, const PlanView& v, int item) {
   p.nrows = min(PRE_QROWS, q_len - p.t0);
   p.kv_end = p.prefix + p.t0 + p.nrows;                   // keys its last row sees
   pre_piece_range(p.w, (p.kv_end + PRE_KEYS - 1) / PRE_KEYS, p.tlo, p.thi);
+  // a sequence longer than its block-table row: no tiles past the row (but one at least,
+  // which the roles count on)
+  const long row_tiles = ((long)a.bt_pitch * HY_BLOCK + PRE_KEYS - 1) / PRE_KEYS;
+  if (p.thi > row_tiles) {
+    hy_flag(a.err, HY_ERR_BOUNDS);
+    p.thi = (int)max(row_tiles, 1L);
+    p.tlo = min(p.tlo, p.thi - 1);
+  }
   return p;
 }
 
 // Expanding warps: thread t of 128 takes row t % 64 of every key tile's K (t < 64) or
 // V: its 64 code bytes and parameters from global memory, the next tile's loaded
 // ahead, to 256 bytes of fp16 in the ring.  Rows past the item's keys become zeros:
-// their scores are masked, and a zero weight times a zero adds nothing.
+// their scores are masked, and a zero weight times a zero adds nothing.  A half of V
+// whose parameters are NaN (its codes are 0 then) is expanded to fp16's lowest number, so
+// that a later token's does not reach the rows that do not see it; its key is noted, and
+// the softmax warps write NaN where a row does see it.  (16 chunks of 512 tokens: 393 us
+// with this, 389 without; zeroing the half in a branch before it is expanded, 402.)
+constexpr uint32_t VALUE_LEAST = 0xfbff0000u;             // parameters are at least (0, -65504)
+constexpr uint32_t KEY_LEAST = 0x7fff7fffu;               // NaN: whatever they are
 struct RowCodes {
   uint4 w[4];
   uint32_t par[2];
@@ -761,10 +776,10 @@ HY_DEVICE void load_row(const Args& a, const PreItem& P, int part, int pos, int 
   x.par[0] = p.x;
   x.par[1] = p.y;
 }
-HY_DEVICE void expand_row(const RowCodes& x, uint8_t* slot, int key) {
+HY_DEVICE void expand_row(const RowCodes& x, uint8_t* slot, int key, uint32_t at_least) {
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const __half2 sm = q4_as_half2(x.par[half]);
+    const __half2 sm = __hmax2(q4_as_half2(x.par[half]), q4_as_half2(at_least));
     const __half2 s2 = __low2half2(sm), m2 = __high2half2(sm);
     uint8_t* row = slot + half * (KV_BYTES / 2) + key * 128;
 #pragma unroll
@@ -776,6 +791,19 @@ HY_DEVICE void expand_row(const RowCodes& x, uint8_t* slot, int key) {
       *reinterpret_cast<uint4*>(row + ((i ^ (key & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
     }
   }
+}
+
+// 64 columns of O become NaN in the lanes that say so (the whole warp takes part).
+HY_DEVICE void nan_half(uint32_t t, bool on) {
+#pragma unroll 1
+  for (int i = 0; i < 64; i += 16) {
+    float o[16];
+    tmem_ld16(t + i, o);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) o[k] = on ? __int_as_float(0x7fffffff) : o[k];
+    tmem_st16(t + i, o);
+  }
+  tmem_wait_st();
 }
 
 // The CTA's prefill items, taken from the counter `next` until there are no more.  Each
@@ -818,6 +846,7 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
         if (n > 0) ok = mbar_wait(&sh.itemfree, (n - 1) & 1, a.err);
         if (!ok) break;
         sh.item[n & 1] = N;
+        sh.nan_at[n & 1][0] = sh.nan_at[n & 1][1] = INT_MAX;
         mbar_arrive(&sh.itemfull);
         if (N.seq < 0) break;
         if (n > 0) ok = mbar_wait(&sh.qfree, (n - 1) & 1, a.err);
@@ -851,7 +880,13 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
         if (t == ntiles - 1 && lane == 0) mbar_arrive(&sh.expdone);
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.free_[slot], ((c / PS) & 1) ^ 1, a.err));
         if (!ok) break;
-        expand_row(cur, ring + slot * KV_BYTES, key);
+        expand_row(cur, ring + slot * KV_BYTES, key, part ? VALUE_LEAST : KEY_LEAST);
+        // a minimum of NaN: above the scale's 16 bits, an exponent of ones and a mantissa
+        if (max(cur.par[0] << 1, cur.par[1] << 1) >= 0xf8020000u && part) {
+          for (int half = 0; half < 2; ++half)
+            if ((half ? cur.par[1] : cur.par[0]) << 1 >= 0xf8020000u)
+              atomicMin(&sh.nan_at[n & 1][half], pos - PRE_KEYS);
+        }
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.full[slot]);
@@ -1035,6 +1070,9 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
         const uint32_t c = c0 - 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.odone[X][c & 1], (c >> 1) & 1, a.err));
         tc_fence_after();
+        for (int half = 0; half < 2; ++half)
+          if (__any_sync(0xffffffffu, sh.nan_at[n & 1][half] <= lim))
+            nan_half(tO + 64 * half, sh.nan_at[n & 1][half] <= lim);
       }
       const bool store = ok && real;
       __nv_bfloat16* op = a.out + ((size_t)(P.row0 + P.t0 + j) * a.q_heads + P.g * HY_GROUP + 2 * X + (r >> 6)) *
@@ -1346,6 +1384,7 @@ cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap& q_map, const void* q, void
   a.num_blocks = num_blocks;
   a.layer = layer;
   a.num_seqs = S;
+  a.block_cap = hy_dec_block_cap(S, kv_heads);
   a.block_tables = block_tables;
   a.bt_pitch = bt_pitch;
   a.seq_bt_row = seq_bt_row;

@@ -17,10 +17,7 @@ namespace {
 constexpr int Q4_THREADS = 256;
 constexpr int Q4_LANES = HY_HEAD_DIM / 16;            // lanes per row
 constexpr int Q4_ROWS = Q4_THREADS / Q4_LANES;        // rows per CTA pass
-#ifndef HY_Q4_UNROLL
-#define HY_Q4_UNROLL 2
-#endif
-constexpr int Q4_UNROLL = HY_Q4_UNROLL;               // rows in flight per lane
+constexpr int Q4_UNROLL = 2;                          // rows in flight per lane
 
 // min and max that are NaN if either operand is
 HY_DEVICE float min_nan(float a, float b) {

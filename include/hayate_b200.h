@@ -233,11 +233,15 @@ int hy_varlen_attention_noalloc(const void* q, void* out, int32_t num_tokens, in
 /* hy_varlen_attention over the 4-bit cache: the same sequences, block tables,
  * plan and workspace, with kv_cache [num_layers][num_blocks][kv_heads][2]
  * [HY_Q4_TILE_BYTES] (16-byte aligned) and keys and values what their codes
- * stand for; scale is finite and not negative.  Rows of q past the last sequence (cu_seqlens_q[num_seqs]) leave
- * out as it was.  A block id outside the pool, a sequence longer than its
- * block-table row or with fewer keys than query tokens ORs HY_DEV_BOUNDS into
- * err; the sequence's output rows are then not meaningful.  bf16 needs the
- * planned workspace; fp32 runs a scalar kernel for parity runs and ignores it.
+ * stand for; scale is finite and not negative.  Rows of q past the last
+ * sequence (cu_seqlens_q[num_seqs]) leave out as it was.  A block id outside
+ * the pool or a sequence longer than its block-table row ORs HY_DEV_BOUNDS into
+ * err, and the sequence's output rows are not meaningful; so does one of fewer
+ * keys than query tokens (or of more than 2^28), which the plan refuses with
+ * its whole batch: a bf16 call then writes no row.  A NaN in the cache reaches
+ * the query rows that see its key, of its KV head (a value's half row: that
+ * half of their outputs), and no others.  bf16 needs the planned workspace;
+ * fp32 runs a scalar kernel for parity runs and ignores it.
  * Replaces: as hy_varlen_attention. */
 int hy_varlen_attention_q4(int32_t dtype, const void* q, void* out, int32_t num_tokens,
                            int32_t q_heads, int32_t kv_heads, const void* kv_cache,
