@@ -130,6 +130,7 @@ struct Shared {
   uint64_t tc_odone[2][2];   // O_X += P_X[b] V complete (once per use of buffer b)
   uint64_t tc_drain[2];      // error path: all MMAs an issuing warp issued are complete
   uint64_t tc_qfull;         // the item's Q landed (TMA transaction bytes, once per item)
+  uint64_t tc_qfree;         // S of both sub-tiles' last tile complete (2 commits, once per item)
   uint32_t tmem_base;        // TMEM columns from tcgen05.alloc
   int pre_item;              // prefill item handed to this CTA
   int pre_last;              // this CTA's piece of a split prefill item finished last
@@ -965,10 +966,9 @@ HY_DEVICE bool pre_issue_tile(const CUtensorMap* kgroups, const CUtensorMap* til
 // rescale O.
 // c = c0 + t counts key tiles over all items of the launch; each barrier
 // completes exactly once per use of its buffer (sfull, pfull, odone: every second
-// tile) or per use of its slot (ring barriers), and no role can
-// run a full phase ahead of the role that waits on it, so a wait is always on
-// the current or the previous phase (the load warps, which can get ahead of
-// the S MMAs of a short item, wait for its S phases in order).  Returns false if a wait ran out; the
+// tile), per use of its slot (ring barriers) or per item (qfull, qfree), and no role
+// can run a full phase ahead of the role that waits on it, so a wait is always on
+// the current or the previous phase.  Returns false if a wait ran out; the
 // roles then drain their own asynchronous work before the item ends.
 __device__ bool prefill_item_tc(const CUtensorMap* kgroups, const CUtensorMap* tiles,
                                 const CUtensorMap* qmap, const MainArgs& a, const PlanView& v,
@@ -1030,16 +1030,9 @@ __device__ bool prefill_item_tc(const CUtensorMap* kgroups, const CUtensorMap* t
       int nx = ok ? atomicAdd(next_ctr, 1) : 0x7fffffff;
       bool go = nx < n_pre;
       if (go) {
-        // S of this item's last tile cl, after S of tile cl - 2 (the same S
-        // buffer): waiting in order keeps each parity wait on the barrier's
-        // current or previous phase (a short item whose tiles were all loaded
-        // ahead gets here before its first S, two phases behind; phases before
-        // cl - 2 completed before the load of tile cl was issued, or belong to
-        // the previous item)
-        const uint32_t cl = c0 + ntiles - 1;
-        for (uint32_t c = ntiles >= 3 ? cl - 2 : cl; go && c <= cl; c += 2)
-          go = mbar_wait(&sh.tc_sfull[0][c & 1], (c >> 1) & 1, a.err) &&
-               mbar_wait(&sh.tc_sfull[1][c & 1], (c >> 1) & 1, a.err);
+        // once per item: no later phase can complete before this one is seen (a wait on
+        // the S barriers, which complete every second tile, could come after two)
+        go = mbar_wait(&sh.tc_qfree, qpar, a.err);
         if (!go) {                              // the CTA stops after this item
           ok = false;
           nx = 0x7fffffff;
@@ -1108,6 +1101,7 @@ __device__ bool prefill_item_tc(const CUtensorMap* kgroups, const CUtensorMap* t
                         dK + (uint64_t)((((kk >> 2) * 1024) + (kk & 3) * 32) >> 4), ID_S,
                         kk > 0);
           tc_commit(&sh.tc_sfull[X][c & 1]);
+          if (t == ntiles - 1) tc_commit(&sh.tc_qfree);
         }
         if (t > 0) {                            // O_X += P_X(t-1) V_{t-1}
           const uint32_t c = c0 + t - 1, slot = c % TC_NS;
@@ -1284,6 +1278,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_main_kernel(
         mbar_init(&sh.tc_odone[x][b], 1);
       }
     }
+    mbar_init(&sh.tc_qfree, 2);
     mbar_init(&sh.tc_drain[0], 1);
     mbar_init(&sh.tc_drain[1], 1);
     mbar_init(&sh.tc_qfull, 1);
