@@ -102,8 +102,10 @@ cudaError_t hy_launch_attn_fp32(const float* q, float* out, int T, int q_heads, 
                                 const int32_t* seq_lens_k, int S, float scale, int32_t* err,
                                 cudaStream_t st);
 
-// The 4-bit cache (attention_q4.cu); cache_layer: the layer's first tile.
-cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap& q_map, const void* q, void* out, int q_heads, int kv_heads,
+// The 4-bit cache (attention_q4.cu); cache_layer: the layer's first tile.  q_map null:
+// the kernel for decode steps.
+cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap* q_map, const void* q, void* out, int tokens,
+                                   int q_heads, int kv_heads,
                                    const void* cache_layer, int num_blocks, int layer,
                                    const int32_t* block_tables, int bt_pitch,
                                    const int32_t* seq_bt_row, const int32_t* cu_q,

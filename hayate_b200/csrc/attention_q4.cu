@@ -33,7 +33,7 @@ constexpr int NS = 2;                                     // stages of a decode 
 constexpr int RING_BYTES = NS * STAGE_BYTES;
 // a warp's partial result of one (sequence, head): O [4][128], then (m, l) [4]
 constexpr int PART_FLOATS = HY_GROUP * HY_HEAD_DIM + 2 * HY_GROUP;
-constexpr int DEC_SMEM = NW * (RING_BYTES + 2 * PART_FLOATS * 4);
+constexpr int DEC_SMEM = NW * (RING_BYTES + 2 * PART_FLOATS * 4) + 1024;   // + alignment
 constexpr float RESCALE_LOG2 = 8.0f;                      // see decode_warp
 
 // Prefill: warps 0-3 / 4-7 softmax of sub-tile 0 / 1, 8-11 expand, 12 / 13 issue the
@@ -48,7 +48,7 @@ constexpr int Q_BYTES = 128 * HY_HEAD_DIM * 2;            // Q of one sub-tile: 
 constexpr int KV_BYTES = PRE_KEYS * HY_HEAD_DIM * 2;      // K or V of one tile: 16 KB
 constexpr int K_OFF = 2 * Q_BYTES, V_OFF = K_OFF + PS * KV_BYTES;
 constexpr int PRE_SMEM = V_OFF + PS * KV_BYTES;           // 192 KB
-constexpr int SMEM_BYTES = (PRE_SMEM > DEC_SMEM ? PRE_SMEM : DEC_SMEM) + 1024;   // + alignment
+constexpr int MIXED_SMEM = PRE_SMEM + 1024 > DEC_SMEM ? PRE_SMEM + 1024 : DEC_SMEM;
 // TMEM columns: two S buffers per sub-tile, P (fp16 pairs) written over the first half
 // of its S; O at 256 + 128 X.
 constexpr uint32_t TMEM_COLS = 512, TM_O = 256;
@@ -58,7 +58,7 @@ struct Args {
   const __nv_bfloat16* q;
   __nv_bfloat16* out;
   const uint8_t* cache;   // this layer's tiles
-  int q_heads, kv_heads, num_blocks, layer, num_seqs;
+  int q_heads, kv_heads, num_blocks, layer, num_seqs, num_tokens;
   int block_cap;          // hy_dec_block_cap
   const int32_t* block_tables;
   int bt_pitch;
@@ -569,28 +569,16 @@ struct Units {            // `total` blocks in n units whose sizes differ by at 
   }
 };
 
-// (small: a unit is the pair `unit` / `unit` % kv_heads alone)
-HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units, int unit, bool small,
-                           const SeqInfo& top, uint8_t* payload, Shared& sh, uint32_t& ring_pos,
-                           uint32_t& ring_par) {
+// alone: the unit is the n blocks of one pair, k; else blocks f0 .. f0 + n - 1.
+HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units, int unit, bool alone,
+                           Cursor k, int f0, int n, const SeqInfo& top, uint8_t* payload, Shared& sh,
+                           uint32_t& ring_pos, uint32_t& ring_par) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   float* parts = reinterpret_cast<float*>(payload + NW * RING_BYTES);
   if (lane < 2) sh.part[2 * warp + lane].pair = -1;
-  const int f0 = small ? 0 : units.start(unit);
-  Cursor k;
-  int n;
-  if (small) {
-    k.seq = unit / a.kv_heads;
-    k.g = unit - k.seq * a.kv_heads;
-    cursor_sequence(a, k, seq_info(a, v, k.seq));
-    const int q_len = a.cu_q[k.seq + 1] - k.tok;          // not a decode sequence: no blocks
-    n = q_len == 1 && seq_fits(q_len, k.kv_len) ? k.nb : 0;
-  } else {
-    n = units.start(unit + 1) - f0;
-  }
   const int per = n / NW, more = n - per * NW;            // the first `more` warps take one more
   const int at = warp * per + min(warp, more), count = per + (warp < more);
-  if (small) k.b = at;
+  if (alone) k.b = at;
   else if (count > 0) k = cursor_at(a, v, top, f0 + at);
   if (lane < 2) sh.cur[warp][lane] = k;
   __syncwarp();
@@ -1106,33 +1094,41 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
   return !__syncthreads_or(!ok);
 }
 
-// The step's decode sequences.  Alone in the launch, their key blocks are dealt evenly
-// over the CTAs; a small step's pairs go one to a CTA, which merges them in shared memory;
-// beside prefill items, whose CTAs come late, CTAs take the even shares as they become
-// free (a share costs about 10 us beside its blocks: 4 chunks and 128 decodes take 147 us
-// with a share per CTA, 159 with two smaller ones and 169 with three).  Returns false if a wait ran out.
-__device__ bool decode_all(const Args& a, const PlanView& v, int n_pre, int n_pairs, int blocks,
-                           SeqInfo top, uint8_t* payload, Shared& sh) {
+// The decode sequences of a step with prefill items: their key blocks in even shares, one
+// per CTA, that CTAs take as they become free (a share costs about 10 us beside its
+// blocks: 4 chunks and 128 decodes take 147 us with a share per CTA, 159 with two smaller
+// ones and 169 with three).  Returns false if a wait ran out.
+__device__ bool decode_shares(const Args& a, const PlanView& v, int n_pre, int blocks, uint8_t* payload,
+                              Shared& sh) {
   uint32_t ring_pos = 0, ring_par = 0;
   const int total = blocks * a.kv_heads;                  // below 2^31: the host checks the tables' size
   if (total == 0) return true;
   const Units units(total, (int)gridDim.x);
   int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
-  int u = blockIdx.x;
   for (;;) {
-    if (n_pre > 0) {
-      if (threadIdx.x == 0) sh.unit = atomicAdd(&grab[0], 1);
-      __syncthreads();
-      u = sh.unit;
-      __syncthreads();
-      top = seq_top(a, v);
-    }
-    if (u >= (n_pairs > 0 ? n_pairs : units.n)) return true;
-    if (!decode_unit(a, v, units, u, n_pairs > 0, top, payload, sh, ring_pos, ring_par)) return false;
-    if (n_pre == 0) return true;
+    if (threadIdx.x == 0) sh.unit = atomicAdd(&grab[0], 1);
+    __syncthreads();
+    const int u = sh.unit;
+    __syncthreads();
+    if (u >= units.n) return true;
+    const int f0 = units.start(u);
+    if (!decode_unit(a, v, units, u, false, Cursor{}, f0, units.start(u + 1) - f0, seq_top(a, v), payload,
+                     sh, ring_pos, ring_par))
+      return false;
   }
 }
 
+// The sequence of query row `tok`: the last that starts at or before it.
+HY_DEVICE int seq_of_row(const Args& a, int tok) {
+  int lo = 0, hi = a.num_seqs;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu_q[mid] <= tok) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// Steps that may hold prefill chunks (more query rows than sequences).
 __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(const __grid_constant__ CUtensorMap q_map,
                                                           Args a, PlanView v) {
   __shared__ Shared sh;
@@ -1167,8 +1163,7 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(const __grid_constant__ 
   hy_grid_wait();
   hy_grid_trigger();
   const uint64_t keep = l2_keep_policy();
-  const SeqInfo top = seq_top(a, v);
-  const int n_pre = ld_keep(v.header, keep), n_pairs = ld_keep(v.header + 4, keep);
+  const int n_pre = ld_keep(v.header, keep);
   const int blocks = ld_keep(v.header + 5, keep);         // key blocks of the decode sequences
   int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
   bool ok = true;
@@ -1189,15 +1184,66 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(const __grid_constant__ 
       tmem_dealloc(tmem, TMEM_COLS);
     }
   }
-  if (ok) decode_all(a, v, n_pre, n_pairs, blocks, top, payload, sh);
+  if (ok) decode_shares(a, v, n_pre, blocks, payload, sh);
   __syncthreads();
-  if (n_pre > 0 && threadIdx.x == 0) {
+  if (threadIdx.x == 0) {
     __threadfence();                                      // the last CTA out resets the counters
     if (atomicAdd(&grab[1], 1) == (int)gridDim.x - 1) {
       atomicExch(&grab[0], 0);
       atomicExch(&grab[2], 0);
       atomicExch(&grab[1], 0);
     }
+  }
+}
+
+// Steps of no more query rows than sequences, which are decode steps but for sequences
+// without a token: without the prefill's code a launch takes up to 2 us less (10 sequences
+// of 600 keys 10.0 against 10.3 us, one of 40960 23.3 against 25.3).  The key blocks are dealt
+// evenly over the CTAs; a small step's pairs go one to a CTA, which merges them in shared
+// memory.  Rows of longer chunks that such a step may hold all the same are taken one
+// (row, head) at a time, a CTA each.
+__global__ void __launch_bounds__(NT, 1) attn_q4_decode_kernel(Args a, PlanView v) {
+  __shared__ Shared sh;
+  extern __shared__ uint8_t dyn_smem[];
+  uint8_t* payload = dyn_smem + ((1024u - (smem_u32(dyn_smem) & 1023u)) & 1023u);
+  if (threadIdx.x < NW * NS) {
+    mbar_init(&sh.bar[0][0] + threadIdx.x, 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  hy_grid_wait();
+  hy_grid_trigger();
+  const uint64_t keep = l2_keep_policy();
+  const SeqInfo top = seq_top(a, v);                      // with the header: needed by most steps
+  const int n_pre = ld_keep(v.header, keep), n_pairs = ld_keep(v.header + 4, keep);
+  const int total = ld_keep(v.header + 5, keep) * a.kv_heads;   // below 2^31, see decode_shares
+  uint32_t ring_pos = 0, ring_par = 0;
+  const Units units(total, (int)gridDim.x);
+  const int shares = n_pairs > 0 ? n_pairs : total > 0 ? units.n : 0;
+  const long n = shares + (n_pre > 0 ? (long)min(a.num_tokens, a.cu_q[a.num_seqs]) * a.kv_heads : 0);
+  for (long u = blockIdx.x; u < n; u += gridDim.x) {
+    const bool alone = n_pairs > 0 || u >= shares;
+    Cursor k = {};
+    int f0 = 0, blocks;
+    if (alone) {
+      const int i = (int)(u < shares ? u : u - shares) / a.kv_heads;
+      k.g = (int)(u < shares ? u : u - shares) - i * a.kv_heads;
+      k.seq = u < shares ? i : seq_of_row(a, i);
+      SeqInfo s = seq_info(a, v, k.seq);
+      const int q_len = a.cu_q[k.seq + 1] - s.tok;
+      bool take = q_len == 1 && seq_fits(q_len, s.kv_len);
+      if (u >= shares) {                                  // row i, which sees kv_len - (rows after it) keys
+        take = q_len > 1;
+        s.kv_len -= s.tok + q_len - 1 - i;
+        s.tok = i;
+      }
+      cursor_sequence(a, k, s);
+      blocks = take ? k.nb : 0;                           // the others are not this unit's
+    } else {
+      f0 = units.start((int)u);
+      blocks = units.start((int)u + 1) - f0;
+    }
+    if (!decode_unit(a, v, units, (int)u, alone, k, f0, blocks, top, payload, sh, ring_pos, ring_par)) return;
   }
 }
 
@@ -1361,7 +1407,8 @@ cudaError_t hy_launch_attn_q4_fp32(const void* q, void* out, int tokens, int q_h
                    block_tables, bt_pitch, seq_bt_row, cu_q, seq_lens_k, S, scale, err);
 }
 
-cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap& q_map, const void* q, void* out, int q_heads, int kv_heads,
+cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap* q_map, const void* q, void* out, int tokens,
+                                   int q_heads, int kv_heads,
                                    const void* cache_layer, int num_blocks, int layer,
                                    const int32_t* block_tables, int bt_pitch,
                                    const int32_t* seq_bt_row, const int32_t* cu_q,
@@ -1370,8 +1417,10 @@ cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap& q_map, const void* q, void
                                    cudaStream_t st) {
   static std::atomic<bool> attr_set[64];                  // per device, set on its first call
   if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_q4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               SMEM_BYTES);
+    cudaError_t e = cudaFuncSetAttribute(attn_q4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         MIXED_SMEM);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(attn_q4_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DEC_SMEM);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
   }
@@ -1384,6 +1433,7 @@ cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap& q_map, const void* q, void
   a.num_blocks = num_blocks;
   a.layer = layer;
   a.num_seqs = S;
+  a.num_tokens = tokens;
   a.block_cap = hy_dec_block_cap(S, kv_heads);
   a.block_tables = block_tables;
   a.bt_pitch = bt_pitch;
@@ -1392,6 +1442,8 @@ cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap& q_map, const void* q, void
   a.seq_lens_k = seq_lens_k;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = err;
-  return hy_launch(attn_q4_kernel, dim3(hy_attn_num_sms(dev)), dim3(NT), SMEM_BYTES, st, q_map,
-                   a, hy_attn_plan_view(ws, dims));
+  const dim3 grid(hy_attn_num_sms(dev)), block(NT);
+  const PlanView v = hy_attn_plan_view(ws, dims);
+  if (q_map == nullptr) return hy_launch(attn_q4_decode_kernel, grid, block, DEC_SMEM, st, a, v);
+  return hy_launch(attn_q4_kernel, grid, block, MIXED_SMEM, st, *q_map, a, v);
 }

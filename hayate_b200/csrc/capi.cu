@@ -503,10 +503,15 @@ int hy_varlen_attention_q4(int32_t dtype, const void* q, void* out, int32_t num_
   const PlanDims d = hy_attn_plan_dims(max_seqs, max_tokens, kv_heads, dev);
   if (workspace_bytes < hy_attn_workspace_bytes(d))
     return fail(HY_E_INVALID, "hy_varlen_attention_q4: workspace too small for max_seqs/max_tokens");
+  // a step of no more rows than sequences is a decode step but for odd batches, which the
+  // decode kernel runs too
+  const bool decode = num_tokens <= num_seqs;
   CUtensorMap qmap;
-  const int rc = hy_attention_q_map(q, num_tokens, q_heads, &qmap);
-  if (rc) return rc;
-  return cuda_result(hy_launch_attn_q4_bf16(qmap, q, out, q_heads, kv_heads, base,
+  if (!decode) {
+    const int rc = hy_attention_q_map(q, num_tokens, q_heads, &qmap);
+    if (rc) return rc;
+  }
+  return cuda_result(hy_launch_attn_q4_bf16(decode ? nullptr : &qmap, q, out, num_tokens, q_heads, kv_heads, base,
                                             num_blocks, layer, block_tables, bt_pitch, seq_bt_row,
                                             cu_seqlens_q, seq_lens_k, num_seqs, scale, d,
                                             workspace, err, dev, as_stream(stream)),

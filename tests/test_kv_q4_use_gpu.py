@@ -67,6 +67,7 @@ def test_nan_rows_reach_only_the_rows_that_see_them(q_len, kv_len, at, dt):
     (1, [1] * 1100, [1 + 7 * i % 90 for i in range(1100)]),           # more sequences than CTAs and than 32^2
     (2, [1, 0, 3] * 120, [1 + i % 40 + (i % 3) * 2 for i in range(360)]),
     (1, [1] * 300 + [100], [1 + 11 * i % 300 for i in range(300)] + [900]),
+    (2, [0] * 80 + [70, 1], [3] * 80 + [1500, 600]), (8, [0, 2, 0, 1, 2, 0, 1], [9, 2, 5, 700, 33, 1, 1]),
     (1, [1], [100003]), (1, [70], [30011]), (2, [1] * 33 + [5], [40] * 33 + [20000]),
 ])
 def test_attention_many_and_long_sequences(heads, q_lens, kv_lens):
