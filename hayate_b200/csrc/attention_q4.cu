@@ -83,6 +83,13 @@ struct Cursor {
   int first, tok, kv_len, row;                            // of the sequence, see SeqInfo
 };
 
+// Maximum over the warp; NaN only if every lane's is.
+HY_DEVICE float warp_max(float x) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // What a warp leaves of a pair that it did not finish alone.
 struct Part {
   int pair;               // sequence * kv_heads + head, -1: none
@@ -408,9 +415,7 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
           __hmax2(__hmax2(q4_as_half2(va[1].x), q4_as_half2(va[1].y)), __hmax2(q4_as_half2(vb[1].x), q4_as_half2(vb[1].y))));
       const bool grow = mx[0] > thr[0] || mx[1] > thr[1] || __hgt(__low2half(smax2), vcap);
       if (__any_sync(0xffffffffu, grow)) {
-        float smax = __low2float(smax2);
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, d));
+        const float smax = warp_max(__low2float(smax2));
         float vr = 1.f;                                   // change of vs
         if (smax > __half2float(vcap)) {                  // vs = 2^(6 - exponent), at most 2^15
           const int e = min(max((__float_as_int(smax) >> 23) & 255, 118), 254) - 127;
@@ -612,22 +617,29 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
     }
     if ((turn & 3) != (warp >> 2)) continue;              // warp-uniform
     const int tok = __shfl_sync(0xffffffffu, mine.tok, i);
-    float M = in ? ml.x : -INFINITY;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float M = warp_max(in ? ml.x : -INFINITY);
     const float wt = in ? ex2_ftz(ml.x - (M == -INFINITY ? 0.f : M)) : 0.f;
     float L = wt * ml.y;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (unsigned g = group; g; g &= g - 1) {
-      const int j = __ffs(g) - 1;
-      const float w = __shfl_sync(0xffffffffu, wt, j);
-      const float4 p = *reinterpret_cast<const float4*>(parts + j * PART_FLOATS + head * HY_HEAD_DIM + 4 * lane);
-      acc.x = fmaf(w, p.x, acc.x);
-      acc.y = fmaf(w, p.y, acc.y);
-      acc.z = fmaf(w, p.z, acc.z);
-      acc.w = fmaf(w, p.w, acc.w);
+    for (unsigned g = group; g;) {                        // four parts in flight
+      float w[4];
+      float4 p[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int j = g ? __ffs(g) - 1 : i;
+        w[t] = g ? __shfl_sync(0xffffffffu, wt, j) : 0.f;
+        p[t] = *reinterpret_cast<const float4*>(parts + j * PART_FLOATS + head * HY_HEAD_DIM + 4 * lane);
+        g &= g - 1;
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        acc.x = fmaf(w[t], p[t].x, acc.x);
+        acc.y = fmaf(w[t], p[t].y, acc.y);
+        acc.z = fmaf(w[t], p[t].z, acc.z);
+        acc.w = fmaf(w[t], p[t].w, acc.w);
+      }
     }
     const int seq = pair / a.kv_heads, g = pair - seq * a.kv_heads;
     if (blocks == nb) {
@@ -645,18 +657,17 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
     return true;
   }
   __syncthreads();
-  if (tid == 0) {
+  if (warp == 0) {
     __threadfence();                                      // this CTA's partials, before the count
-    int last = 0;
-    for (int j = 0; j < n_open; ++j) {
-      const Part& p = sh.part[open_at[j]];
+    bool mine_last = false;
+    if (lane < n_open) {
+      const int mine_blocks = lane == 0 ? open_blocks[0] : open_blocks[1];
+      const Part& p = sh.part[lane == 0 ? open_at[0] : open_at[1]];
       int* ctr = &v.counters[p.pair];
-      if (atomicAdd(ctr, open_blocks[j]) + open_blocks[j] == p.nb) {
-        last |= 1 << j;
-        *ctr = 0;                                         // for the next launch on this plan
-      }
+      mine_last = atomicAdd(ctr, mine_blocks) + mine_blocks == p.nb;
+      if (mine_last) *ctr = 0;                            // for the next launch on this plan
     }
-    sh.last = last;
+    sh.last = (int)__ballot_sync(0xffffffffu, mine_last);
     __threadfence();                                      // the others' partials, after the count
   }
   __syncthreads();
@@ -664,40 +675,79 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
   if (last == 0) return true;
   for (int j = 0; j < n_open; ++j) {
     if (!((last >> j) & 1)) continue;
-    const Part p = sh.part[open_at[j]];
-    const int g = p.pair % a.kv_heads, h = tid >> 7;
+    // warps 4 i + h, i = 0..3, take every fourth partial's head h, one float4 per lane
+    const Part p = sh.part[j == 0 ? open_at[0] : open_at[1]];
+    const int g = p.pair % a.kv_heads, quarter = warp >> 2;
     const int u0 = units.of(p.first), u1 = units.of(p.first + p.nb - 1);
     const int inside = p.first > units.start(u0);
     auto slot = [&](int u) { return (size_t)(2 * u + (u == u0 ? inside : 0)); };
-    float M = -INFINITY, L = 0.f, acc = 0.f;
-    for (int c0 = u0; c0 <= u1; c0 += 32) {               // 32 partials (none is empty), one weight per lane
-      const int cnt = min(32, u1 - c0 + 1);
-      float po[8];                                        // 8 partials in flight, beside the weights
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c0 = u0 + quarter; c0 <= u1; c0 += 128) {    // 32 partials (none is empty), one weight per lane
+      const int cnt = min(32, (u1 - c0) / 4 + 1);
+      float4 po[8];                                       // 8 partials in flight, beside the weights
       auto load8 = [&](int i) {
 #pragma unroll
         for (int t = 0; t < 8; ++t)
-          po[t] = i + t < cnt ? __ldcg(v.part_o + slot(c0 + i + t) * (HY_GROUP * HY_HEAD_DIM) + tid) : 0.f;
+          if (i + t < cnt)
+            po[t] = __ldcg(reinterpret_cast<const float4*>(
+                               v.part_o + (slot(c0 + 4 * (i + t)) * HY_GROUP + head) * HY_HEAD_DIM) + lane);
+          else po[t] = make_float4(0.f, 0.f, 0.f, 0.f);
       };
       load8(0);
-      const float2 e = lane < cnt ? __ldcg(v.part_ml + slot(c0 + lane) * HY_GROUP + h) : make_float2(-INFINITY, 0.f);
-      float m_new = fmaxf(M, e.x);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, o));
+      const float2 e = lane < cnt ? __ldcg(v.part_ml + slot(c0 + 4 * lane) * HY_GROUP + head)
+                                  : make_float2(-INFINITY, 0.f);
+      const float m_new = warp_max(fmaxf(M, e.x));
       const float mu = m_new == -INFINITY ? 0.f : m_new, old = ex2_ftz(M - mu);
       const float w = ex2_ftz(e.x - mu);
       float lw = w * e.y;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, o);
       L = fmaf(L, old, lw);
-      acc *= old;
+      acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
       for (int i = 0; i < cnt; i += 8) {
         if (i > 0) load8(i);
 #pragma unroll
-        for (int t = 0; t < 8; ++t) acc = fmaf(__shfl_sync(0xffffffffu, w, (i + t) & 31), po[t], acc);
+        for (int t = 0; t < 8; ++t) {
+          const float wt = __shfl_sync(0xffffffffu, w, (i + t) & 31);
+          acc.x = fmaf(wt, po[t].x, acc.x);
+          acc.y = fmaf(wt, po[t].y, acc.y);
+          acc.z = fmaf(wt, po[t].z, acc.z);
+          acc.w = fmaf(wt, po[t].w, acc.w);
+        }
       }
       M = m_new;
     }
-    a.out[((size_t)p.tok * a.q_heads + g * HY_GROUP) * HY_HEAD_DIM + tid] = __float2bfloat16_rn(acc / L);
+    // the four quarters, through shared memory (the warps' parts are read)
+    float* mine4 = parts + (quarter * HY_GROUP + head) * (HY_HEAD_DIM + 4);
+    *reinterpret_cast<float4*>(mine4 + 4 * lane) = acc;
+    if (lane == 0) *reinterpret_cast<float2*>(mine4 + HY_HEAD_DIM) = make_float2(M, L);
+    __syncthreads();
+    if (quarter == 0) {
+      float mm[4], ll[4], m_all = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float2 e = *reinterpret_cast<const float2*>(parts + (t * HY_GROUP + head) * (HY_HEAD_DIM + 4) + HY_HEAD_DIM);
+        mm[t] = e.x;
+        ll[t] = e.y;
+        m_all = fmaxf(m_all, e.x);
+      }
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float w = ex2_ftz(mm[t] - (m_all == -INFINITY ? 0.f : m_all));
+        const float4 x = *reinterpret_cast<const float4*>(parts + (t * HY_GROUP + head) * (HY_HEAD_DIM + 4) + 4 * lane);
+        sum = fmaf(w, ll[t], sum);
+        o.x = fmaf(w, x.x, o.x);
+        o.y = fmaf(w, x.y, o.y);
+        o.z = fmaf(w, x.z, o.z);
+        o.w = fmaf(w, x.w, o.w);
+      }
+      const float inv = 1.f / sum;
+      *reinterpret_cast<uint2*>(a.out + ((size_t)p.tok * a.q_heads + g * HY_GROUP + head) * HY_HEAD_DIM + 4 * lane) =
+          make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    }
+    if (j == 0 && n_open > 1) __syncthreads();            // before the next pair's quarters
   }
   __syncthreads();                                        // sh.part is read
   return true;
