@@ -83,6 +83,9 @@ struct Cursor {
   int first, tok, kv_len, row;                            // of the sequence, see SeqInfo
 };
 
+// 1 / x of a power of two whose inverse is normal.
+HY_DEVICE float pow2_inverse(float x) { return __int_as_float(0x7f000000 - __float_as_int(x)); }
+
 // Maximum over the warp; NaN only if every lane's is.
 HY_DEVICE float warp_max(float x) {
   float r;
@@ -420,7 +423,7 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
         if (smax > __half2float(vcap)) {                  // vs = 2^(6 - exponent), at most 2^15
           const int e = min(max((__float_as_int(smax) >> 23) & 255, 118), 254) - 127;
           const float vs = __int_as_float((6 - e + 127) << 23);
-          vr = __half2float(vcap) < 0.f ? 1.f : vs / __low2float(vs1);
+          vr = __half2float(vcap) < 0.f ? 1.f : vs * pow2_inverse(__low2float(vs1));
           vs1 = __floats2half2_rn(vs, 1.f);
           vcap = __float2half_rn(__int_as_float((e + 127) << 23) * 1.9990234375f);   // the last below 2^(e + 1)
         }
@@ -503,8 +506,8 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
       }
       inv[e] = whole ? 1.f / l[e] : 1.f;
     }
-    const float vs = __low2float(vs1);
-    const float unit0 = 0x1p24f / vs, unit1 = 0x1p20f / vs;       // m-tiles of bits 0-3, 4-7
+    const float per_vs = pow2_inverse(__low2float(vs1));
+    const float unit0 = 0x1p24f * per_vs, unit1 = 0x1p20f * per_vs;   // m-tiles of bits 0-3, 4-7
     if (c < 2) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
@@ -643,7 +646,7 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
     }
     const int seq = pair / a.kv_heads, g = pair - seq * a.kv_heads;
     if (blocks == nb) {
-      const float inv = 1.f / L;
+      const float inv = __fdividef(1.f, L);
       *reinterpret_cast<uint2*>(a.out + ((size_t)tok * a.q_heads + g * HY_GROUP + head) * HY_HEAD_DIM + 4 * lane) =
           make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
     } else {
@@ -743,7 +746,7 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
         o.z = fmaf(w, x.z, o.z);
         o.w = fmaf(w, x.w, o.w);
       }
-      const float inv = 1.f / sum;
+      const float inv = __fdividef(1.f, sum);
       *reinterpret_cast<uint2*>(a.out + ((size_t)p.tok * a.q_heads + g * HY_GROUP + head) * HY_HEAD_DIM + 4 * lane) =
           make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
     }
