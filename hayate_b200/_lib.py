@@ -67,6 +67,8 @@ class HayateError(RuntimeError):
 def load() -> C.CDLL:
     """Load the library once; raise if it is absent (no CPU fallback exists)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -7,7 +7,6 @@ word (bits ``DEV_*``).
 """
 from __future__ import annotations
 
-import contextlib
 from typing import Optional
 
 import torch
@@ -20,21 +19,17 @@ ATTN_EARLY = 1                      # hy_varlen_attention flag HY_ATTN_EARLY
 Q4_TILE_BYTES = 1152                # HY_Q4_TILE_BYTES: one (block, head, K or V) of the 4-bit cache
 DTYPES = {torch.bfloat16: 0, torch.float32: 1}
 
-_HERE = contextlib.nullcontext()
-
 
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+# a device's current stream's handle, without a Stream object around it
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _stream():
-    # the current stream's handle, without building a Stream object around it
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
-
-
-def _on(device: int):
-    """Make ``device`` current for a launch (a no-op context when it already is)."""
-    return _HERE if device == torch.cuda.current_device() else torch.cuda.device(device)
+    return _raw_stream(torch.cuda.current_device())
 
 
 def _i32(t: torch.Tensor, name: str):
@@ -162,19 +157,24 @@ def kv_cache_q4(layers: int, num_blocks: int, kv_heads: int, device="cuda") -> t
                        device=device)
 
 
+# The wrappers of the 4-bit cache: a decode step calls them for microseconds of GPU work, so the
+# checks are few Python steps each, and a call for another device than the current one starts
+# again with that one current.
 def _q4_layer(cache: torch.Tensor, ndim: int):
     """The shape of a 4-bit cache (or one layer of it), checked."""
     shape = cache.shape
-    if cache.dtype != torch.uint8 or len(shape) != ndim or not cache.is_contiguous() or \
+    if cache.dtype is not torch.uint8 or len(shape) != ndim or not cache.is_contiguous() or \
             shape[-2] != 2 or shape[-1] != Q4_TILE_BYTES:
         raise ValueError("the 4-bit cache must be contiguous uint8 "
                          f"{'[layers]' * (ndim - 4)}[blocks][kv_heads][2][{Q4_TILE_BYTES}]")
     return shape
 
 
-def _q4_index(t: torch.Tensor, name: str, device: int):
-    if t.dtype != torch.int32 or device < 0 or t.get_device() != device or not t.is_contiguous():
+def _q4_index(t: torch.Tensor, name: str, device: int) -> int:
+    """The address of an int32 tensor on the cache's device, checked."""
+    if t.dtype is not torch.int32 or device < 0 or t.get_device() != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 CUDA tensor on the cache's device")
+    return t.data_ptr()
 
 
 def kv_append_q4(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
@@ -184,24 +184,25 @@ def kv_append_q4(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
     the other slots of a call are distinct.  The heads of a token are contiguous;
     the tokens may be strided (v as a part of the QKV rows)."""
     NB, heads, _, _ = _q4_layer(kv_cache_layer, 4)
-    dev, want, T = kv_cache_layer.get_device(), k.shape, k.shape[0]
-    if want != (T, heads, 128) or v.shape != want or v.dtype != k.dtype or \
+    dev, want = kv_cache_layer.get_device(), k.shape
+    T = want[0]
+    if want != (T, heads, 128) or v.shape != want or v.dtype is not k.dtype or \
             k.get_device() != dev or v.get_device() != dev:
         raise ValueError(f"k and v must be (tokens, {heads}, 128) of one dtype on the cache's device")
     ks, vs = k.stride(), v.stride()
     if T and (ks[2] != 1 or vs[2] != 1 or (heads > 1 and (ks[1] != 128 or vs[1] != 128))):
         raise ValueError("the heads of a token must be contiguous in k and v")
-    _q4_index(slot_mapping, "slot_mapping", dev)
+    slots = _q4_index(slot_mapping, "slot_mapping", dev)
     if slot_mapping.numel() != T:
         raise ValueError("slot_mapping needs one entry per token")
-    if err is not None:
-        _q4_index(err, "err", dev)
+    word = None if err is None else _q4_index(err, "err", dev)
+    if torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return kv_append_q4(k, v, slot_mapping, kv_cache_layer, err)
     row = heads * 128                       # a single token's stride says nothing
-    with _on(dev):
-        check(_lib.load().hy_kv_append_q4(
-            _dt(k), k.data_ptr(), ks[0] if T > 1 else row, v.data_ptr(), vs[0] if T > 1 else row, T,
-            heads, slot_mapping.data_ptr(), kv_cache_layer.data_ptr(), NB, _ptr(err), _stream()),
-            "hy_kv_append_q4")
+    check(_lib.load().hy_kv_append_q4(
+        _dt(k), k.data_ptr(), ks[0] if T > 1 else row, v.data_ptr(), vs[0] if T > 1 else row, T,
+        heads, slots, kv_cache_layer.data_ptr(), NB, word, _raw_stream(dev)), "hy_kv_append_q4")
 
 
 def kv_read_q4(kv_cache_layer: torch.Tensor, slot_mapping: torch.Tensor, dtype: torch.dtype,
@@ -212,23 +213,24 @@ def kv_read_q4(kv_cache_layer: torch.Tensor, slot_mapping: torch.Tensor, dtype: 
     slot)."""
     NB, heads, _, _ = _q4_layer(kv_cache_layer, 4)
     dev, T = kv_cache_layer.get_device(), slot_mapping.numel()
-    _q4_index(slot_mapping, "slot_mapping", dev)
-    if err is not None:
-        _q4_index(err, "err", dev)
+    slots = _q4_index(slot_mapping, "slot_mapping", dev)
+    word = None if err is None else _q4_index(err, "err", dev)
     want = (T, heads, 128)
-    device = kv_cache_layer.device
-    if k_out is None:
-        k_out = torch.empty(want, dtype=dtype, device=device)
-    if v_out is None:
-        v_out = torch.empty(want, dtype=dtype, device=device)
     for t in (k_out, v_out):
-        if t.shape != want or t.dtype != dtype or t.get_device() != dev or not t.is_contiguous():
+        if t is not None and (t.shape != want or t.dtype is not dtype or t.get_device() != dev or
+                              not t.is_contiguous()):
             raise ValueError(f"outputs must be contiguous (tokens, {heads}, 128) {dtype} tensors "
                              "on the cache's device")
-    with _on(dev):
-        check(_lib.load().hy_kv_read_q4(
-            _dt(k_out), kv_cache_layer.data_ptr(), NB, heads, slot_mapping.data_ptr(), T,
-            k_out.data_ptr(), v_out.data_ptr(), _ptr(err), _stream()), "hy_kv_read_q4")
+    if torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return kv_read_q4(kv_cache_layer, slot_mapping, dtype, k_out, v_out, err)
+    if k_out is None:
+        k_out = kv_cache_layer.new_empty(want, dtype=dtype)
+    if v_out is None:
+        v_out = kv_cache_layer.new_empty(want, dtype=dtype)
+    check(_lib.load().hy_kv_read_q4(
+        _dt(k_out), kv_cache_layer.data_ptr(), NB, heads, slots, T, k_out.data_ptr(),
+        v_out.data_ptr(), word, _raw_stream(dev)), "hy_kv_read_q4")
     return k_out, v_out
 
 
@@ -278,38 +280,38 @@ def varlen_attention_q4(q: torch.Tensor, out: torch.Tensor, kv_cache: torch.Tens
     """``varlen_attention`` over a 4-bit cache (``kv_cache_q4``): the same plan,
     workspace and block tables."""
     L, NB, kv_heads, _, _ = _q4_layer(kv_cache, 5)
-    T, q_heads, D = q.shape
-    dev = kv_cache.get_device()
-    if D != 128 or out.shape != q.shape or out.dtype != q.dtype or not q.is_contiguous() or \
+    shape, dev = q.shape, kv_cache.get_device()
+    T, q_heads, D = shape
+    if D != 128 or out.shape != shape or out.dtype is not q.dtype or not q.is_contiguous() or \
             not out.is_contiguous() or q.get_device() != dev or out.get_device() != dev:
         raise ValueError("q and out must be contiguous (tokens, q_heads, 128) of one dtype on the "
                          "cache's device")
-    _q4_index(block_tables, "block_tables", dev)
-    _q4_index(cu_seqlens_q, "cu_seqlens_q", dev)
-    _q4_index(seq_lens_k, "seq_lens_k", dev)
-    if block_tables.dim() != 2 or (seq_bt_row is None and block_tables.shape[0] < num_seqs):
+    tables = _q4_index(block_tables, "block_tables", dev)
+    cu = _q4_index(cu_seqlens_q, "cu_seqlens_q", dev)
+    lens = _q4_index(seq_lens_k, "seq_lens_k", dev)
+    if block_tables.dim() != 2 or (seq_bt_row is None and len(block_tables) < num_seqs):
         raise ValueError("block_tables must be [rows][pitch] with a row per sequence")
     if cu_seqlens_q.numel() <= num_seqs or seq_lens_k.numel() < num_seqs:
         raise ValueError("cu_seqlens_q or seq_lens_k is too small for num_seqs")
+    row = None
     if seq_bt_row is not None:
-        _q4_index(seq_bt_row, "seq_bt_row", dev)
+        row = _q4_index(seq_bt_row, "seq_bt_row", dev)
         if seq_bt_row.numel() < num_seqs:
             raise ValueError("seq_bt_row is too small for num_seqs")
-    if err is not None:
-        _q4_index(err, "err", dev)
-    if workspace is None:
-        ws_bytes = 0
-    else:
+    word = None if err is None else _q4_index(err, "err", dev)
+    ws, ws_bytes = None, 0
+    if workspace is not None:
         if workspace.get_device() != dev or not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous and on the cache's device")
-        ws_bytes = workspace.numel() * workspace.element_size()
-    scale = 128 ** -0.5 if scale is None else scale
-    with _on(dev):
-        check(_lib.load().hy_varlen_attention_q4(
-            _dt(q), q.data_ptr(), out.data_ptr(), T, q_heads, kv_heads, kv_cache.data_ptr(), L, NB,
-            layer, block_tables.data_ptr(), block_tables.shape[1], _ptr(seq_bt_row),
-            cu_seqlens_q.data_ptr(), seq_lens_k.data_ptr(), num_seqs, scale, max_seqs, max_tokens,
-            _ptr(workspace), ws_bytes, _ptr(err), _stream()), "hy_varlen_attention_q4")
+        ws, ws_bytes = workspace.data_ptr(), workspace.nbytes
+    if torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return varlen_attention_q4(q, out, kv_cache, layer, block_tables, cu_seqlens_q, seq_lens_k,
+                                       num_seqs, max_seqs, max_tokens, workspace, seq_bt_row, scale, err)
+    check(_lib.load().hy_varlen_attention_q4(
+        _dt(q), q.data_ptr(), out.data_ptr(), T, q_heads, kv_heads, kv_cache.data_ptr(), L, NB, layer,
+        tables, block_tables.size(1), row, cu, lens, num_seqs, 128 ** -0.5 if scale is None else scale,
+        max_seqs, max_tokens, ws, ws_bytes, word, _raw_stream(dev)), "hy_varlen_attention_q4")
 
 
 def add_rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float,
