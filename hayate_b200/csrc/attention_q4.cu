@@ -1309,7 +1309,7 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_decode_kernel(Args a, PlanView 
 constexpr int F_WARPS = 8, F_KEYS = 32;
 struct F32Shared {
   float q[HY_GROUP][HY_HEAD_DIM];
-  float p[F_WARPS][F_KEYS][HY_GROUP];                     // weights of a warp's 32 keys
+  float2 p[F_WARPS][F_KEYS][HY_GROUP];                    // weights of a warp's 32 keys, each twice
   float o[F_WARPS][HY_GROUP][HY_HEAD_DIM];
   float2 ml[F_WARPS][HY_GROUP];
 };
@@ -1345,11 +1345,13 @@ __global__ void __launch_bounds__(F_WARPS * 32) attn_q4_fp32_kernel(
     if (tid < HY_GROUP * HY_HEAD_DIM / 4)
       reinterpret_cast<float4*>(sh.q)[tid] = reinterpret_cast<const float4*>(q + at)[tid];
     __syncthreads();
-    float m[HY_GROUP], l[HY_GROUP], acc[HY_GROUP][4];
+    float m[HY_GROUP], l[HY_GROUP];
+    float2 acc[HY_GROUP][2];
 #pragma unroll
     for (int h = 0; h < HY_GROUP; ++h) {
       m[h] = -INFINITY;
-      l[h] = acc[h][0] = acc[h][1] = acc[h][2] = acc[h][3] = 0.f;
+      l[h] = 0.f;
+      acc[h][0] = acc[h][1] = make_float2(0.f, 0.f);
     }
     for (int k0 = warp * F_KEYS; k0 < key_end; k0 += F_WARPS * F_KEYS) {
       const int key = k0 + lane, cnt = min(F_KEYS, key_end - k0);
@@ -1359,27 +1361,34 @@ __global__ void __launch_bounds__(F_WARPS * 32) attn_q4_fp32_kernel(
         blk = 0;
       }
       const uint8_t* tile = cache_layer + q4_tile(blk, g, 0, kv_heads);
-      float s[HY_GROUP] = {0.f, 0.f, 0.f, 0.f};
+      float s[HY_GROUP];
       {
         const uint4* codes = reinterpret_cast<const uint4*>(tile + (key % HY_BLOCK) * Q4_ROW_BYTES);
         const uint2 par = *reinterpret_cast<const uint2*>(tile + Q4_PARAM_OFF + (key % HY_BLOCK) * Q4_PARAM_BYTES);
+        float2 s2[HY_GROUP];                              // sums of even and odd dimensions
+#pragma unroll
+        for (int h = 0; h < HY_GROUP; ++h) s2[h] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint4 w4 = codes[i];
           const float2 sm = __half22float2(q4_as_half2(i < 2 ? par.x : par.y));
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            float x[8];
+            float2 x[4];
             q4_values(w == 0 ? w4.x : w == 1 ? w4.y : w == 2 ? w4.z : w4.w, sm.x, sm.y, x);
 #pragma unroll
             for (int h = 0; h < HY_GROUP; ++h) {
               const float4* qp = reinterpret_cast<const float4*>(&sh.q[h][32 * i + 8 * w]);
               const float4 a = qp[0], b = qp[1];
-              s[h] = fmaf(a.x, x[0], fmaf(a.y, x[1], fmaf(a.z, x[2], fmaf(a.w, x[3], s[h]))));
-              s[h] = fmaf(b.x, x[4], fmaf(b.y, x[5], fmaf(b.z, x[6], fmaf(b.w, x[7], s[h]))));
+              s2[h] = __ffma2_rn(make_float2(a.x, a.y), x[0], s2[h]);
+              s2[h] = __ffma2_rn(make_float2(a.z, a.w), x[1], s2[h]);
+              s2[h] = __ffma2_rn(make_float2(b.x, b.y), x[2], s2[h]);
+              s2[h] = __ffma2_rn(make_float2(b.z, b.w), x[3], s2[h]);
             }
           }
         }
+#pragma unroll
+        for (int h = 0; h < HY_GROUP; ++h) s[h] = s2[h].x + s2[h].y;
       }
       float p[HY_GROUP];
 #pragma unroll
@@ -1394,29 +1403,36 @@ __global__ void __launch_bounds__(F_WARPS * 32) attn_q4_fp32_kernel(
         m[h] = m_new;
         l[h] = fmaf(l[h], alpha, p[h]);                   // this lane's part of the sum
 #pragma unroll
-        for (int d = 0; d < 4; ++d) acc[h][d] *= alpha;
+        for (int d = 0; d < 2; ++d) acc[h][d] = __fmul2_rn(acc[h][d], make_float2(alpha, alpha));
       }
-      *reinterpret_cast<float4*>(sh.p[warp][lane]) = make_float4(p[0], p[1], p[2], p[3]);
+      float4* pw = reinterpret_cast<float4*>(sh.p[warp][lane]);
+      pw[0] = make_float4(p[0], p[0], p[1], p[1]);
+      pw[1] = make_float4(p[2], p[2], p[3], p[3]);
       __syncwarp();
       // this lane's 4 dimensions (4 lane ..) of each key's value: half a code word
-      const uint32_t v_off = Q4_TILE_BYTES + 4 * (lane >> 1), p_off = Q4_TILE_BYTES + Q4_PARAM_OFF + 4 * (lane >> 4);
       const int sh8 = 8 * (lane & 1);
+      for (int half = 0; half < 2; ++half) {              // a block of 16 keys each
+        const int b = __shfl_sync(0xffffffffu, blk, 16 * half), n = min(HY_BLOCK, cnt - 16 * half);
+        const uint8_t* vt = cache_layer + q4_tile(b, g, 1, kv_heads);
+        const uint8_t* w_at = vt + 4 * (lane >> 1);
+        const uint8_t* p_at = vt + Q4_PARAM_OFF + 4 * (lane >> 4);
 #pragma unroll 8
-      for (int j = 0; j < cnt; ++j) {
-        const int b = __shfl_sync(0xffffffffu, blk, j), off = (k0 + j) % HY_BLOCK;
-        const uint8_t* vt = cache_layer + q4_tile(b, g, 0, kv_heads);
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(vt + v_off + off * Q4_ROW_BYTES) >> sh8;
-        const float2 sm = __half22float2(
-            *reinterpret_cast<const __half2*>(vt + p_off + off * Q4_PARAM_BYTES));
-        // nibbles j, j + 1 and, 16 bits up, their partners
-        const float x[4] = {fmaf(q4_nibble(w, 0), sm.x, sm.y), fmaf(q4_nibble(w, 16), sm.x, sm.y),
-                            fmaf(q4_nibble(w, 4), sm.x, sm.y), fmaf(q4_nibble(w, 20), sm.x, sm.y)};
-        const float4 pj = *reinterpret_cast<const float4*>(sh.p[warp][j]);
-        const float ph[HY_GROUP] = {pj.x, pj.y, pj.z, pj.w};
+        for (int j = 0; j < n; ++j) {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(w_at + j * Q4_ROW_BYTES) >> sh8;
+          const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(p_at + j * Q4_PARAM_BYTES));
+          const float2 scale2 = make_float2(sm.x, sm.x), low2 = make_float2(sm.y, sm.y);
+          // nibbles j, j + 1 and, 16 bits up, their partners
+          const float2 x0 = __ffma2_rn(q4_nibbles(w, 0), scale2, low2), x1 = __ffma2_rn(q4_nibbles(w, 4), scale2, low2);
+          const float4* pj = reinterpret_cast<const float4*>(sh.p[warp][16 * half + j]);
+          const float4 pa = pj[0], pb = pj[1];
+          const float2 ph[HY_GROUP] = {make_float2(pa.x, pa.y), make_float2(pa.z, pa.w), make_float2(pb.x, pb.y),
+                                       make_float2(pb.z, pb.w)};
 #pragma unroll
-        for (int h = 0; h < HY_GROUP; ++h)
-#pragma unroll
-          for (int d = 0; d < 4; ++d) acc[h][d] = fmaf(ph[h], x[d], acc[h][d]);
+          for (int h = 0; h < HY_GROUP; ++h) {
+            acc[h][0] = __ffma2_rn(ph[h], x0, acc[h][0]);
+            acc[h][1] = __ffma2_rn(ph[h], x1, acc[h][1]);
+          }
+        }
       }
       __syncwarp();
     }
@@ -1425,7 +1441,7 @@ __global__ void __launch_bounds__(F_WARPS * 32) attn_q4_fp32_kernel(
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
       if (lane == 0) sh.ml[warp][h] = make_float2(m[h], l[h]);
-      *reinterpret_cast<float4*>(&sh.o[warp][h][4 * lane]) = make_float4(acc[h][0], acc[h][1], acc[h][2], acc[h][3]);
+      *reinterpret_cast<float4*>(&sh.o[warp][h][4 * lane]) = make_float4(acc[h][0].x, acc[h][0].y, acc[h][1].x, acc[h][1].y);
     }
     __syncthreads();
     for (int i = tid; i < HY_GROUP * HY_HEAD_DIM; i += F_WARPS * 32) {

@@ -36,21 +36,21 @@ HY_DEVICE size_t q4_tile(int blk, int head, int kv, int kv_heads) {
 HY_DEVICE __half2 q4_as_half2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 HY_DEVICE uint32_t q4_as_u32(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 
-// The nibble at bit `at` (0, 4, 8, 12, 16, 20, 24 or 28) of w as a float: under the
-// exponent of 2^23 it is 2^23 + n, exactly (a conversion instruction runs at a quarter
-// of the rate of the two that this takes).
-HY_DEVICE float q4_nibble(uint32_t w, int at) {
-  return __uint_as_float(((w >> at) & 15u) | 0x4b000000u) - 8388608.0f;
+// The nibbles at bits `at` (0, 4, 8 or 12) and 16 + at of w, two neighbouring dimensions,
+// as floats: under the exponent of 2^23 a nibble n is 2^23 + n, exactly (a conversion
+// instruction runs at a quarter of the rate).
+HY_DEVICE float2 q4_nibbles(uint32_t w, int at) {
+  return __fadd2_rn(make_float2(__uint_as_float(((w >> at) & 15u) | 0x4b000000u),
+                                __uint_as_float(((w >> (16 + at)) & 15u) | 0x4b000000u)),
+                    make_float2(-8388608.0f, -8388608.0f));
 }
 
 // The 8 values (dimensions 8i..8i+7, in order) of word i in fp32.  scale * code is
 // exact (11 + 4 bits), so the sum is the only rounding.
-HY_DEVICE void q4_values(uint32_t w, float scale, float low, float (&x)[8]) {
+HY_DEVICE void q4_values(uint32_t w, float scale, float low, float2 (&x)[4]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    x[2 * j] = fmaf(q4_nibble(w, 4 * j), scale, low);
-    x[2 * j + 1] = fmaf(q4_nibble(w, 16 + 4 * j), scale, low);
-  }
+  for (int j = 0; j < 4; ++j)
+    x[j] = __ffma2_rn(q4_nibbles(w, 4 * j), make_float2(scale, scale), make_float2(low, low));
 }
 
 // The values of a word's nibbles as fp16 pairs: x[j] = (nibble j, nibble 4 + j),
