@@ -6,14 +6,21 @@
 // masks of hayate/model/qwen.py:66-106); here a key or value is what its codes
 // stand for, scale * code + minimum.
 //
-// bf16 runs on the tensor cores.  Decode sequences (one query token): the key blocks of all
-// (sequence, head) pairs, one after the other, are dealt evenly over every warp of the
-// grid; a warp streams its blocks (2304 bytes: K and V of one block and head are adjacent)
-// through a ring of bulk copies and feeds their codes to mma.sync as they are; warps of a
-// CTA merge what they share in shared memory, CTAs through the workspace.
-// Prefill items (64 query tokens x one KV head, 256 score rows) run on tcgen05: four
-// warps expand key tiles to fp16 operands in shared memory, one warp per 128-row
-// sub-tile issues the products, two warpgroups run the softmax.
+// bf16 runs on the tensor cores, in two kernels.  The decode kernel takes steps of one
+// query token per sequence: the key blocks of all (sequence, head) pairs, one after the
+// other, are dealt evenly over every warp of the grid; a warp streams its blocks (2304
+// bytes: K and V of one block and head are adjacent) through a ring of bulk copies and
+// feeds their codes to mma.sync as they are (4 query heads would fill 3 % of a tcgen05
+// tile); warps of a CTA merge what they share in shared memory, CTAs through the
+// workspace.  Bound by the cache's bytes: 256 sequences of 4096 keys take 217 us, 5.6
+// TB/s (of 6.5 for a copy); a launch costs about 9 us beside its blocks, of which the
+// smallest steps consist (one sequence of 600 keys 9.1 us; of 40960 keys 20.8).
+// The other kernel adds prefill items (64 query tokens x one KV head, 256 score rows) on
+// tcgen05: four warps expand key tiles to fp16 operands in shared memory, one warp per
+// 128-row sub-tile issues the products, two warpgroups run the softmax.  Bound by the
+// softmax and the products taking turns in a sub-tile (two sub-tiles overlap): 16 chunks
+// of 512 tokens with 4096 keys take 540 us, 954 TFLOP/s (59 % of a large bf16 product).
+// Key tiles of 128, with one S buffer per sub-tile, ran the same in 793 us.
 // fp32 runs a kernel of its own on the fp32 units.
 #include "attention.cuh"
 #include "attention_pieces.cuh"
@@ -37,10 +44,10 @@ constexpr int DEC_SMEM = NW * (RING_BYTES + 2 * PART_FLOATS * 4) + 1024;   // + 
 constexpr float RESCALE_LOG2 = 8.0f;                      // see decode_warp
 
 // Prefill: warps 0-3 / 4-7 softmax of sub-tile 0 / 1, 8-11 expand, 12 / 13 issue the
-// products of sub-tile 0 / 1, 14 deals out items and loads Q.  Sub-tile X, row r: query head 4 g + 2 X + r / 64, token
-// t0 + r % 64.  Q is [column half][128 rows][64] per sub-tile, a K or V ring slot [column
-// half][64 keys][64], rows of 128 bytes with the 128-byte swizzle: the K-major operand
-// of S = Q K^T and the MN-major operand of P V.
+// products of sub-tile 0 / 1, 14 deals out items and loads Q.  Sub-tile X, row r: query
+// head 4 g + 2 X + r / 64, token t0 + r % 64.  Q is [column half][128 rows][64] per
+// sub-tile, a K or V ring slot [column half][64 keys][64], rows of 128 bytes with the
+// 128-byte swizzle: the K-major operand of S = Q K^T and the MN-major operand of P V.
 constexpr int EXP_WARP = 8, MMA_WARP = 12, ITEM_WARP = 14;
 constexpr int ITEM_READERS = 14;                          // the warps before ITEM_WARP
 constexpr int PS = 4;                                     // K and V ring slots
@@ -121,7 +128,8 @@ struct Shared {
   uint64_t qfree;         // both sub-tiles' last S is done (one commit each)
   uint64_t itemfull;      // item[n % 2] is the CTA's item n
   uint64_t itemfree;      // every warp has read it (one arrival each)
-  uint64_t expdone;       // the item's last tile is about to be expanded (one arrival per expanding warp)
+  uint64_t expdone;       // the item's last tile is about to be expanded (one arrival per
+                          // expanding warp)
   PreItem item[2];
   int nan_at[2][2];       // [item n % 2][half]: the first key whose value is NaN there
   uint32_t tmem_base;
@@ -212,8 +220,8 @@ HY_DEVICE void cursor_next_pair(const Args& a, const PlanView& v, Cursor& k) {
   cursor_sequence(a, k, seq_info(a, v, k.seq));
 }
 
-// One warp: n_blocks key blocks of the flattened list from cur[0] (= cur[1]) on, pair by pair, two blocks
-// (32 keys) at a time.
+// One warp: n_blocks key blocks of the flattened list from cur[0] (= cur[1]) on, pair by
+// pair, two blocks (32 keys) at a time.
 //
 // Scores are computed transposed, S^T = K Q^T (16 keys x 8 columns, 4 of them heads),
 // and so is the output, O^T = V^T P^T: the codes then fill the 16-row operand of
@@ -537,7 +545,7 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
           *reinterpret_cast<float2*>(part + slot * PART_FLOATS + HY_GROUP * HY_HEAD_DIM + 2 * (2 * c + e)) =
               make_float2(m[e], l[e]);
     }
-    if (!whole && lane == 0) 
+    if (!whole && lane == 0)
       parts[slot] = Part{k.seq * a.kv_heads + k.g, n, k.nb, k.first * a.kv_heads + k.g * k.nb, k.tok};
     first_pair = false;
     if (left > 0) {
@@ -562,12 +570,6 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
   return ok;
 }
 
-// The CTA runs key blocks [f0, f1) of the flattened list: its warps take equal parts,
-// then thread t merges head t / 128, dimension t % 128 of every pair that a warp did not
-// finish alone.  A pair that reaches out of the range (its first or last) leaves one
-// partial in the workspace (slot 2 unit, or 2 unit + 1 where the pair starts inside the
-// range), and the CTA whose count of blocks completes a pair joins its partials.
-// Returns false if a wait ran out.
 struct Units {            // `total` blocks in n units whose sizes differ by at most one
   int n, size, more;      // the first `more` units have size + 1 blocks
   HY_DEVICE Units(int total, int units) : n(units), size(total / units), more(total - size * units) {}
@@ -577,6 +579,11 @@ struct Units {            // `total` blocks in n units whose sizes differ by at 
   }
 };
 
+// The CTA runs the key blocks of one unit: its warps take equal parts, then merge, a head
+// each, every pair that no warp finished alone.  A pair that reaches out of the unit (its
+// first or last) leaves one partial in the workspace (slot 2 unit, or 2 unit + 1 where the
+// pair starts inside the unit), and the CTA whose count of blocks completes a pair joins
+// its partials, in their order whoever comes last.  Returns false if a wait ran out.
 // alone: the unit is the n blocks of one pair, k; else blocks f0 .. f0 + n - 1.
 HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units, int unit, bool alone,
                            Cursor k, int f0, int n, const SeqInfo& top, uint8_t* payload, Shared& sh,
@@ -1148,9 +1155,9 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
 }
 
 // The decode sequences of a step with prefill items: their key blocks in even shares, one
-// per CTA, that CTAs take as they become free (a share costs about 10 us beside its
-// blocks: 4 chunks and 128 decodes take 147 us with a share per CTA, 159 with two smaller
-// ones and 169 with three).  Returns false if a wait ran out.
+// per CTA, that CTAs take as they become free (a share costs about 8 us beside its
+// blocks: 4 chunks and 128 decodes take 135 us with a share per CTA, 145 with two smaller
+// ones and 154 with three).  Returns false if a wait ran out.
 __device__ bool decode_shares(const Args& a, const PlanView& v, int n_pre, int blocks, uint8_t* payload,
                               Shared& sh) {
   uint32_t ring_pos = 0, ring_par = 0;
@@ -1302,8 +1309,9 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_decode_kernel(Args a, PlanView 
 
 // ------------------------------------------------------------------ fp32 path
 // fp32 throughout, for the parity engine.  A CTA takes one (query token, KV head): its
-// four query heads share every key and value read.  The warps take 32 keys at a time in
-// turn: one key per lane for the scores (the whole 128-long product in a lane, no exchange
+// four query heads share every key and value read (188 rows of 2 KV heads with 60 to 700
+// keys: 17 us, bound by the instructions per value; a pair of dimensions shares most).  The
+// warps take 32 keys at a time in turn: one key per lane for the scores (the whole 128-long product in a lane, no exchange
 // between lanes), four dimensions per lane for the values; each keeps a running maximum
 // and sum, merged at the end.
 constexpr int F_WARPS = 8, F_KEYS = 32;

@@ -6,7 +6,9 @@
 // cache do (hayate/model/attention.py:52-54 keeps the cache in the model dtype; the
 // reference has no quantised one).
 //
-// Bound by memory (a bf16 row moves 256 + 72 bytes) as long as the instructions per
+// Bound by memory (a bf16 row moves 256 + 72 bytes: 8192 tokens of 8 heads are written in
+// 11.8 us, 3.6 TB/s, and 40001 tokens read back in 48.6 us, 4.3 TB/s, where filling the
+// outputs alone takes 45.8) as long as the instructions per
 // element stay few: the codes are rounded and collected by additions instead of
 // conversions (which run at a quarter of the rate), read back by masks, and a thread's
 // row of the token is found once, not per row.
@@ -17,7 +19,9 @@ namespace {
 constexpr int Q4_THREADS = 256;
 constexpr int Q4_LANES = HY_HEAD_DIM / 16;            // lanes per row
 constexpr int Q4_ROWS = Q4_THREADS / Q4_LANES;        // rows per CTA pass
-constexpr int Q4_UNROLL = 2;                          // rows in flight per lane
+// rows in flight per lane (8192 tokens of 8 heads written / read: 12.7 / 12.5 us with 1,
+// 11.8 / 10.8 with 2, 13.8 / 12.0 with 4)
+constexpr int Q4_UNROLL = 2;
 
 // min and max that are NaN if either operand is
 HY_DEVICE float min_nan(float a, float b) {
