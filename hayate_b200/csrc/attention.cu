@@ -228,6 +228,35 @@ HY_DEVICE int mul_div(int a, int b, int c) {
   return p <= 0x7fffffffLL ? (int)((unsigned)p / (unsigned)c) : (int)(p / c);
 }
 
+// The 4-bit cache's kernel, for a step of n prefill items and `blocks` key blocks of
+// decodes (all heads): how many CTAs take prefill items, and the shares of decode work.
+// As a rule every CTA begins with items while there are any, and the decode work, in a
+// share per CTA, fills up what they leave.  With fewer items than CTAs the two sides may
+// be kept apart instead: an item is long (its tiles, 1.3 us each), so the CTAs that the
+// longer side leaves, a share each, should get through the decode work in the time of k
+// whole rounds of items.  Of the rule and k = 1 to 4 the least estimate is taken (8 heads,
+// 512 tokens at 2560 keys beside 128 decodes of 2048: 108 us, 126 by the rule; at 4096
+// beside 256 of 4096: 273, 307; at 512 beside 10 of 600: 20.1, 24.7; steps of more items
+// than CTAs were no faster apart: 4 chunks at 2560 beside 128 of 2048 168, 170).
+constexpr int TILE_BLOCKS = 28;                 // key blocks that a CTA gets through in a tile's time
+constexpr int SHARE_BLOCKS = 180;               // and in the time that a share costs by itself
+HY_DEVICE void plan_sides(int n, long tiles, long blocks, int ctas, int& pre_ctas, int& shares) {
+  pre_ctas = min(n, ctas);
+  shares = ctas;
+  if (n == 0 || n >= ctas || blocks == 0) return;
+  const float pre = (float)tiles * TILE_BLOCKS, dec = (float)blocks;
+  float best = (pre + dec + dec / 2) / ctas + 1.5f * SHARE_BLOCKS;
+  for (int k = 1; k <= 4; ++k) {
+    const int p = (n + k - 1) / k;
+    const float t = fmaxf(k * pre / n, dec / (ctas - p) + SHARE_BLOCKS);
+    if (t < best) {
+      best = t;
+      pre_ctas = p;
+      shares = ctas - p;
+    }
+  }
+}
+
 __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ seq_lens_k, int S,
     int kv_heads, int warp_slots, int block_cap, PlanView v, int32_t* err) {
@@ -439,6 +468,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
     v.header[3] = s_bad;
     v.header[4] = group && !bad ? S * kv_heads : 0;   // per-CTA decode: its pair count
     v.header[5] = bad ? 0 : s_cblk;
+    plan_sides(bad ? 0 : min(s_cpre, v.max_pre), tiles_all, (long)s_cblk * kv_heads, n_sm, v.header[6],
+               v.header[7]);
     if (S <= v.max_seqs) v.dec_blocks[S] = s_cblk;
     if (bad) hy_flag(err, s_bad);
   }

@@ -37,7 +37,8 @@ struct PlanDims {
 struct PlanView {
   int* header;        // n_pre, n_dec, split, status, (sequence, KV head) pairs of a
                       // per-CTA decode step (0: decode items split over all warps),
-                      // key blocks of all decode sequences
+                      // key blocks of all decode sequences; of the 4-bit cache's kernel:
+                      // CTAs that take prefill items, shares of the decode work
   int4* pre;          // prefill items by sequence (plan scratch)
   int4* pre_sorted;   // the same items, most key tiles first (what the kernel runs)
   int4* dec;          // per decode item: (seq, kv head, first block, end block), then

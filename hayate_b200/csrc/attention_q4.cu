@@ -1154,16 +1154,16 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
   return !__syncthreads_or(!ok);
 }
 
-// The decode sequences of a step with prefill items: their key blocks in even shares, one
-// per CTA, that CTAs take as they become free (a share costs about 8 us beside its
-// blocks: 4 chunks and 128 decodes take 135 us with a share per CTA, 145 with two smaller
-// ones and 154 with three).  Returns false if a wait ran out.
-__device__ bool decode_shares(const Args& a, const PlanView& v, int n_pre, int blocks, uint8_t* payload,
+// The decode sequences of a step with prefill items: their key blocks in even shares that
+// CTAs take as they become free (as many as plan_sides says; a share costs about 8 us
+// beside its blocks: 4 chunks and 128 decodes take 135 us with a share per CTA, 145 with
+// two smaller ones and 154 with three).  Returns false if a wait ran out.
+__device__ bool decode_shares(const Args& a, const PlanView& v, int shares, int blocks, uint8_t* payload,
                               Shared& sh) {
   uint32_t ring_pos = 0, ring_par = 0;
   const int total = blocks * a.kv_heads;                  // below 2^31: the host checks the tables' size
   if (total == 0) return true;
-  const Units units(total, (int)gridDim.x);
+  const Units units(total, shares);
   int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
   for (;;) {
     if (threadIdx.x == 0) sh.unit = atomicAdd(&grab[0], 1);
@@ -1225,9 +1225,10 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(const __grid_constant__ 
   const uint64_t keep = l2_keep_policy();
   const int n_pre = ld_keep(v.header, keep);
   const int blocks = ld_keep(v.header + 5, keep);         // key blocks of the decode sequences
+  const int pre_ctas = ld_keep(v.header + 6, keep), shares = ld_keep(v.header + 7, keep);
   int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
   bool ok = true;
-  if ((int)blockIdx.x < n_pre) {                          // the first n_pre CTAs take prefill items
+  if ((int)blockIdx.x < pre_ctas) {                       // these CTAs take prefill items
     if (warp == 0) {
       tmem_alloc(&sh.tmem_base, TMEM_COLS);
       tmem_relinquish();
@@ -1244,7 +1245,7 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(const __grid_constant__ 
       tmem_dealloc(tmem, TMEM_COLS);
     }
   }
-  if (ok) decode_shares(a, v, n_pre, blocks, payload, sh);
+  if (ok) decode_shares(a, v, shares, blocks, payload, sh);
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();                                      // the last CTA out resets the counters

@@ -108,6 +108,35 @@ def test_attention_offsets_past_32_bits(lens, dt):
     s.check()
 
 
+def test_padding_rows_behind_a_decode_step():
+    """More rows than sequences, though every sequence decodes one token."""
+    b = Batch([1, 1, 0, 1, 1], [5003, 37, 8, 1, 640], 2, BF, seed=25, pad_rows=9)
+    s = Step(b)
+    s.plan()
+    for layer in (0, 1, 0):
+        s.out.fill_(7.0)
+        s.attend(layer)
+        b.layer = layer
+        s.check()
+        assert (s.out[b.T:] == 7.0).all()
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", [
+    ([512, 300] + [1] * 60, [2500, 900] + [100 + 61 * i for i in range(60)]),    # both kinds of work on most CTAs
+    ([64] + [1] * 40, [64] + [4000 - 90 * i for i in range(40)]), ([512] * 4 + [1], [3000] * 4 + [50])])
+def test_prefill_beside_decodes(q_lens, kv_lens):
+    b = Batch(q_lens, kv_lens, 8, BF, layers=2, layer=0, seed=26)
+    s = Step(b)
+    s.plan()
+    first = None
+    for _ in range(6):
+        s.out.fill_(7.0)
+        s.attend()
+        first = s.out.clone() if first is None else first
+        assert torch.equal(s.out, first)
+    s.check()
+
+
 def test_capacities_above_the_batch():
     b = Batch([1, 40, 1], [300, 90, 17], 2, BF, seed=22, pad_rows=3)
     s = Step(b, max_seqs=200, max_tokens=4000)
