@@ -108,10 +108,17 @@ struct Part {
   int tok;                // query row
 };
 
+// Where the partials of an open pair are: units u0 .. u1, u0's in its second slot if the
+// pair starts inside it; and the pair's first row of the output.
+struct Join {
+  int u0, u1, inside, row;
+};
+
 struct Shared {
   uint64_t bar[NW][NS];
   int unit;               // the CTA's next unit of decode work
   int last;               // bit j: this CTA finished pair j of its two open ones
+  Join join[2];
   Part part[2 * NW];      // each warp's two parts, in block order
   Cursor cur[NW][2];      // each warp's pair computed, and next block to load
   // prefill; ring barriers complete once per use of their slot, sfull, pfull and odone
@@ -606,27 +613,26 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
   // empty ones between them).  Warps 4 i + h, i = 0..3, take head h of every fourth pair.
   static_assert(2 * NW == 32 && NW == 4 * HY_GROUP, "one part per lane, four warps per head");
   const int head = warp & 3;
-  const Part mine = sh.part[lane];
-  const float2 ml = mine.pair < 0 ? make_float2(-INFINITY, 0.f)
+  const int my_pair = sh.part[lane].pair, my_blocks = sh.part[lane].blocks;
+  const float2 ml = my_pair < 0 ? make_float2(-INFINITY, 0.f)
                                   : *reinterpret_cast<const float2*>(
                                         parts + lane * PART_FLOATS + HY_GROUP * HY_HEAD_DIM + 2 * head);
-  unsigned todo = __ballot_sync(0xffffffffu, mine.pair >= 0);
+  unsigned todo = __ballot_sync(0xffffffffu, my_pair >= 0);
   int open_at[2], open_blocks[2], n_open = 0;             // pairs that reach out: first part, blocks here
   for (int turn = 0; todo; ++turn) {
     const int i = __ffs(todo) - 1;
-    const int pair = __shfl_sync(0xffffffffu, mine.pair, i);
-    const bool in = mine.pair == pair;
+    const Part& part = sh.part[i];                        // its pair, number of blocks, query row
+    const int pair = part.pair, nb = part.nb;
+    const bool in = my_pair == pair;
     const unsigned group = __ballot_sync(0xffffffffu, in);
     todo &= ~group;
-    const int blocks = __reduce_add_sync(0xffffffffu, in ? mine.blocks : 0);
-    const int nb = __shfl_sync(0xffffffffu, mine.nb, i);
+    const int blocks = __reduce_add_sync(0xffffffffu, in ? my_blocks : 0);
     if (blocks != nb) {
       open_at[n_open & 1] = i;
       open_blocks[n_open & 1] = blocks;
       ++n_open;
     }
     if ((turn & 3) != (warp >> 2)) continue;              // warp-uniform
-    const int tok = __shfl_sync(0xffffffffu, mine.tok, i);
     const float M = warp_max(in ? ml.x : -INFINITY);
     const float wt = in ? ex2_ftz(ml.x - (M == -INFINITY ? 0.f : M)) : 0.f;
     float L = wt * ml.y;
@@ -654,10 +660,10 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
     const int seq = pair / a.kv_heads, g = pair - seq * a.kv_heads;
     if (blocks == nb) {
       const float inv = __fdividef(1.f, L);
-      *reinterpret_cast<uint2*>(a.out + ((size_t)tok * a.q_heads + g * HY_GROUP + head) * HY_HEAD_DIM + 4 * lane) =
+      *reinterpret_cast<uint2*>(a.out + ((size_t)part.tok * a.q_heads + g * HY_GROUP + head) * HY_HEAD_DIM + 4 * lane) =
           make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
     } else {
-      const size_t slot = 2 * unit + (__shfl_sync(0xffffffffu, mine.first, i) > f0);
+      const size_t slot = 2 * unit + (part.first > f0);
       __stcg(reinterpret_cast<float4*>(v.part_o + (slot * HY_GROUP + head) * HY_HEAD_DIM) + lane, acc);
       if (lane == 0) __stcg(v.part_ml + slot * HY_GROUP + head, make_float2(M, L));
     }
@@ -679,6 +685,11 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
     }
     sh.last = (int)__ballot_sync(0xffffffffu, mine_last);
     __threadfence();                                      // the others' partials, after the count
+  } else if (warp == 1 && lane < n_open) {                // meanwhile, should this CTA be the last
+    const Part& p = sh.part[lane == 0 ? open_at[0] : open_at[1]];
+    const int u0 = units.of(p.first);
+    sh.join[lane] = Join{u0, units.of(p.first + p.nb - 1), p.first > units.start(u0),
+                         p.tok * a.q_heads + p.pair % a.kv_heads * HY_GROUP};
   }
   __syncthreads();
   const int last = sh.last;
@@ -686,11 +697,9 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
   for (int j = 0; j < n_open; ++j) {
     if (!((last >> j) & 1)) continue;
     // warps 4 i + h, i = 0..3, take every fourth partial's head h, one float4 per lane
-    const Part p = sh.part[j == 0 ? open_at[0] : open_at[1]];
-    const int g = p.pair % a.kv_heads, quarter = warp >> 2;
-    const int u0 = units.of(p.first), u1 = units.of(p.first + p.nb - 1);
-    const int inside = p.first > units.start(u0);
-    auto slot = [&](int u) { return (size_t)(2 * u + (u == u0 ? inside : 0)); };
+    const Join at = sh.join[j];
+    const int u0 = at.u0, u1 = at.u1, quarter = warp >> 2;
+    auto slot = [&](int u) { return (size_t)(2 * u + (u == u0 ? at.inside : 0)); };
     float M = -INFINITY, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c0 = u0 + quarter; c0 <= u1; c0 += 128) {    // 32 partials (none is empty), one weight per lane
@@ -754,7 +763,7 @@ HY_DEVICE bool decode_unit(const Args& a, const PlanView& v, const Units& units,
         o.w = fmaf(w, x.w, o.w);
       }
       const float inv = __fdividef(1.f, sum);
-      *reinterpret_cast<uint2*>(a.out + ((size_t)p.tok * a.q_heads + g * HY_GROUP + head) * HY_HEAD_DIM + 4 * lane) =
+      *reinterpret_cast<uint2*>(a.out + (size_t)(at.row + head) * HY_HEAD_DIM + 4 * lane) =
           make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
     }
     if (j == 0 && n_open > 1) __syncthreads();            // before the next pair's quarters
@@ -1260,9 +1269,12 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(const __grid_constant__ 
 // Steps of no more query rows than sequences, which are decode steps but for sequences
 // without a token: without the prefill's code a launch takes up to 2 us less (10 sequences
 // of 600 keys 10.0 against 10.3 us, one of 40960 23.3 against 25.3).  The key blocks are dealt
-// evenly over the CTAs; a small step's pairs go one to a CTA, which merges them in shared
-// memory.  Rows of longer chunks that such a step may hold all the same are taken one
-// (row, head) at a time, a CTA each.
+// evenly over the CTAs; a small step's pairs (the plan's choice) go one to a CTA, which
+// merges them in shared memory, unless there are at most 16 of more than 64 blocks each (8
+// pairs of 64 / 96 / 128 blocks dealt 9.6 / 9.9 / 10.3 us, a CTA each 10.0 / 11.7 / 13.6;
+// 16 of 64 / 128 10.6 / 11.5 and 10.0 / 13.5; 32 of 128 14.9 and 13.6).  Rows of longer
+// chunks that such a step may hold all the same are taken one (row, head) at a time, a CTA
+// each.
 __global__ void __launch_bounds__(NT, 1) attn_q4_decode_kernel(Args a, PlanView v) {
   __shared__ Shared sh;
   extern __shared__ uint8_t dyn_smem[];
@@ -1276,8 +1288,10 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_decode_kernel(Args a, PlanView 
   hy_grid_trigger();
   const uint64_t keep = l2_keep_policy();
   const SeqInfo top = seq_top(a, v);                      // with the header: needed by most steps
-  const int n_pre = ld_keep(v.header, keep), n_pairs = ld_keep(v.header + 4, keep);
+  const int n_pre = ld_keep(v.header, keep);
+  int n_pairs = ld_keep(v.header + 4, keep);
   const int total = ld_keep(v.header + 5, keep) * a.kv_heads;   // below 2^31, see decode_shares
+  if (n_pairs <= 16 && total > 64 * n_pairs) n_pairs = 0;       // few, not short: dealt after all
   uint32_t ring_pos = 0, ring_par = 0;
   const Units units(total, (int)gridDim.x);
   const int shares = n_pairs > 0 ? n_pairs : total > 0 ? units.n : 0;
