@@ -14,7 +14,7 @@
 // tile); warps of a CTA merge what they share in shared memory, CTAs through the
 // workspace.  Bound by the cache's bytes: 256 sequences of 4096 keys take 217 us, 5.6
 // TB/s (of 6.5 for a copy); a launch costs about 9 us beside its blocks, of which the
-// smallest steps consist (one sequence of 600 keys 9.1 us; of 40960 keys 20.8).
+// smallest steps consist (one sequence of 600 keys 9.2 us; of 40960 keys 20.3).
 // The other kernel adds prefill items (64 query tokens x one KV head, 256 score rows) on
 // tcgen05: four warps expand key tiles to fp16 operands in shared memory, one warp per
 // 128-row sub-tile issues the products, two warpgroups run the softmax.  Bound by the
