@@ -230,7 +230,7 @@ HY_DEVICE void cursor_next_pair(const Args& a, const PlanView& v, Cursor& k) {
 // One warp: n_blocks key blocks of the flattened list from cur[0] (= cur[1]) on, pair by
 // pair, two blocks (32 keys) at a time.
 //
-// Scores are computed transposed, S^T = K Q^T (16 keys x 8 columns, 4 of them heads),
+// Scores are computed transposed, S^T = K Q^T (16 keys x 8 columns, the 4 heads twice),
 // and so is the output, O^T = V^T P^T: the codes then fill the 16-row operand of
 // mma.sync, where the 4 heads alone would leave three quarters of it empty.  The codes
 // enter the products as they are (q4_bits), and the parameters outside them:
@@ -242,8 +242,9 @@ HY_DEVICE void cursor_next_pair(const Args& a, const PlanView& v, Cursor& k) {
 // p scale_V is kept inside fp16's normal range by a power of two vs: p is at most 2^8
 // (the maximum is only raised when a score exceeds it by more than that, so that most
 // blocks need no exchange between lanes), scale_V vs at most 2^7.
-// Lane (r, c) = (lane / 4, lane % 4) with c < 2 ends with heads 2 c + k (k = 0, 1) at
-// dimensions 8 r + i and 64 + 8 r + i.  ring_pos: the ring's next stage, ring_par the
+// The 8 columns hold the 4 heads twice: the products with V use the second ones for the
+// odd dimensions.  Lane (r, c) = (lane / 4, lane % 4) ends with heads 2 (c % 2) + k (k = 0,
+// 1) at dimensions 8 r + 2 i + c / 2 of either half.  ring_pos: the ring's next stage, ring_par the
 // parity of its next pass.  Returns false if a wait ran out.
 HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], int n_blocks, uint8_t* ring_ptr,
                            float* part, Part* parts, uint64_t* bars,
@@ -255,11 +256,9 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
   uint4 qraw[4];                                          // this lane's part of Q
   auto load_q = [&]() {
     const __nv_bfloat16* qp =
-        a.q + ((size_t)cur[0].tok * a.q_heads + cur[0].g * HY_GROUP + r) * HY_HEAD_DIM + 16 * c;
+        a.q + ((size_t)cur[0].tok * a.q_heads + cur[0].g * HY_GROUP + (r & 3)) * HY_HEAD_DIM + 16 * c;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      qraw[i] = r < HY_GROUP ? *reinterpret_cast<const uint4*>(qp + 64 * (i >> 1) + 8 * (i & 1))
-                             : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < 4; ++i) qraw[i] = *reinterpret_cast<const uint4*>(qp + 64 * (i >> 1) + 8 * (i & 1));
   };
   load_q();
 
@@ -309,6 +308,8 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
   const uint32_t v_off0 = Q4_TILE_BYTES + key_of(c, 0, 0) * Q4_ROW_BYTES + 4 * r;
   const uint32_t v_off1 = Q4_TILE_BYTES + key_of(c, 1, 0) * Q4_ROW_BYTES + 4 * r;
   constexpr uint32_t ROW4 = 4 * Q4_ROW_BYTES, PAR4 = 4 * Q4_PARAM_BYTES;
+  // column r of P^T: its key's weight where the row of the pair is the column's parity
+  const uint32_t sel0 = r < 4 ? 0x4410u : 0x1044u, sel1 = r < 4 ? 0x4432u : 0x3244u;
   uint32_t get = ring_pos, par = ring_par;
   bool ok = true, first_pair = true;
   int pending = 0;
@@ -319,7 +320,7 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
     // those that are full: the pair's last one may not be
     const int full = cur[0].b + n == cur[0].nb && (cur[0].kv_len & (HY_BLOCK - 1)) ? n - 1 : n;
     // Q in fp16 (q4_query_scale): lane (r, c) holds head r's words 2 c, 2 c + 1 (dimensions
-    // 16 c ..) of both halves; rows 4-7 are zero.  Codes in bits 0-3 meet 2^14 q, codes
+    // 16 c ..) of both halves; rows 4-7 repeat rows 0-3.  Codes in bits 0-3 meet 2^14 q, codes
     // in bits 4-7 2^10 q, so that a score comes out as 2^-10 code . q.
     uint32_t qb[2][2][4], qs = 0u;                        // qs: the operand of the sums of q
     float mult[2];                                        // scale to log2 units of heads 2 c + k
@@ -366,7 +367,7 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
       mult[0] = fmaxf(a.scale_log2 * (1024.f * __shfl_sync(0xffffffffu, up, 8 * c)), 1e-30f);
       mult[1] = fmaxf(a.scale_log2 * (1024.f * __shfl_sync(0xffffffffu, up, 8 * c + 4)), 1e-30f);
     }
-    float o[8][4];                                        // O^T, in 2^-24 / vs (odd m-tiles 2^-20 / vs)
+    float o[4][4];                                        // O^T, in 2^-24 / vs (odd m-tiles 2^-20 / vs)
     float z[2][2] = {{0.f, 0.f}, {0.f, 0.f}};             // [half][k]: sum of p times V's minimum
     float m[2] = {-INFINITY, -INFINITY};                  // running maximum (log2 units)
     float thr[2] = {-INFINITY, -INFINITY};                // score at which it is raised
@@ -374,7 +375,7 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
     __half2 vs1 = q4_as_half2(0x3c003c00u);               // (vs, 1)
     __half vcap = __ushort_as_half(0xbc00);               // the largest scale that vs fits: -1, none yet
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    for (int j = 0; j < 4; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
 #pragma unroll 1
     for (int i = 0; i < n; i += 2) {
@@ -455,7 +456,7 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
           z[1][e] *= alpha;
           const float ao = alpha * vr;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) { o[j][e] *= ao; o[j][2 + e] *= ao; }
+          for (int j = 0; j < 4; ++j) { o[j][e] *= ao; o[j][2 + e] *= ao; }
         }
       }
       const float ms[2] = {m[0] == -INFINITY ? 0.f : -m[0], m[1] == -INFINITY ? 0.f : -m[1]};
@@ -466,35 +467,30 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
         l[0] += x[b][0] + x[b][2];
         l[1] += x[b][1] + x[b][3];
         const __half2 pa = __floats2half2_rn(x[b][0], x[b][1]), pc = __floats2half2_rn(x[b][2], x[b][3]);
-        uint32_t pt[2][2];                                // P^T operands [half][keys 0-7, 8-15]
+        // O^T += V^T (scale P)^T, a half of the dimensions and 8 keys at a time.  A register
+        // of V^T is what q4_bits leaves of a key's word: an even and the next odd
+        // dimension, contracted together; the even one's outputs are columns 0-3, whose P
+        // is 0 where the odd one's codes are, the odd one's columns 4-7 the other way
+        // round.  Nibbles of equal weight share an m-tile (rows 0-7 nibble e, rows 8-15
+        // nibble e + 2 of words 0-7).
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           const __half2 ua = q4_as_half2(hf ? va[b].y : va[b].x), uc = q4_as_half2(hf ? vb[b].y : vb[b].x);
-          pt[hf][0] = movmatrix_trans(q4_as_u32(__hmul2(pa, __low2half2(__hmul2(ua, vs1)))));
-          pt[hf][1] = movmatrix_trans(q4_as_u32(__hmul2(pc, __low2half2(__hmul2(uc, vs1)))));
           const float na = __high2float(ua), nc = __high2float(uc);
           z[hf][0] = fmaf(x[b][0], na, fmaf(x[b][2], nc, z[hf][0]));
           z[hf][1] = fmaf(x[b][1], na, fmaf(x[b][3], nc, z[hf][1]));
-        }
-        // O^T += V^T (scale P)^T, a half of the dimensions per product: the lane's word r of
-        // four keys holds dimensions 8 r .. 8 r + 7; nibbles of equal weight share an m-tile
-        // (rows 0-7 nibble j, rows 8-15 nibble j + 2)
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t y[2][2][4];                            // [keys 0-7, 8-15][low, high nibbles]
+          const uint32_t pt[2] = {
+              movmatrix_trans(q4_as_u32(__hmul2(pa, __low2half2(__hmul2(ua, vs1))))),
+              movmatrix_trans(q4_as_u32(__hmul2(pc, __low2half2(__hmul2(uc, vs1)))))};
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t w0 = lds32(v_at0 + b * BLK_BYTES + 32 * hf + ROW4 * h);
-            const uint32_t w1 = lds32(v_at1 + b * BLK_BYTES + 32 * hf + ROW4 * h);
-            q4_bits(__byte_perm(w0, w1, 0x5410), y[h][0]);
-            q4_bits(__byte_perm(w0, w1, 0x7632), y[h][1]);
+            uint32_t y0[4], y1[4];                        // keys of rows 2 c, 2 c + 1 (+ 8 h)
+            q4_bits(lds32(v_at0 + b * BLK_BYTES + 32 * hf + ROW4 * h), y0);
+            q4_bits(lds32(v_at1 + b * BLK_BYTES + 32 * hf + ROW4 * h), y1);
+            const uint32_t p0 = __byte_perm(pt[h], 0u, sel0), p1 = __byte_perm(pt[h], 0u, sel1);
+            mma_f16_16816(o[2 * hf], y0[0], y0[2], y1[0], y1[2], p0, p1);
+            mma_f16_16816(o[2 * hf + 1], y0[1], y0[3], y1[1], y1[3], p0, p1);
           }
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              mma_f16_16816(o[4 * hf + 2 * e + j], y[0][e][j], y[0][e][j + 2], y[1][e][j], y[1][e][j + 2],
-                            pt[hf][0], pt[hf][1]);
         }
       }
       if (++get == NS) {
@@ -523,35 +519,36 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
     }
     const float per_vs = pow2_inverse(__low2float(vs1));
     const float unit0 = 0x1p24f * per_vs, unit1 = 0x1p20f * per_vs;   // m-tiles of bits 0-3, 4-7
-    if (c < 2) {
+    // lanes c < 2 hold the even dimensions of heads 2 c + k, lanes c + 2 the odd ones; the
+    // former take the odd ones of k = 0, the latter the even ones of k = 1
+    const bool odd = c >= 2;
+    const int head = 2 * (c & 1) + odd;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+    for (int hf = 0; hf < 2; ++hf) {
+      float y[8];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          // nibble i (of 8): m-tile 4 hf + 2 (i / 4) + i % 2, row group (i % 4) / 2
-          float y[8];
+      for (int i = 0; i < 4; ++i) {                       // nibble i: m-tile 2 hf + i % 2, row group i / 2
+        float u[2];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float u = o[4 * hf + 2 * (i >> 2) + (i & 1)][2 * ((i & 3) >> 1) + e];
-            y[i < 4 ? 2 * i : 2 * (i - 4) + 1] = fmaf(u, (i & 1) ? unit1 : unit0, z[hf][e]) * inv[e];
-          }
-          const int at = (2 * c + e) * HY_HEAD_DIM + 64 * hf + 8 * r;
-          if (whole) {
-            *reinterpret_cast<uint4*>(a.out + ((size_t)k.tok * a.q_heads + k.g * HY_GROUP) * HY_HEAD_DIM + at) =
-                make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]),
-                           pack_bf16(y[6], y[7]));
-          } else {
-            float4* p4 = reinterpret_cast<float4*>(part + slot * PART_FLOATS + at);
-            p4[0] = make_float4(y[0], y[1], y[2], y[3]);
-            p4[1] = make_float4(y[4], y[5], y[6], y[7]);
-          }
-        }
-      if (!whole && r == 0)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          *reinterpret_cast<float2*>(part + slot * PART_FLOATS + HY_GROUP * HY_HEAD_DIM + 2 * (2 * c + e)) =
-              make_float2(m[e], l[e]);
+        for (int k = 0; k < 2; ++k)
+          u[k] = fmaf(o[2 * hf + (i & 1)][2 * (i >> 1) + k], (i & 1) ? unit1 : unit0, z[hf][k]) * inv[k];
+        const float got = __shfl_xor_sync(0xffffffffu, odd ? u[0] : u[1], 2);
+        y[2 * i] = odd ? got : u[0];
+        y[2 * i + 1] = odd ? u[1] : got;
+      }
+      const int at = head * HY_HEAD_DIM + 64 * hf + 8 * r;
+      if (whole) {
+        *reinterpret_cast<uint4*>(a.out + ((size_t)k.tok * a.q_heads + k.g * HY_GROUP) * HY_HEAD_DIM + at) =
+            make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+      } else {
+        float4* p4 = reinterpret_cast<float4*>(part + slot * PART_FLOATS + at);
+        p4[0] = make_float4(y[0], y[1], y[2], y[3]);
+        p4[1] = make_float4(y[4], y[5], y[6], y[7]);
+      }
     }
+    if (!whole && r == 0)
+      *reinterpret_cast<float2*>(part + slot * PART_FLOATS + HY_GROUP * HY_HEAD_DIM + 2 * head) =
+          make_float2(odd ? m[1] : m[0], odd ? l[1] : l[0]);
     if (!whole && lane == 0)
       parts[slot] = Part{k.seq * a.kv_heads + k.g, n, k.nb, k.first * a.kv_heads + k.g * k.nb, k.tok};
     first_pair = false;
