@@ -12,14 +12,14 @@
 // bytes: K and V of one block and head are adjacent) through a ring of bulk copies and
 // feeds their codes to mma.sync as they are (4 query heads would fill 3 % of a tcgen05
 // tile); warps of a CTA merge what they share in shared memory, CTAs through the
-// workspace.  Bound by the cache's bytes: 256 sequences of 4096 keys take 217 us, 5.6
+// workspace.  Bound by the cache's bytes: 256 sequences of 4096 keys take 216 us, 5.6
 // TB/s (of 6.5 for a copy); a launch costs about 9 us beside its blocks, of which the
-// smallest steps consist (one sequence of 600 keys 9.2 us; of 40960 keys 20.3).
+// smallest steps consist (one sequence of 600 keys 8.8 us; of 40960 keys 19.8).
 // The other kernel adds prefill items (64 query tokens x one KV head, 256 score rows) on
 // tcgen05: four warps expand key tiles to fp16 operands in shared memory, one warp per
 // 128-row sub-tile issues the products, two warpgroups run the softmax.  Bound by the
 // softmax and the products taking turns in a sub-tile (two sub-tiles overlap): 16 chunks
-// of 512 tokens with 4096 keys take 540 us, 954 TFLOP/s (59 % of a large bf16 product).
+// of 512 tokens with 4096 keys take 523 us, 985 TFLOP/s (61 % of a large bf16 product).
 // Key tiles of 128, with one S buffer per sub-tile, ran the same in 793 us.
 // fp32 runs a kernel of its own on the fp32 units.
 #include "attention.cuh"
