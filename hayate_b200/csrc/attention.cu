@@ -1172,9 +1172,12 @@ __device__ bool prefill_item_tc(const CUtensorMap* kgroups, const CUtensorMap* t
       if (!ok) break;
       tc_fence_after();
       float s[64];
-      tmem_ld32(tS, *reinterpret_cast<float(*)[32]>(&s[0]));
-      tmem_ld32(tS + 32, *reinterpret_cast<float(*)[32]>(&s[32]));
-      tmem_wait_ld();
+      float (&s_lo)[32] = *reinterpret_cast<float(*)[32]>(&s[0]);
+      float (&s_hi)[32] = *reinterpret_cast<float(*)[32]>(&s[32]);
+      tmem_ld32(tS, s_lo);
+      tmem_ld32(tS + 32, s_hi);
+      tmem_wait_ld(s_lo);
+      tmem_wait_ld(s_hi);
       const int kb = (tlo + t) * TC_KEYS;
       if (kb + TC_KEYS - 1 > prefix + t0) {     // the tile reaches the diagonal or the end
 #pragma unroll
@@ -1210,7 +1213,7 @@ __device__ bool prefill_item_tc(const CUtensorMap* kgroups, const CUtensorMap* t
           for (int cc = 0; cc < 4; ++cc) {
             float o[32];
             tmem_ld32(tO + 32 * cc, o);
-            tmem_wait_ld();
+            tmem_wait_ld(o);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const float2 r2 = __fmul2_rn(make_float2(o[2 * i], o[2 * i + 1]), make_float2(alpha, alpha));
@@ -1265,7 +1268,7 @@ __device__ bool prefill_item_tc(const CUtensorMap* kgroups, const CUtensorMap* t
       for (int cc = 0; cc < 4; ++cc) {
         float o[32];
         tmem_ld32(tO + 32 * cc, o);
-        tmem_wait_ld();
+        tmem_wait_ld(o);
         if (store) {
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {

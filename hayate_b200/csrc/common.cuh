@@ -482,8 +482,9 @@ HY_DEVICE void tmem_st16(uint32_t taddr, const float (&v)[16]) {
       : "memory");
 }
 
-HY_DEVICE void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// The same, naming the 32 values it waits for: no use of them can be scheduled before it.
+// Wait for this thread's TMEM loads.  It names the 32 values it waits for, so that no use
+// of them can be scheduled before it: a "memory" clobber does not order arithmetic on
+// registers.  Two loads in flight take one wait each.
 HY_DEVICE void tmem_wait_ld(float (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
       : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]),

@@ -345,9 +345,12 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lm_head_argmax_kernel(
 #pragma unroll 1
         for (int c0 = 0; c0 < LM_N; c0 += 64) {   // columns past 208 of the last pair unused
           float v[64];
-          tmem_ld32(tb + c0, *reinterpret_cast<float(*)[32]>(&v[0]));
-          tmem_ld32(tb + c0 + 32, *reinterpret_cast<float(*)[32]>(&v[32]));
-          tmem_wait_ld();
+          float (&v_lo)[32] = *reinterpret_cast<float(*)[32]>(&v[0]);
+          float (&v_hi)[32] = *reinterpret_cast<float(*)[32]>(&v[32]);
+          tmem_ld32(tb + c0, v_lo);
+          tmem_ld32(tb + c0 + 32, v_hi);
+          tmem_wait_ld(v_lo);
+          tmem_wait_ld(v_hi);
 #pragma unroll
           for (int i = 0; i < 64; i += 2) {
             const __nv_bfloat162 h = __floats2bfloat162_rn(v[i], v[i + 1]);
