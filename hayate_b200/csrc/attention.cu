@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
         atomicOr(&s_bad, HY_ERR_PLAN);
       } else if (blockIdx.x == 0) {
         v.seqinfo[i] = make_int2(d0, ns);
-        v.dec_blocks[i] = s_cblk + sums[BLK];
+        v.seqs[i] = make_int4(s_cblk + sums[BLK], s_row[threadIdx.x], s_kv[threadIdx.x], 0);
         for (int g = 0; g < kv_heads; ++g) v.counters[i * kv_heads + g] = 0;
       }
     }
@@ -468,9 +468,15 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
     v.header[3] = s_bad;
     v.header[4] = group && !bad ? S * kv_heads : 0;   // per-CTA decode: its pair count
     v.header[5] = bad ? 0 : s_cblk;
-    plan_sides(bad ? 0 : min(s_cpre, v.max_pre), tiles_all, (long)s_cblk * kv_heads, n_sm, v.header[6],
-               v.header[7]);
-    if (S <= v.max_seqs) v.dec_blocks[S] = s_cblk;
+    HyQ4Plan& p = *reinterpret_cast<HyQ4Plan*>(v.header + 8);
+    p.blocks = v.header[5];
+    p.work = v.header[4] > 0 ? -v.header[4] : v.header[0];
+    p.seqs = S;
+    p.key = v.key;
+    plan_sides(bad ? 0 : min(s_cpre, v.max_pre), tiles_all, (long)s_cblk * kv_heads, n_sm, p.pre_ctas, p.shares);
+    p.first_row = cu_q[0];
+    p.end_row = cu_q[S];
+    if (S <= v.max_seqs) v.seqs[S] = make_int4(s_cblk, cu_q[S], 0, 0);
     if (bad) hy_flag(err, s_bad);
   }
 }
@@ -1541,7 +1547,7 @@ size_t hy_attn_workspace_bytes(const PlanDims& d) {
   off = align256(off + (size_t)d.max_pre_part * PRE_PART_F4 * sizeof(float4));
   off = align256(off + (size_t)d.max_pre_part * 256 * sizeof(float2));
   off = align256(off + (size_t)d.max_pre_part * sizeof(int));
-  off = align256(off + (size_t)(d.max_seqs + 1) * sizeof(int));
+  off = align256(off + (size_t)(d.max_seqs + 1) * sizeof(int4));
   return off;
 }
 
@@ -1575,11 +1581,15 @@ PlanView hy_attn_plan_view(void* ws, const PlanDims& d) {
   off = align256(off + (size_t)d.max_pre_part * 256 * sizeof(float2));
   v.pre_ctr = reinterpret_cast<int*>(p + off);
   off = align256(off + (size_t)d.max_pre_part * sizeof(int));
-  v.dec_blocks = reinterpret_cast<int*>(p + off);
+  v.seqs = reinterpret_cast<int4*>(p + off);
   v.max_pre = d.max_pre;
   v.max_dec = d.max_dec;
   v.max_seqs = d.max_seqs;
   v.max_pre_part = d.max_pre_part;
+  unsigned key = 0x9e3779b9u;
+  for (int x : {d.kv_heads, d.max_seqs, d.max_pre, d.max_dec, d.max_pre_part})
+    key = (key ^ (unsigned)x) * 0x01000193u;
+  v.key = (int)key;
   return v;
 }
 

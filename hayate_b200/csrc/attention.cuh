@@ -37,8 +37,8 @@ struct PlanDims {
 struct PlanView {
   int* header;        // n_pre, n_dec, split, status, (sequence, KV head) pairs of a
                       // per-CTA decode step (0: decode items split over all warps),
-                      // key blocks of all decode sequences; of the 4-bit cache's kernel:
-                      // CTAs that take prefill items, shares of the decode work
+                      // key blocks of all decode sequences; then what the 4-bit cache's
+                      // kernels read, [8]: HyQ4Plan
   int4* pre;          // prefill items by sequence (plan scratch)
   int4* pre_sorted;   // the same items, most key tiles first (what the kernel runs)
   int4* dec;          // per decode item: (seq, kv head, first block, end block), then
@@ -58,13 +58,26 @@ struct PlanView {
   float2* pre_part_ml;// [max_pre_part][256] (running max in log2 units, sum) per row
   int* pre_ctr;       // [max_pre_part] finished pieces, at a split item's first slot
                       // (zeroed by the plan and by the merging piece)
-  int* dec_blocks;    // [max_seqs + 1] key blocks (as hy_dec_block_cap cuts them) of the
-                      // decode sequences before each sequence (the 4-bit cache's kernel
-                      // deals blocks, not items)
+  int4* seqs;         // [max_seqs + 1] per sequence: key blocks (as hy_dec_block_cap cuts
+                      // them) of the decode sequences before it, first query row, key
+                      // length (the 4-bit cache's kernels deal blocks, not items, and take
+                      // the sequences from here)
   int max_pre, max_dec, max_seqs, max_pre_part;
+  int key;            // of the workspace's capacities (the layout above follows from them)
 };
 
-// The most key blocks that dec_blocks counts of one sequence, so that those of all S
+// A plan as the 4-bit cache's kernels take it, two 16-byte loads.
+struct HyQ4Plan {
+  int blocks;         // key blocks of all decode sequences, of one KV head
+  int work;           // >= 0: prefill items; < 0: none, and minus the pairs of a per-CTA
+                      // decode step
+  int seqs, key;      // the batch's sequences and PlanView::key: others are another plan's
+  int pre_ctas;       // CTAs that take prefill items
+  int shares;         // shares of the decode work
+  int first_row, end_row;   // query rows of the sequences
+};
+
+// The most key blocks that PlanView::seqs counts of one sequence, so that those of all S
 // sequences and KV heads stay below 2^31.  hy_varlen_attention_q4 refuses block tables
 // with longer rows: only a sequence longer than its row is cut.
 inline int hy_dec_block_cap(int S, int kv_heads) {
@@ -109,8 +122,7 @@ cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap* q_map, const void* q, void
                                    int q_heads, int kv_heads,
                                    const void* cache_layer, int num_blocks, int layer,
                                    const int32_t* block_tables, int bt_pitch,
-                                   const int32_t* seq_bt_row, const int32_t* cu_q,
-                                   const int32_t* seq_lens_k, int S, float scale,
+                                   const int32_t* seq_bt_row, int S, float scale,
                                    const PlanDims& d, void* ws, int32_t* err, int dev,
                                    cudaStream_t st);
 cudaError_t hy_launch_attn_q4_fp32(const void* q, void* out, int tokens, int q_heads, int kv_heads,

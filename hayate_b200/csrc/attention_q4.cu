@@ -70,8 +70,6 @@ struct Args {
   const int32_t* block_tables;
   int bt_pitch;
   const int32_t* seq_bt_row;
-  const int32_t* cu_q;
-  const int32_t* seq_lens_k;
   float scale_log2;
   int32_t* err;
 };
@@ -164,12 +162,28 @@ HY_DEVICE void q4_bits(uint32_t w, uint32_t (&x)[4]) {
 }
 
 // What a sequence is to the decode: its first block in the list of all sequences' key
-// blocks, query row, key length and block-table row.
+// blocks, query row, key length and block-table row.  All but the last are the plan's, so
+// that they agree with its counts of blocks whatever the caller's arrays hold by now.
 struct SeqInfo {
   int first, tok, kv_len, row;
 };
 HY_DEVICE SeqInfo seq_info(const Args& a, const PlanView& v, int seq) {
-  return SeqInfo{v.dec_blocks[seq], a.cu_q[seq], a.seq_lens_k[seq], a.seq_bt_row ? a.seq_bt_row[seq] : seq};
+  const int4 s = v.seqs[seq];
+  return SeqInfo{s.x, s.y, s.z, a.seq_bt_row ? a.seq_bt_row[seq] : seq};
+}
+// The workspace's plan.  One of other sequences or capacities (or none), or of query rows
+// that q does not have, is reported and holds no work.
+HY_DEVICE HyQ4Plan load_plan(const Args& a, const PlanView& v) {
+  const uint64_t keep = l2_keep_policy();
+  const int4 x = ld_keep(reinterpret_cast<const int4*>(v.header + 8), keep);
+  const int4 y = ld_keep(reinterpret_cast<const int4*>(v.header + 12), keep);
+  const int bad = x.z != a.num_seqs || x.w != v.key ? HY_ERR_PLAN
+                  : y.z < 0 || y.w > a.num_tokens ? HY_ERR_BOUNDS : 0;
+  if (bad) {
+    if (threadIdx.x == 0) hy_flag(a.err, bad);
+    return HyQ4Plan{};
+  }
+  return HyQ4Plan{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 }
 // The search of cursor_at begins with sequences `top_step` apart, one per lane; they are
 // loaded before the kernel knows whether it has decode work.
@@ -223,7 +237,7 @@ HY_DEVICE void cursor_next_pair(const Args& a, const PlanView& v, Cursor& k) {
   k.g = 0;
   do {
     ++k.seq;
-  } while (v.dec_blocks[k.seq + 1] == v.dec_blocks[k.seq]);
+  } while (v.seqs[k.seq + 1].x == v.seqs[k.seq].x);
   cursor_sequence(a, k, seq_info(a, v, k.seq));
 }
 
@@ -777,9 +791,10 @@ HY_DEVICE PreItem pre_item_geom(const Args& a, const PlanView& v, int item) {
   p.g = it.y;
   p.t0 = it.z;
   p.w = it.w;
-  p.row0 = a.cu_q[p.seq];
-  const int q_len = a.cu_q[p.seq + 1] - p.row0;
-  p.prefix = a.seq_lens_k[p.seq] - q_len;
+  const int4 s = v.seqs[p.seq];
+  p.row0 = s.y;
+  const int q_len = v.seqs[p.seq + 1].y - p.row0;
+  p.prefix = s.z - q_len;
   p.nrows = min(PRE_QROWS, q_len - p.t0);
   p.kv_end = p.prefix + p.t0 + p.nrows;                   // keys its last row sees
   pre_piece_range(p.w, (p.kv_end + PRE_KEYS - 1) / PRE_KEYS, p.tlo, p.thi);
@@ -1185,11 +1200,11 @@ __device__ bool decode_shares(const Args& a, const PlanView& v, int shares, int 
 }
 
 // The sequence of query row `tok`: the last that starts at or before it.
-HY_DEVICE int seq_of_row(const Args& a, int tok) {
+HY_DEVICE int seq_of_row(const Args& a, const PlanView& v, int tok) {
   int lo = 0, hi = a.num_seqs;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (a.cu_q[mid] <= tok) lo = mid; else hi = mid;
+    if (v.seqs[mid].y <= tok) lo = mid; else hi = mid;
   }
   return lo;
 }
@@ -1228,13 +1243,11 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(const __grid_constant__ 
   __syncthreads();
   hy_grid_wait();
   hy_grid_trigger();
-  const uint64_t keep = l2_keep_policy();
-  const int n_pre = ld_keep(v.header, keep);
-  const int blocks = ld_keep(v.header + 5, keep);         // key blocks of the decode sequences
-  const int pre_ctas = ld_keep(v.header + 6, keep), shares = ld_keep(v.header + 7, keep);
+  const HyQ4Plan plan = load_plan(a, v);
+  if (plan.work <= 0 && plan.blocks == 0) return;         // every CTA: no counter is touched
   int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
   bool ok = true;
-  if ((int)blockIdx.x < pre_ctas) {                       // these CTAs take prefill items
+  if ((int)blockIdx.x < plan.pre_ctas) {                     // these CTAs take prefill items
     if (warp == 0) {
       tmem_alloc(&sh.tmem_base, TMEM_COLS);
       tmem_relinquish();
@@ -1243,7 +1256,7 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(const __grid_constant__ 
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem_base;
-    ok = prefill_all(&q_map, a, v, n_pre, &grab[2], payload, sh, tmem);
+    ok = prefill_all(&q_map, a, v, plan.work, &grab[2], payload, sh, tmem);
     tc_fence_before();
     __syncthreads();
     if (warp == 0) {
@@ -1251,7 +1264,7 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(const __grid_constant__ 
       tmem_dealloc(tmem, TMEM_COLS);
     }
   }
-  if (ok) decode_shares(a, v, shares, blocks, payload, sh);
+  if (ok) decode_shares(a, v, plan.shares, plan.blocks, payload, sh);
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();                                      // the last CTA out resets the counters
@@ -1283,16 +1296,15 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_decode_kernel(Args a, PlanView 
   __syncthreads();
   hy_grid_wait();
   hy_grid_trigger();
-  const uint64_t keep = l2_keep_policy();
   const SeqInfo top = seq_top(a, v);                      // with the header: needed by most steps
-  const int n_pre = ld_keep(v.header, keep);
-  int n_pairs = ld_keep(v.header + 4, keep);
-  const int total = ld_keep(v.header + 5, keep) * a.kv_heads;   // below 2^31, see decode_shares
+  const HyQ4Plan plan = load_plan(a, v);
+  int n_pairs = max(-plan.work, 0);
+  const int total = plan.blocks * a.kv_heads;             // below 2^31, see decode_shares
   if (n_pairs <= 16 && total > 64 * n_pairs) n_pairs = 0;       // few, not short: dealt after all
   uint32_t ring_pos = 0, ring_par = 0;
   const Units units(total, (int)gridDim.x);
   const int shares = n_pairs > 0 ? n_pairs : total > 0 ? units.n : 0;
-  const long n = shares + (n_pre > 0 ? (long)min(a.num_tokens, a.cu_q[a.num_seqs]) * a.kv_heads : 0);
+  const long n = shares + (plan.work > 0 ? (long)plan.end_row * a.kv_heads : 0);
   for (long u = blockIdx.x; u < n; u += gridDim.x) {
     const bool alone = n_pairs > 0 || u >= shares;
     Cursor k = {};
@@ -1300,16 +1312,16 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_decode_kernel(Args a, PlanView 
     if (alone) {
       const int i = (int)(u < shares ? u : u - shares) / a.kv_heads;
       k.g = (int)(u < shares ? u : u - shares) - i * a.kv_heads;
-      k.seq = u < shares ? i : seq_of_row(a, i);
+      k.seq = u < shares ? i : seq_of_row(a, v, i);
       SeqInfo s = seq_info(a, v, k.seq);
-      const int q_len = a.cu_q[k.seq + 1] - s.tok;
-      bool take = q_len == 1 && seq_fits(q_len, s.kv_len);
+      const int q_len = v.seqs[k.seq + 1].y - s.tok;
+      bool take = q_len == 1;                             // (of a plan that fits)
       if (u >= shares) {                                  // row i, which sees kv_len - (rows after it) keys
-        take = q_len > 1;
+        take = q_len > 1 && i >= s.tok;
         s.kv_len -= s.tok + q_len - 1 - i;
         s.tok = i;
       }
-      cursor_sequence(a, k, s);
+      if (take) cursor_sequence(a, k, s);
       blocks = take ? k.nb : 0;                           // the others are not this unit's
     } else {
       f0 = units.start((int)u);
@@ -1344,7 +1356,11 @@ __global__ void __launch_bounds__(F_WARPS * 32) attn_q4_fp32_kernel(
   hy_grid_wait();
   hy_grid_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const long total = (long)min(tokens, cu_q[S]) * kv_heads;   // rows past the last sequence stay
+  const long total = (long)cu_q[S] * kv_heads;            // rows past the last sequence stay
+  if (cu_q[0] < 0 || cu_q[S] > tokens) {                  // rows that q does not have
+    if (tid == 0) hy_flag(err, HY_ERR_BOUNDS);
+    return;
+  }
   for (long u = blockIdx.x; u < total; u += gridDim.x) {
     const int row = (int)(u / kv_heads), g = (int)(u % kv_heads);
     int lo = 0, hi = S;                     // seq = last i with cu_q[i] <= row
@@ -1353,6 +1369,7 @@ __global__ void __launch_bounds__(F_WARPS * 32) attn_q4_fp32_kernel(
       if (cu_q[mid] <= row) lo = mid; else hi = mid;
     }
     const int seq = lo;
+    if (row < cu_q[seq]) continue;                        // before the first sequence
     const int prefix = seq_lens_k[seq] - (cu_q[seq + 1] - cu_q[seq]);
     const int key_end = prefix + (row - cu_q[seq]) + 1;
     if (prefix < 0 || (long)key_end > (long)bt_pitch * HY_BLOCK) {
@@ -1500,8 +1517,7 @@ cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap* q_map, const void* q, void
                                    int q_heads, int kv_heads,
                                    const void* cache_layer, int num_blocks, int layer,
                                    const int32_t* block_tables, int bt_pitch,
-                                   const int32_t* seq_bt_row, const int32_t* cu_q,
-                                   const int32_t* seq_lens_k, int S, float scale,
+                                   const int32_t* seq_bt_row, int S, float scale,
                                    const PlanDims& dims, void* ws, int32_t* err, int dev,
                                    cudaStream_t st) {
   static std::atomic<bool> attr_set[64];                  // per device, set on its first call
@@ -1527,8 +1543,6 @@ cudaError_t hy_launch_attn_q4_bf16(const CUtensorMap* q_map, const void* q, void
   a.block_tables = block_tables;
   a.bt_pitch = bt_pitch;
   a.seq_bt_row = seq_bt_row;
-  a.cu_q = cu_q;
-  a.seq_lens_k = seq_lens_k;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = err;
   const dim3 grid(hy_attn_num_sms(dev)), block(NT);

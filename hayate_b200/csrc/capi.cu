@@ -513,8 +513,7 @@ int hy_varlen_attention_q4(int32_t dtype, const void* q, void* out, int32_t num_
   }
   return cuda_result(hy_launch_attn_q4_bf16(decode ? nullptr : &qmap, q, out, num_tokens, q_heads, kv_heads, base,
                                             num_blocks, layer, block_tables, bt_pitch, seq_bt_row,
-                                            cu_seqlens_q, seq_lens_k, num_seqs, scale, d,
-                                            workspace, err, dev, as_stream(stream)),
+                                            num_seqs, scale, d, workspace, err, dev, as_stream(stream)),
                      "hy_varlen_attention_q4(bf16)");
 }
 

@@ -46,7 +46,7 @@ def _dt(t: torch.Tensor) -> int:
 
 def describe_error(word: int) -> str:
     names = [(DEV_BOUNDS, "index out of range"), (DEV_TIMEOUT, "wait timed out"),
-             (DEV_POOL, "KV block pool exhausted"), (DEV_PLAN, "attention plan overflow")]
+             (DEV_POOL, "KV block pool exhausted"), (DEV_PLAN, "attention plan overflow or mismatch")]
     return ", ".join(n for b, n in names if word & b) or "none"
 
 

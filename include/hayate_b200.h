@@ -42,7 +42,7 @@ extern "C" {
 #define HY_DEV_BOUNDS 1       /* device error word bits */
 #define HY_DEV_TIMEOUT 2
 #define HY_DEV_POOL 4
-#define HY_DEV_PLAN 8
+#define HY_DEV_PLAN 8         /* the plan overflows its workspace, or is another batch's */
 
 #define HY_DTYPE_BF16 0
 #define HY_DTYPE_FP32 1
@@ -238,7 +238,12 @@ int hy_varlen_attention_noalloc(const void* q, void* out, int32_t num_tokens, in
  * the pool or a sequence longer than its block-table row ORs HY_DEV_BOUNDS into
  * err, and the sequence's output rows are not meaningful; so does one of fewer
  * keys than query tokens (or of more than 2^28), which the plan refuses with
- * its whole batch: a bf16 call then writes no row.  A NaN in the cache reaches
+ * its whole batch: a bf16 call then writes no row.  A bf16 call takes the
+ * sequences' query rows and key lengths from the plan (fp32: from the arrays);
+ * a workspace without a plan, or with one for another number of sequences,
+ * KV heads or capacities, ORs HY_DEV_PLAN into err and no row is written.  Nor
+ * is any where the sequences have query rows that q does not (cu_seqlens_q past
+ * num_tokens, or negative): HY_DEV_BOUNDS.  A NaN in the cache reaches
  * the query rows that see its key, of its KV head (a value's half row: that
  * half of their outputs), and no others.  bf16 needs the planned workspace;
  * fp32 runs a scalar kernel for parity runs and ignores it.
