@@ -468,14 +468,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(
     v.header[3] = s_bad;
     v.header[4] = group && !bad ? S * kv_heads : 0;   // per-CTA decode: its pair count
     v.header[5] = bad ? 0 : s_cblk;
-    HyQ4Plan& p = *reinterpret_cast<HyQ4Plan*>(v.header + 8);
+    HyPlan& p = *reinterpret_cast<HyPlan*>(v.header + 8);
     p.blocks = v.header[5];
     p.work = v.header[4] > 0 ? -v.header[4] : v.header[0];
     p.seqs = S;
     p.key = v.key;
     plan_sides(bad ? 0 : min(s_cpre, v.max_pre), tiles_all, (long)s_cblk * kv_heads, n_sm, p.pre_ctas, p.shares);
-    p.first_row = cu_q[0];
-    p.end_row = cu_q[S];
+    p.first_row = v.header[6] = cu_q[0];
+    p.end_row = v.header[7] = cu_q[S];
     if (S <= v.max_seqs) v.seqs[S] = make_int4(s_cblk, cu_q[S], 0, 0);
     if (bad) hy_flag(err, s_bad);
   }
@@ -486,7 +486,7 @@ struct MainArgs {
   const __nv_bfloat16* cache;   // the whole cache: tensor-map row r starts at cache + 128 r
   const __nv_bfloat16* q;
   __nv_bfloat16* out;
-  int q_heads, kv_heads;
+  int q_heads, kv_heads, num_tokens;
   int layer;              // layer index (selects the work counters)
   int layer_row_base;     // first tensor-map row of this layer
   int oob_row;            // a row past the end of the map: loads there read zeros
@@ -1368,8 +1368,17 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_main_kernel(
   hy_grid_wait();
   hy_grid_trigger();
   const uint64_t keep = l2_keep_policy();
-  const int n_pre = ld_keep(v.header, keep), n_dec = ld_keep(v.header + 1, keep);
-  const int n_pairs = ld_keep(v.header + 4, keep);    // per-CTA decode when > 0
+  const int4 h0 = ld_keep(reinterpret_cast<const int4*>(v.header), keep);
+  const int4 h1 = ld_keep(reinterpret_cast<const int4*>(v.header + 4), keep);
+  int n_pre = h0.x, n_dec = h0.y;
+  int n_pairs = h1.x;                                 // per-CTA decode when > 0
+  if (h1.z < 0 || h1.w > a.num_tokens) {              // sequences with query rows that q does not have
+    if (threadIdx.x == 0) hy_flag(a.err, HY_ERR_BOUNDS);
+    n_pre = n_dec = n_pairs = 0;
+    if (have_pre)                                     // loads issued early land before the CTA exits
+      for (int s = 0; s < DEC_STAGES; ++s)
+        if ((pre_issued >> s) & 1u) mbar_wait(&sh.dec_bar[warp][s], 0u, nullptr);
+  }
   const bool use_tmem = (int)blockIdx.x < n_pre;      // the first n_pre CTAs take prefill items
   uint32_t dec_phase = 0, tile_ctr = 0;
   bool ok = true;
@@ -1602,7 +1611,7 @@ cudaError_t hy_launch_attn_plan(const int32_t* cu_q, const int32_t* seq_lens_k, 
 }
 
 cudaError_t hy_launch_attn_bf16(const KvMaps& maps, const CUtensorMap& qmap, const void* cache,
-                                const void* q, void* out, int q_heads,
+                                const void* q, void* out, int num_tokens, int q_heads,
                                 int kv_heads, int layer_row_base, int oob_row, int num_blocks,
                                 const int32_t* block_tables, int bt_pitch,
                                 const int32_t* seq_bt_row, const int32_t* cu_q,
@@ -1623,6 +1632,7 @@ cudaError_t hy_launch_attn_bf16(const KvMaps& maps, const CUtensorMap& qmap, con
   a.cache = static_cast<const __nv_bfloat16*>(cache);
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.out = static_cast<__nv_bfloat16*>(out);
+  a.num_tokens = num_tokens;
   a.q_heads = q_heads;
   a.kv_heads = kv_heads;
   a.layer_row_base = layer_row_base;

@@ -37,8 +37,8 @@ struct PlanDims {
 struct PlanView {
   int* header;        // n_pre, n_dec, split, status, (sequence, KV head) pairs of a
                       // per-CTA decode step (0: decode items split over all warps),
-                      // key blocks of all decode sequences; then what the 4-bit cache's
-                      // kernels read, [8]: HyQ4Plan
+                      // key blocks of all decode sequences, first and end query row; [8]:
+                      // HyPlan
   int4* pre;          // prefill items by sequence (plan scratch)
   int4* pre_sorted;   // the same items, most key tiles first (what the kernel runs)
   int4* dec;          // per decode item: (seq, kv head, first block, end block), then
@@ -67,7 +67,7 @@ struct PlanView {
 };
 
 // A plan as the 4-bit cache's kernels take it, two 16-byte loads.
-struct HyQ4Plan {
+struct HyPlan {
   int blocks;         // key blocks of all decode sequences, of one KV head
   int work;           // >= 0: prefill items; < 0: none, and minus the pairs of a per-CTA
                       // decode step
@@ -102,7 +102,7 @@ cudaError_t hy_launch_attn_plan(const int32_t* cu_q, const int32_t* seq_lens_k, 
 // 2 x 2 (one prefill sub-tile's Q, 32 KB, 128-byte swizzle).
 int hy_attention_q_map(const void* q, int num_tokens, int q_heads, CUtensorMap* out);
 cudaError_t hy_launch_attn_bf16(const KvMaps& maps, const CUtensorMap& qmap, const void* cache,
-                                const void* q, void* out, int q_heads,
+                                const void* q, void* out, int num_tokens, int q_heads,
                                 int kv_heads, int layer_row_base, int oob_row, int num_blocks,
                                 const int32_t* block_tables, int bt_pitch,
                                 const int32_t* seq_bt_row, const int32_t* cu_q,

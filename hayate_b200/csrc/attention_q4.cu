@@ -173,7 +173,7 @@ HY_DEVICE SeqInfo seq_info(const Args& a, const PlanView& v, int seq) {
 }
 // The workspace's plan.  One of other sequences or capacities (or none), or of query rows
 // that q does not have, is reported and holds no work.
-HY_DEVICE HyQ4Plan load_plan(const Args& a, const PlanView& v) {
+HY_DEVICE HyPlan load_plan(const Args& a, const PlanView& v) {
   const uint64_t keep = l2_keep_policy();
   const int4 x = ld_keep(reinterpret_cast<const int4*>(v.header + 8), keep);
   const int4 y = ld_keep(reinterpret_cast<const int4*>(v.header + 12), keep);
@@ -181,9 +181,9 @@ HY_DEVICE HyQ4Plan load_plan(const Args& a, const PlanView& v) {
                   : y.z < 0 || y.w > a.num_tokens ? HY_ERR_BOUNDS : 0;
   if (bad) {
     if (threadIdx.x == 0) hy_flag(a.err, bad);
-    return HyQ4Plan{};
+    return HyPlan{};
   }
-  return HyQ4Plan{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  return HyPlan{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 }
 // The search of cursor_at begins with sequences `top_step` apart, one per lane; they are
 // loaded before the kernel knows whether it has decode work.
@@ -1243,7 +1243,7 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(const __grid_constant__ 
   __syncthreads();
   hy_grid_wait();
   hy_grid_trigger();
-  const HyQ4Plan plan = load_plan(a, v);
+  const HyPlan plan = load_plan(a, v);
   if (plan.work <= 0 && plan.blocks == 0) return;         // every CTA: no counter is touched
   int* grab = v.grab + HY_GRAB_INTS * (a.layer & 63);
   bool ok = true;
@@ -1297,7 +1297,7 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_decode_kernel(Args a, PlanView 
   hy_grid_wait();
   hy_grid_trigger();
   const SeqInfo top = seq_top(a, v);                      // with the header: needed by most steps
-  const HyQ4Plan plan = load_plan(a, v);
+  const HyPlan plan = load_plan(a, v);
   int n_pairs = max(-plan.work, 0);
   const int total = plan.blocks * a.kv_heads;             // below 2^31, see decode_shares
   if (n_pairs <= 16 && total > 64 * n_pairs) n_pairs = 0;       // few, not short: dealt after all

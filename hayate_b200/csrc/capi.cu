@@ -457,7 +457,7 @@ int hy_varlen_attention(int32_t dtype, const void* q, void* out, int32_t num_tok
   rc = hy_attention_q_map(q, num_tokens, q_heads, &qmap);
   if (rc) return rc;
   return cuda_result(
-      hy_launch_attn_bf16(map, qmap, kv_cache, q, out, q_heads, kv_heads, (int)(layer * layer_rows), (int)rows,
+      hy_launch_attn_bf16(map, qmap, kv_cache, q, out, num_tokens, q_heads, kv_heads, (int)(layer * layer_rows), (int)rows,
                           num_blocks, block_tables, bt_pitch, seq_bt_row, cu_seqlens_q,
                           seq_lens_k, num_seqs, scale, d, workspace, err, dev, as_stream(stream),
                           flags),

@@ -191,7 +191,9 @@ int hy_attention_plan(const int32_t* cu_seqlens_q, const int32_t* seq_lens_k, in
  * hy_attention_plan for the same workspace.  The first bf16 call after a plan
  * caches each decode item's block-table row and first block ids in the
  * workspace for the later calls: block_tables and seq_bt_row must not change
- * between a plan and the last call that uses it.
+ * between a plan and the last call that uses it.  A bf16 call whose planned
+ * sequences have query rows that q does not (cu_seqlens_q past num_tokens, or
+ * negative) sets HY_DEV_BOUNDS and writes no row.
  * flags: 0, or HY_ATTN_EARLY when the plan, the block tables and the cache
  * (but for the keys and values of this call's query tokens) were written at
  * least two launches before this one on the stream, and the call is not the
