@@ -27,6 +27,7 @@
 #include "q4.cuh"
 
 #include <atomic>
+#include <float.h>
 #include <limits.h>
 #include <math.h>
 
@@ -42,6 +43,22 @@ constexpr int RING_BYTES = NS * STAGE_BYTES;
 constexpr int PART_FLOATS = HY_GROUP * HY_HEAD_DIM + 2 * HY_GROUP;
 constexpr int DEC_SMEM = NW * (RING_BYTES + 2 * PART_FLOATS * 4) + 1024;   // + alignment
 constexpr float RESCALE_LOG2 = 8.0f;                      // see decode_warp
+// A weight is 2^(score mult - m), m the running maximum in log2 units, by one multiply-add.
+// m is rounded to fp32, which scales all weights alike, by next to nothing while |m| is
+// at most this (2^-24 of it is 2^-4).  Past it the factor could leave fp16's range: the
+// threshold above which m is raised is then the largest score itself, without slack, and
+// the weights are 2^((score - threshold) mult), in a branch that ordinary rows never enter.
+constexpr float FAR_LOG2 = 1048576.0f;
+HY_DEVICE float raise_above(float score, float m, float mult) {
+  return fabsf(m) <= FAR_LOG2 ? (m + RESCALE_LOG2) / mult : score;
+}
+// What scores (of a query row scaled by 1 / up) are multiplied with: log2 units.  Not 0 (a
+// scale of 0, a row of tiny elements): masked scores are -inf times it.  Not infinite:
+// where it would be, scores that differ are so far apart that a smaller factor gives the
+// same weights.
+HY_DEVICE float score_mult(float scale_log2, float up) {
+  return fminf(fmaxf(scale_log2 * up, 1e-30f), FLT_MAX);
+}
 
 // Prefill: warps 0-3 / 4-7 softmax of sub-tile 0 / 1, 8-11 expand, 12 / 13 issue the
 // products of sub-tile 0 / 1, 14 deals out items and loads Q.  Sub-tile X, row r: query
@@ -377,9 +394,8 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
       const float2 back = __half22float2(hi);
       const __half2 lo = __floats2half2_rn(sum[0] * 256.f - back.x, sum[1] * 256.f - back.y);
       qs = c == 0 ? q4_as_u32(hi) : c == 1 ? q4_as_u32(lo) : 0u;
-      // not 0 (a scale of 0, a row of tiny elements): masked scores are -inf times it
-      mult[0] = fmaxf(a.scale_log2 * (1024.f * __shfl_sync(0xffffffffu, up, 8 * c)), 1e-30f);
-      mult[1] = fmaxf(a.scale_log2 * (1024.f * __shfl_sync(0xffffffffu, up, 8 * c + 4)), 1e-30f);
+      mult[0] = score_mult(a.scale_log2 * 1024.f, __shfl_sync(0xffffffffu, up, 8 * c));
+      mult[1] = score_mult(a.scale_log2 * 1024.f, __shfl_sync(0xffffffffu, up, 8 * c + 4));
     }
     float o[4][4];                                        // O^T, in 2^-24 / vs (odd m-tiles 2^-20 / vs)
     float z[2][2] = {{0.f, 0.f}, {0.f, 0.f}};             // [half][k]: sum of p times V's minimum
@@ -461,10 +477,10 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], d));
-          const float m_new = fmaxf(m[e], mx[e] * mult[e]);
+          const float m_mx = mx[e] * mult[e], m_new = fmaxf(m[e], m_mx);
           const float alpha = m_new == -INFINITY ? 1.f : ex2_ftz(m[e] - m_new);
+          if (mx[e] > thr[e] || m_mx > m[e]) thr[e] = raise_above(mx[e], m_new, mult[e]);
           m[e] = m_new;
-          thr[e] = (m_new + RESCALE_LOG2) / mult[e];
           l[e] *= alpha;
           z[0][e] *= alpha;
           z[1][e] *= alpha;
@@ -473,7 +489,18 @@ HY_DEVICE bool decode_warp(const Args& a, const PlanView& v, Cursor (&cur)[2], i
           for (int j = 0; j < 4; ++j) { o[j][e] *= ao; o[j][2 + e] *= ao; }
         }
       }
-      const float ms[2] = {m[0] == -INFINITY ? 0.f : -m[0], m[1] == -INFINITY ? 0.f : -m[1]};
+      float ms[2] = {m[0] == -INFINITY ? 0.f : -m[0], m[1] == -INFINITY ? 0.f : -m[1]};
+      if (fmaxf(fabsf(ms[0]), fabsf(ms[1])) > FAR_LOG2) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (fabsf(ms[e]) > FAR_LOG2) {
+            x[0][e] -= thr[e];
+            x[0][2 + e] -= thr[e];
+            x[1][e] -= thr[e];
+            x[1][2 + e] -= thr[e];
+            ms[e] = 0.f;
+          }
+      }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
 #pragma unroll
@@ -1029,7 +1056,6 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
       if (named_sync_or(PRE_PIECE_BAR, PRE_ROWS, !ok)) ok = false;
       if (!ok || P.seq < 0) break;
       const int ntiles = P.thi - P.tlo;
-      const bool real = j < P.nrows;                      // rows past the chunk hold other tokens' Q
       // Q row r to fp16 in place (q4_query_scale)
       float sl2;                                          // scale to log2 units of this row
       {
@@ -1043,9 +1069,7 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
             amax = fmax3f(amax, fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u)));
         }
         q4_query_scale(amax, down, up);
-        // not 0 (a scale of 0, a row of tiny elements): masked scores are -inf times it,
-        // and the scores it multiplies, at most 2^24, stay 0 to fp32 either way
-        sl2 = fmaxf(a.scale_log2 * up, 1e-30f);
+        sl2 = score_mult(a.scale_log2, up);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           uint4* at = reinterpret_cast<uint4*>(q_row + (i >> 3) * (Q_BYTES / 2) + (((i & 7) ^ (r & 7)) << 4));
@@ -1062,8 +1086,9 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.qfull);
       }
-      const int lim = P.prefix + P.t0 + j;                // last key row r may see
+      const int lim = min(P.prefix + P.t0 + j, P.kv_end - 1);   // last key row r may see
       float m = NEG_INF, l = 0.f;                         // m in scaled log2 units
+      float thr = NEG_INF;                                // score above which it is raised
       for (int t = 0; t < ntiles; ++t) {
         const uint32_t c = c0 + t;
         const uint32_t tS = tmem + lane_base + tm_s(X, c & 1);
@@ -1081,7 +1106,7 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
         if (kb + PRE_KEYS - 1 > P.prefix + P.t0) {        // the tile reaches the diagonal or the end
 #pragma unroll
           for (int i = 0; i < 64; ++i)
-            if (kb + i > lim || kb + i >= P.kv_end) s[i] = NEG_INF;
+            if (kb + i > lim) s[i] = NEG_INF;
         }
         float mxs[8];                                     // 8 independent chains
 #pragma unroll
@@ -1092,14 +1117,15 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
           for (int k = 0; k < 8; ++k) mxs[k] = fmax3f(mxs[k], s[i + k], s[i + 8 + k]);
 #pragma unroll
         for (int k = 0; k < 8; ++k) mxs[k] = fmaxf(mxs[k], s[56 + k]);
-        const float mx = sl2 * fmax3f(fmax3f(mxs[0], mxs[1], mxs[2]), fmax3f(mxs[3], mxs[4], mxs[5]),
-                                      fmaxf(mxs[6], mxs[7]));
-        const bool grow = mx > m + RESCALE_LOG2;
+        const float mx = fmax3f(fmax3f(mxs[0], mxs[1], mxs[2]), fmax3f(mxs[3], mxs[4], mxs[5]),
+                                fmaxf(mxs[6], mxs[7]));
+        const bool grow = mx > thr;
         if (__any_sync(0xffffffffu, grow)) {
-          const float mnew = grow ? mx : m;
+          const float mnew = grow ? mx * sl2 : m;
           const float alpha = mnew == NEG_INF ? 1.f : ex2_ftz(m - mnew);
           l *= alpha;
           m = mnew;
+          if (grow) thr = raise_above(mx, m, sl2);
           if (t > 0) {                                    // O holds tiles < t: wait for P V(t - 1)
             ok = __all_sync(0xffffffffu, mbar_wait(&sh.odone[X][(c & 1) ^ 1], ((c - 1) >> 1) & 1, a.err));
             tc_fence_after();
@@ -1115,7 +1141,13 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
             if (!ok) break;
           }
         }
-        const float mneg = (m == NEG_INF) ? 0.f : -m;
+        float mneg = (m == NEG_INF) ? 0.f : -m;
+        if (__any_sync(0xffffffffu, fabsf(mneg) > FAR_LOG2)) {
+          const float off = fabsf(mneg) > FAR_LOG2 ? thr : 0.f;
+#pragma unroll
+          for (int i = 0; i < 64; ++i) s[i] -= off;
+          mneg = fabsf(mneg) > FAR_LOG2 ? 0.f : mneg;
+        }
         const float2 sl2v = make_float2(sl2, sl2), mnegv = make_float2(mneg, mneg);
         uint32_t pk[32];
         float2 ls[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
@@ -1143,11 +1175,15 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
           if (__any_sync(0xffffffffu, sh.nan_at[n & 1][half] <= lim))
             nan_half(tO + 64 * half, sh.nan_at[n & 1][half] <= lim);
       }
-      const bool store = ok && real;
-      __nv_bfloat16* op = a.out + ((size_t)(P.row0 + P.t0 + j) * a.q_heads + P.g * HY_GROUP + 2 * X + (r >> 6)) *
+      // read again rather than held in registers over the tiles: no item takes the place
+      // before these warps have read the next one
+      const PreItem& E = sh.item[n & 1];
+      const bool store = ok && j < E.nrows;               // rows past the chunk hold other tokens' Q
+      __nv_bfloat16* op = a.out + ((size_t)(E.row0 + E.t0 + j) * a.q_heads + E.g * HY_GROUP + 2 * X + (r >> 6)) *
                                       HY_HEAD_DIM;
-      if (P.w != 0) {                                     // a piece: every softmax thread takes part
-        ok = prefill_piece_finish(v, P.w, X * 128 + r, tO, m, l, ok, store ? op : nullptr, sh.pre_last);
+      const int piece = E.w;
+      if (piece != 0) {                                   // a piece: every softmax thread takes part
+        ok = prefill_piece_finish(v, piece, X * 128 + r, tO, m, l, ok, store ? op : nullptr, sh.pre_last);
       } else if (ok) {
         const float inv = 1.f / l;
 #pragma unroll 1
