@@ -473,7 +473,8 @@ int hy_varlen_attention_q4(int32_t dtype, const void* q, void* out, int32_t num_
                            int32_t max_seqs, int32_t max_tokens, void* workspace,
                            size_t workspace_bytes, int32_t* err, void* stream) {
   if (!dtype_ok(dtype)) return fail(HY_E_INVALID, "hy_varlen_attention_q4: dtype must be 0 or 1");
-  if (!q || !out || !kv_cache || !block_tables || !cu_seqlens_q || !seq_lens_k ||
+  const bool none = num_tokens == 0;                   // q and out may be null then
+  if ((!none && (!q || !out)) || !kv_cache || !block_tables || !cu_seqlens_q || !seq_lens_k ||
       num_seqs <= 0 || num_tokens < 0 || num_layers <= 0 || num_blocks <= 0 || layer < 0 ||
       layer >= num_layers || bt_pitch <= 0)
     return fail(HY_E_INVALID, "hy_varlen_attention_q4: bad argument");
@@ -483,7 +484,7 @@ int hy_varlen_attention_q4(int32_t dtype, const void* q, void* out, int32_t num_
     return fail(HY_E_INVALID, "hy_varlen_attention_q4: scale must be finite and not negative");
   if (!aligned16(q) || !aligned16(out) || !aligned16(kv_cache))
     return fail(HY_E_INVALID, "hy_varlen_attention_q4: q, out and the cache must be 16-byte aligned");
-  if (num_tokens == 0) return HY_OK;
+  if (none) return HY_OK;
   const uint8_t* base = static_cast<const uint8_t*>(kv_cache) +
                         (size_t)layer * num_blocks * kv_heads * 2 * HY_Q4_TILE_BYTES;
   if (dtype == HY_DTYPE_FP32)

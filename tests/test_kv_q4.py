@@ -108,3 +108,14 @@ def test_engine_refuses_unknown_cache_types():
     from hayate_b200.model import Runner
     with pytest.raises(ValueError, match="kv_cache_dtype"):
         Runner(TINY, EngineConfig(kv_cache_dtype="fp8"), torch.float32, torch.device("cpu"), None, [])
+
+
+def test_attention_of_no_tokens_is_nothing_to_do():
+    """An empty tensor's address is null."""
+    lib = _lib.load()
+    keep, p = _aligned()
+    for dtype in (0, 1):
+        assert lib.hy_varlen_attention_q4(dtype, None, None, 0, 8, 2, p, 2, 4, 0, p, 4, None, p, p, 1, 0.1, 4, 4,
+                                          None, 0, None, None) == 0
+        assert lib.hy_varlen_attention_q4(dtype, None, None, 0, 8, 2, None, 2, 4, 0, p, 4, None, p, p, 1, 0.1, 4,
+                                          4, None, 0, None, None) == -1

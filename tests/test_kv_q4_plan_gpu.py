@@ -98,3 +98,11 @@ def test_bf16_takes_the_sequences_from_the_plan(q_lens, kv_lens):
         s.check()
         s.kv.copy_(keep[0])
         s.cu.copy_(keep[1])
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+def test_no_tokens(dt):
+    s = Step(Batch([1, 3], [40, 50], 2, dt, seed=6))
+    s.q = s.out = torch.zeros(0, 8, 128, dtype=dt, device=dev)
+    s.attend()
+    assert int(s.err.item()) == 0
