@@ -78,7 +78,7 @@ def plant(b, c, ties):
 @pytest.mark.parametrize("dt,c", [(BF, 1e3), (BF, 1e5), (BF, 1e8), (BF, 1e12), (BF, 1e30), (BF, 1e36), (F32, 1e3),
                                   (F32, 1e8), (F32, 1e30)])
 @pytest.mark.parametrize("lens", [([1, 1, 1], [90, 33, 300]), ([1], [5003]), ([1] * 12, [700 - 9 * i for i in range(12)]),
-                                  ([1, 3, 0, 0], [90, 200, 1, 1]), ([70], [300]), ([128], [4000])])
+                                  ([1, 3, 0, 0], [90, 200, 1, 1]), ([70], [300]), ([24], [4000])])
 def test_the_winning_key_s_value_comes_out(lens, dt, c, ties):
     b = Batch(*lens, 2, dt, seed=42)
     want, size = plant(b, c, ties)

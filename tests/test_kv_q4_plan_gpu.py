@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from hayate_b200 import kernels as K
+from hayate_b200._lib import HayateError
 from test_kv_q4_gpu import BF, F32, Batch, dev, i32
 from test_kv_q4_use_gpu import Step
 
@@ -106,3 +107,23 @@ def test_no_tokens(dt):
     s.q = s.out = torch.zeros(0, 8, 128, dtype=dt, device=dev)
     s.attend()
     assert int(s.err.item()) == 0
+
+
+def test_each_refusal_of_a_workspace_says_why():
+    s = Step(Batch([1, 3], [30, 40], 2, BF, seed=7))
+    need = K.attention_workspace_size(2, 4, 2)
+    room = torch.zeros(need + 512, dtype=torch.uint8, device=dev)
+    assert room.data_ptr() % 256 == 0
+
+    def call(ws, seqs=2, max_seqs=2, max_tokens=4):
+        K.varlen_attention_q4(s.q, s.out, s.cache, 0, s.tables, s.cu, s.kv, seqs, max_seqs, max_tokens, ws, err=s.err)
+
+    s.ws = room[256:]                                    # a slice of its own is as good as any
+    s.plan()
+    call(s.ws)
+    assert int(s.err.item()) == 0
+    for ws, kw, why in ((None, {}, "planned, 256-byte aligned"), (room[16:], {}, "planned, 256-byte aligned"),
+                        (room[:need - 1], {}, "too small"), (room, dict(max_seqs=1), "above the workspace's"),
+                        (room, dict(max_tokens=3), "above the workspace's")):
+        with pytest.raises(HayateError, match=why):
+            call(ws, **kw)
