@@ -235,9 +235,9 @@ HY_DEVICE int mul_div(int a, int b, int c) {
 // be kept apart instead: an item is long (its tiles, 1.3 us each), so the CTAs that the
 // longer side leaves, a share each, should get through the decode work in the time of k
 // whole rounds of items.  Of the rule and k = 1 to 4 the least estimate is taken (8 heads,
-// 512 tokens at 2560 keys beside 128 decodes of 2048: 108 us, 126 by the rule; at 4096
-// beside 256 of 4096: 273, 307; at 512 beside 10 of 600: 20.1, 24.7; steps of more items
-// than CTAs were no faster apart: 4 chunks at 2560 beside 128 of 2048 168, 170).
+// when it was added, 512 tokens at 2560 keys beside 128 decodes of 2048: 108 us, 126 by the
+// rule; at 4096 beside 256 of 4096: 273, 307; at 512 beside 10 of 600: 20.1, 24.7; steps of
+// more items than CTAs were no faster apart: 4 chunks at 2560 beside 128 of 2048 168, 170).
 constexpr int TILE_BLOCKS = 28;                 // key blocks that a CTA gets through in a tile's time
 constexpr int SHARE_BLOCKS = 180;               // and in the time that a share costs by itself
 HY_DEVICE void plan_sides(int n, long tiles, long blocks, int ctas, int& pre_ctas, int& shares) {

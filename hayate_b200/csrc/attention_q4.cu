@@ -12,14 +12,16 @@
 // bytes: K and V of one block and head are adjacent) through a ring of bulk copies and
 // feeds their codes to mma.sync as they are (4 query heads would fill 3 % of a tcgen05
 // tile); warps of a CTA merge what they share in shared memory, CTAs through the
-// workspace.  Bound by the cache's bytes: 256 sequences of 4096 keys take 216 us, 5.6
-// TB/s (of 6.5 for a copy); a launch costs about 9 us beside its blocks, of which the
-// smallest steps consist (one sequence of 600 keys 8.8 us; of 40960 keys 19.8).
+// workspace.  Bound by the cache's bytes: 256 sequences of 4096 keys take 214 to 231 us
+// from box to box, 5.2 to 5.6 TB/s (of 6.5 for a copy); a launch costs about 9 us beside
+// its blocks, of which the smallest steps consist (one sequence of 600 keys 8.85 us; of
+// 40960 keys 19.8).
 // The other kernel adds prefill items (64 query tokens x one KV head, 256 score rows) on
 // tcgen05: four warps expand key tiles to fp16 operands in shared memory, one warp per
 // 128-row sub-tile issues the products, two warpgroups run the softmax.  Bound by the
 // softmax and the products taking turns in a sub-tile (two sub-tiles overlap): 16 chunks
-// of 512 tokens with 4096 keys take 523 us, 985 TFLOP/s (61 % of a large bf16 product).
+// of 512 tokens with 4096 keys take 565 to 593 us back to back, 870 to 910 TFLOP/s (55 % of
+// a large bf16 product's burst rate; the bf16 cache's kernel 618 beside 565).
 // Key tiles of 128, with one S buffer per sub-tile, ran the same in 793 us.
 // fp32 runs a kernel of its own on the fp32 units.
 #include "attention.cuh"
@@ -842,8 +844,9 @@ HY_DEVICE PreItem pre_item_geom(const Args& a, const PlanView& v, int item) {
 // their scores are masked, and a zero weight times a zero adds nothing.  A half of V
 // whose parameters are NaN (its codes are 0 then) is expanded to fp16's lowest number, so
 // that a later token's does not reach the rows that do not see it; its key is noted, and
-// the softmax warps write NaN where a row does see it.  (16 chunks of 512 tokens: 393 us
-// with this, 389 without; zeroing the half in a branch before it is expanded, 402.)
+// the softmax warps write NaN where a row does see it.  (16 chunks of 512 tokens, when it
+// was added: 393 us with this, 389 without; zeroing the half in a branch before it is
+// expanded, 402.)
 constexpr uint32_t VALUE_LEAST = 0xfbff0000u;             // parameters are at least (0, -65504)
 constexpr uint32_t KEY_LEAST = 0x7fff7fffu;               // NaN: whatever they are
 struct RowCodes {
@@ -1213,8 +1216,8 @@ __device__ bool prefill_all(const CUtensorMap* q_map, const Args& a, const PlanV
 
 // The decode sequences of a step with prefill items: their key blocks in even shares that
 // CTAs take as they become free (as many as plan_sides says; a share costs about 8 us
-// beside its blocks: 4 chunks and 128 decodes take 135 us with a share per CTA, 145 with
-// two smaller ones and 154 with three).  Returns false if a wait ran out.
+// beside its blocks: 4 chunks and 128 decodes took 135 us with a share per CTA, 145 with
+// two smaller ones and 154 with three, all on one build).  Returns false if a wait ran out.
 __device__ bool decode_shares(const Args& a, const PlanView& v, int shares, int blocks, uint8_t* payload,
                               Shared& sh) {
   uint32_t ring_pos = 0, ring_par = 0;
@@ -1313,14 +1316,16 @@ __global__ void __launch_bounds__(NT, 1) attn_q4_kernel(const __grid_constant__ 
 }
 
 // Steps of no more query rows than sequences, which are decode steps but for sequences
-// without a token: without the prefill's code a launch takes up to 2 us less (10 sequences
-// of 600 keys 10.0 against 10.3 us, one of 40960 23.3 against 25.3).  The key blocks are dealt
-// evenly over the CTAs; a small step's pairs (the plan's choice) go one to a CTA, which
-// merges them in shared memory, unless there are at most 16 of more than 64 blocks each (8
-// pairs of 64 / 96 / 128 blocks dealt 9.6 / 9.9 / 10.3 us, a CTA each 10.0 / 11.7 / 13.6;
-// 16 of 64 / 128 10.6 / 11.5 and 10.0 / 13.5; 32 of 128 14.9 and 13.6).  Rows of longer
-// chunks that such a step may hold all the same are taken one (row, head) at a time, a CTA
-// each.
+// without a token: without the prefill's code a launch takes 2 us less (one sequence of 600
+// keys 8.9 us, 11.1 by the other kernel, one of 40960 19.9 and 22.3).  The key blocks are
+// dealt evenly over the CTAs; a small step's pairs (the plan's choice) go one to a CTA,
+// which merges them in shared memory, unless there are at most 16, of more than 64 blocks
+// on average over all sequences, those without a token included (8 pairs of 64 / 96 / 128
+// blocks dealt 8.8 / 9.1 / 9.4 us, a CTA each 9.8 / 11.7 / 13.5; 16 of 64 / 128 9.6 / 10.7
+// and 9.8 / 13.5; 32 of 128 13.9 and 13.7; 80 of 38 13.7 and 9.3).  The average overlooks
+// a long sequence beside a short one: 8 pairs of 120 blocks and 8 of 1 take 13.3, 9.1 if
+// dealt.  Rows of longer chunks that such a step may hold all the same are taken one (row,
+// head) at a time, a CTA each.
 __global__ void __launch_bounds__(NT, 1) attn_q4_decode_kernel(Args a, PlanView v) {
   __shared__ Shared sh;
   extern __shared__ uint8_t dyn_smem[];

@@ -7,11 +7,11 @@
 // reference has no quantised one).
 //
 // Bound by memory (a bf16 row moves 256 + 72 bytes: 8192 tokens of 8 heads are written in
-// 11.8 us, 3.6 TB/s, and 40001 tokens read back in 48.6 us, 4.3 TB/s, where filling the
-// outputs alone takes 45.8) as long as the instructions per
-// element stay few: the codes are rounded and collected by additions instead of
-// conversions (which run at a quarter of the rate), read back by masks, and a thread's
-// row of the token is found once, not per row.
+// 11.8 us, 3.6 TB/s, from inputs in HBM, in 9.5 where the call before left them in L2, and
+// 40001 tokens read back in 48.6 us, 4.3 TB/s, where filling the outputs alone takes 45.8)
+// as long as the instructions per element stay few: the codes are rounded and collected by
+// additions instead of conversions (which run at a quarter of the rate), read back by
+// masks, and a thread's row of the token is found once, not per row.
 #include "q4.cuh"
 
 namespace {
@@ -19,8 +19,8 @@ namespace {
 constexpr int Q4_THREADS = 256;
 constexpr int Q4_LANES = HY_HEAD_DIM / 16;            // lanes per row
 constexpr int Q4_ROWS = Q4_THREADS / Q4_LANES;        // rows per CTA pass
-// rows in flight per lane (8192 tokens of 8 heads written / read: 12.7 / 12.5 us with 1,
-// 11.8 / 10.8 with 2, 13.8 / 12.0 with 4)
+// rows in flight per lane (8192 tokens of 8 heads written / read, from HBM: 12.7 / 12.5 us
+// with 1, 11.8 / 10.8 with 2, 13.8 / 12.0 with 4)
 constexpr int Q4_UNROLL = 2;
 
 // min and max that are NaN if either operand is
@@ -156,7 +156,7 @@ HY_DEVICE uint2 quantise16(const Raw16<T>& raw, __half2& par) {
 // Rows of a CTA pass: 8 lanes each, `per` rows of a token (all its 2 kv_heads rows, or
 // 32 at a time), as many tokens as fit.  With more than a pass per CTA, the passes in
 // flight take neighbouring tokens, whose parameters share sectors (8192 tokens of 8
-// heads: write 10.9 -> 9.8 us, read 10.7 -> 9.8); a short call spreads over the CTAs.
+// heads, in L2: write 10.9 -> 9.8 us, read 10.7 -> 9.8); a short call spreads over the CTAs.
 struct RowMap {
   int per, tokens, t, r;                                // this thread's token of the pass and row
   int first, near, stride;                              // the CTA's first token, from pass to pass in

@@ -12,10 +12,13 @@
 // 64 dimensions share a scale: with 32 the parameters would be 16 bytes a row (80
 // bytes instead of 72, and the cache is read at HBM speed), with 128 the step
 // would follow the whole row's range.  The parameters are fp16 (11 significant
-// bits: the minimum's rounding stays below a fiftieth of a step), so rows are
-// clamped to +-Q4_LIMIT as they are written; codes are taken against the rounded
-// parameters, which keeps the reconstruction within half a step of the input (plus
-// the parameters' own rounding at the ends of the range).
+// bits), so rows are clamped to +-Q4_LIMIT as they are written; codes are taken against
+// the rounded parameters, which keeps the reconstruction within half a step of the input
+// but for what their rounding cuts off at the ends of the range: up to 15 steps times
+// 2^-11 at the top, and |minimum| 2^-11 at either end.  Where the range holds 0 the minimum
+// is at most 15 steps, and that is a hundredth of a step; a half row that lies far from 0
+// against its range loses accuracy to it (1000 to 1002: a step of 0.133 and an error of
+// up to 0.25, half of fp16's spacing there).
 #pragma once
 
 #include "common.cuh"
@@ -58,6 +61,9 @@ HY_DEVICE void q4_values(uint32_t w, float scale, float low, float2 (&x)[4]) {
 // halves' nibbles.  A nibble under the exponent of 1024 is the number 1024 + n (in
 // bits 0-3) or 1024 + 16 n (in bits 4-7), from which n follows exactly; the only
 // rounding is the last multiply-add's, to fp16 (2^-11 relative, an eighth of bf16's).
+// The exponent trick for 4-bit codes is a published one: Kim, Henry, Fahim, Awadalla, "Who
+// Says Elephants Can't Run: Bringing Large Scale MoE Models into Cloud Scale Production",
+// 2022.
 HY_DEVICE uint32_t q4_lop_or(uint32_t w, uint32_t mask) {
   uint32_t r;                                   // (w & mask) | 0x64006400
   asm("lop3.b32 %0, %1, %2, 0x64006400, 0xea;" : "=r"(r) : "r"(w), "r"(mask));
