@@ -176,6 +176,10 @@ size_t hy_attention_workspace_size(int32_t max_seqs, int32_t max_tokens, int32_t
 
 /* Split the step's sequences into prefill tiles and decode items; the plan is
  * written into the workspace and reused by every layer's hy_varlen_attention.
+ * A sequence of fewer keys than query tokens, or of more than 2^28 keys, ORs
+ * HY_DEV_BOUNDS into err and leaves a plan without work.  The workspace also
+ * takes the partial results of the calls on the plan: calls that may overlap on
+ * the GPU need workspaces of their own.
  * Replaces: the per-step mask construction, hayate/model/qwen.py:79-106. */
 int hy_attention_plan(const int32_t* cu_seqlens_q, const int32_t* seq_lens_k, int32_t num_seqs,
                       int32_t kv_heads, int32_t max_seqs, int32_t max_tokens, void* workspace,
