@@ -13,7 +13,7 @@
 // feeds their codes to mma.sync as they are (4 query heads would fill 3 % of a tcgen05
 // tile); warps of a CTA merge what they share in shared memory, CTAs through the
 // workspace.  Bound by the cache's bytes: 256 sequences of 4096 keys take 214 to 231 us
-// from box to box, 5.2 to 5.6 TB/s (of 6.5 for a copy); a launch costs about 9 us beside
+// from run to run, 5.2 to 5.6 TB/s (of 6.5 for a copy); a launch costs about 9 us beside
 // its blocks, of which the smallest steps consist (one sequence of 600 keys 8.85 us; of
 // 40960 keys 19.8).
 // The other kernel adds prefill items (64 query tokens x one KV head, 256 score rows) on
